@@ -374,6 +374,97 @@ int lg_attn_decode_noalloc(const float* q, const float* k, const float* v, const
 int lg_swiglu_quant(float* hb, const float* hb2, int n, int qtype, void* out_q, void* stream);
 
 /* ===================================================================== */
+/* Many tokens and long contexts (device pointers, asynchronous)          */
+/* ===================================================================== */
+/* Calls for serving loops that keep the caches of one or many sequences
+ * themselves; no counterpart in the reference, which runs one sequence, one
+ * token at a time, with its whole context visible.  Rows are the tokens of
+ * nseq sequences, ntok each: row s * ntok + t.  pos holds nseq * ntok int32
+ * positions in device memory, in any order; a row whose position is negative
+ * or too large holds no token: its outputs are zeros and it writes no cache.
+ * Positions are read by the kernels, so a captured call follows them at every
+ * replay.  Strides are in floats, from one row to the next; pointers and
+ * strides of fp32 rows are multiples of 16 bytes.  The calling thread's
+ * current device must be the one that owns the pointers and the stream.
+ * Nothing is allocated, and no call keeps state for the next. */
+
+/* A layer's cache of nseq sequences in the caller's device memory, for keys
+ * and values alike:
+ *   LG_F16  [n_ctx][n_kv_heads * head_dim] fp16, as the context's own cache
+ *   LG_KV4  [n_kv_heads][n_ctx][head_dim / 2] bytes of 4-bit codes, then
+ *           [n_kv_heads][n_ctx][head_dim / 32] pairs (d, m) of fp16: each
+ *           group of 32 values of a head's row has a step d and a least value
+ *           m, and code c stands for the fp16 number nearest c * d + m (one
+ *           rounding).  A little-endian 32-bit word holds eight codes: value
+ *           2j in bits 4j..4j+3, value 2j + 1 in bits 16+4j..19+4j.
+ *           head_dim is a multiple of 32.
+ * Sequence s lies at k + s * seq_bytes, v + s * seq_bytes; k, v and seq_bytes
+ * are multiples of 16, seq_bytes at least lg_kv_bytes (any for one sequence). */
+#define LG_KV4 64
+typedef struct {
+    void *k, *v;
+    int32_t type;               /* LG_F16 or LG_KV4 */
+    int32_t n_ctx, n_kv_heads, head_dim;
+    size_t seq_bytes;
+} lg_kv_cache;
+
+/* bytes of one sequence's keys (or values), -1 for a type or shape that no
+ * cache has */
+int64_t lg_kv_bytes(int type, int n_ctx, int n_kv_heads, int head_dim);
+
+/* Rotary frequencies for contexts beyond the trained one (host call): freq
+ * receives rope_dim / 2 floats, freq[i] = base^(-2i / rope_dim) (rope_freq of
+ * fast/common.cpp:38-39) scaled for `factor` times the context:
+ *   LG_ROPE_PLAIN   as trained
+ *   LG_ROPE_LINEAR  every frequency divided by factor
+ *   LG_ROPE_NTK     base times factor^(rope_dim / (rope_dim - 2))
+ *   LG_ROPE_YARN    dims that turn more than p0 times over the trained
+ *                   context (orig_ctx) as trained, those that turn less than
+ *                   p1 times divided by factor, a linear ramp over the dim
+ *                   index between; *mscale = 1 + 0.1 ln(factor) (usual: p0
+ *                   32, p1 1)
+ *   LG_ROPE_BANDS   wavelengths below orig_ctx / p0 as trained, above
+ *                   orig_ctx / p1 divided by factor, between them a blend
+ *                   that is linear in orig_ctx / wavelength (usual: p0 4, p1 1)
+ * *mscale, the factor of cos and sin, is 1 for the others; p0 and p1 are read
+ * by the last two only.  Worked out in double, rounded once. */
+#define LG_ROPE_PLAIN 0
+#define LG_ROPE_LINEAR 1
+#define LG_ROPE_NTK 2
+#define LG_ROPE_YARN 3
+#define LG_ROPE_BANDS 4
+int lg_rope_table(int scaling, int rope_dim, double base, double factor, int orig_ctx, double p0, double p1,
+                  float* freq, float* mscale);
+
+/* Per-head RMSNorm of queries and keys (qw, kw: head_dim floats, NULL to
+ * skip; head_dim even, <= 256), rotation of the first rope_dim values of each
+ * head (even, 0: none) by pos * freq[i], and the cache write of the new rows
+ * -- lg_qk_norm_rope_kv for many tokens.  A pair (a, b) becomes
+ * mscale (a cos - b sin, a sin + b cos); pair i is values 2i, 2i + 1
+ * (LG_ROPE_ADJACENT) or i, i + rope_dim / 2 (LG_ROPE_HALF).  Angles are
+ * worked out in double.  q_out and k_out receive the rotated rows; they may
+ * be q and k themselves (with the same stride), k_out may be NULL when a
+ * cache is given, q and q_out when n_heads is 0.  With a cache (NULL: none)
+ * row pos[r] of each sequence receives k and v, v unchanged; two rows of one
+ * sequence must not have the same position.  LG_KV4 rows: m = fp16(min),
+ * d = fp16(fp32((max - m) / 15)), code = (x - m) / d to the nearest, ties to
+ * even, within 0..15, worked out in double; values beyond +-60000 count as
+ * +-60000, a NaN makes its group's values NaN. */
+#define LG_ROPE_ADJACENT 0
+#define LG_ROPE_HALF 1
+int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q_out, int64_t q_out_stride, const float* k,
+                           int64_t k_stride, float* k_out, int64_t k_out_stride, const float* v, int64_t v_stride,
+                           const float* qw, const float* kw, int n_heads, int n_kv_heads, int head_dim, int rope_dim,
+                           int layout, const float* freq, float mscale, float eps, const int* pos, int nseq, int ntok,
+                           const lg_kv_cache* cache, void* stream);
+
+/* rows [pos0, pos0 + npos) of an LG_KV4 cache as the fp16 values they stand
+ * for: k_out, v_out [nseq][npos][n_kv_heads * head_dim] (lg_state_save's and
+ * lg_kv_write's form of a row) */
+int lg_kv4_read(const lg_kv_cache* cache, int nseq, int pos0, int npos, uint16_t* k_out, uint16_t* v_out,
+                void* stream);
+
+/* ===================================================================== */
 /* BERT sentence embedding and the vector memory (fast/vdb.cpp)           */
 /* ===================================================================== */
 /* The chat driver's retrieval memory embeds every logged user turn and each

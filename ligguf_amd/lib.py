@@ -23,6 +23,9 @@ BLOCK = {F32: (1, 4), F16: (1, 2), Q8_0: (32, 34), Q1_0: (32, 6), Q1_G: (128, 18
 
 ARCH_LLAMA, ARCH_QWEN3 = 0, 1
 PATH_AUTO, PATH_PERSISTENT, PATH_MULTI, PATH_FUSED = 0, 1, 2, 3
+KV4 = 64                                    # a cache in 4 bits (lg_kv_cache)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = 0, 1, 2, 3, 4
+ROPE_ADJACENT, ROPE_HALF = 0, 1
 PREFILL_AUTO, PREFILL_STEPS, PREFILL_BATCHED = 0, 1, 2
 
 _vp = C.c_void_p
@@ -62,6 +65,11 @@ class LgBertDesc(C.Structure):
                 ("n_context", C.c_int32), ("vocab_size", C.c_int32), ("tok_cls", C.c_int32), ("tok_sep", C.c_int32),
                 ("eps", C.c_float), ("tok_embd", LgWeight), ("pos_embd", LgWeight), ("tok_types", LgWeight),
                 ("emb_norm_w", _vp), ("emb_norm_b", _vp), ("layers", _vp)]
+
+
+class LgKvCache(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("type", C.c_int32), ("n_ctx", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("seq_bytes", C.c_size_t)]
 
 
 # Every exported symbol of include/ligguf_hip.h with its ctypes signature.
@@ -110,6 +118,13 @@ SIGNATURES = {
     "lg_attn_scratch_bytes": (C.c_size_t, []),
     "lg_attn_decode_noalloc": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]),
     "lg_swiglu_quant": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp]),
+    "lg_kv_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "lg_rope_table": (C.c_int, [C.c_int, C.c_int, C.c_double, C.c_double, C.c_int, C.c_double, C.c_double, _vp,
+                                C.POINTER(C.c_float)]),
+    "lg_qk_norm_rope_tokens": (C.c_int, [_vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64,
+                                         _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_float,
+                                         C.c_float, _vp, C.c_int, C.c_int, _vp, _vp]),
+    "lg_kv4_read": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]),
     "lg_bert_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "lg_bert_destroy": (C.c_int, [_vp]),
     "lg_bert_last_error": (C.c_char_p, [_vp]),

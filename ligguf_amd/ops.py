@@ -6,9 +6,12 @@ and raises LgError on failure; there is no CPU path.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
-from .lib import BLOCK, F32, Q8_0, Q8_K, check, load
+from . import lib as L
+from .lib import BLOCK, F16, F32, KV4, Q8_0, Q8_K, LgError, check, load
 
 
 def _stream():
@@ -101,5 +104,133 @@ def swiglu_quant(hb: torch.Tensor, hb2: torch.Tensor, qtype: int = Q8_K):
     return q
 
 
+# --------------------------------------------------------------------------
+# many tokens and long contexts
+# --------------------------------------------------------------------------
+def _refuse(msg):
+    raise LgError(f"LG_ERR_ARG: {msg}")
+
+
+def _on(dev, fn, *args):
+    """fn(*args, stream) on dev and its current stream."""
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _rows(t, pos, width, name):
+    """(pointer, floats from row to row) of fp32 rows [nseq, ntok, width]; the
+    last axis is dense and the first two are one run of rows."""
+    if t.dtype != torch.float32 or t.device != pos.device:
+        _refuse(f"{name}: fp32 rows on {pos.device} wanted")
+    if t.shape != (*pos.shape, width):
+        _refuse(f"{name}: shape {tuple(t.shape)}, {(*pos.shape, width)} wanted")
+    s = t.stride()
+    row = s[1] if t.shape[1] > 1 else s[0] if t.shape[0] > 1 else (width + 3) // 4 * 4
+    if (width > 1 and s[2] != 1) or (t.shape[0] > 1 and s[0] != row * t.shape[1]):
+        _refuse(f"{name}: rows of strides {s} are not one run")
+    return t.data_ptr(), row
+
+
+def _pos(pos):
+    if not pos.is_cuda or pos.dtype != torch.int32 or pos.dim() != 2 or not pos.is_contiguous():
+        _refuse("pos: contiguous int32 [nseq, ntok] on the GPU wanted")
+    return pos.data_ptr()
+
+
+def _vec(t, n, like, name):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.device != like.device or not t.is_contiguous() or t.numel() < n:
+        _refuse(f"{name}: {n} contiguous fp32 values on {like.device} wanted")
+    return t.data_ptr()
+
+
+class KvCache:
+    """One layer's keys and values of nseq sequences (lg_kv_cache): F16 tensors
+    [nseq, n_ctx, n_kv_heads * head_dim] -- a context's own cache has that form
+    -- or KV4 bytes [nseq, lg_kv_bytes or more, a multiple of 16 for several sequences]."""
+
+    def __init__(self, k, v, n_kv_heads: int, head_dim: int, type: int = F16, n_ctx: int = None):
+        if n_ctx is None:
+            if type != F16:
+                _refuse("n_ctx is needed for a cache in 4 bits")
+            n_ctx = k.shape[1]
+        need = load().lg_kv_bytes(type, n_ctx, n_kv_heads, head_dim)
+        want = torch.float16 if type == F16 else torch.uint8
+        if need < 0 or (type not in (F16, KV4)):
+            _refuse(f"no cache of type {type}, {n_ctx} rows, {n_kv_heads} heads of {head_dim}")
+        for t in (k, v):
+            if not t.is_cuda or t.device != k.device or t.dtype != want or t.shape != k.shape or not t.is_contiguous():
+                _refuse(f"k and v: contiguous {want} tensors of one shape on one GPU wanted")
+        size = k.numel() // k.shape[0] * k.element_size() if k.dim() > 1 and k.shape[0] else -1
+        if size < need or (type == F16 and size != need):
+            _refuse(f"k and v: {need} bytes a sequence wanted, shape {tuple(k.shape)} given")
+        self.k, self.v, self.type, self.n_ctx, self.nseq = k, v, type, n_ctx, k.shape[0]
+        self.n_kv_heads, self.head_dim, self.device = n_kv_heads, head_dim, k.device
+        self.desc = L.LgKvCache(k.data_ptr(), v.data_ptr(), type, n_ctx, n_kv_heads, head_dim, size)
+
+    @classmethod
+    def empty(cls, type: int, n_ctx: int, n_kv_heads: int, head_dim: int, nseq: int = 1, device="cuda") -> "KvCache":
+        """A cache of zeros."""
+        need = load().lg_kv_bytes(type, n_ctx, n_kv_heads, head_dim)
+        if need < 0 or nseq < 1:
+            _refuse(f"no cache of type {type}, {nseq} x {n_ctx} rows, {n_kv_heads} heads of {head_dim}")
+        shape, dt = ((nseq, n_ctx, n_kv_heads * head_dim), torch.float16) if type == F16 else ((nseq, (need + 15) // 16 * 16), torch.uint8)
+        return cls(*(torch.zeros(shape, dtype=dt, device=device) for _ in range(2)), n_kv_heads, head_dim, type, n_ctx)
+
+
+def rope_table(rope_dim: int, base: float, scaling: int = L.ROPE_PLAIN, factor: float = 1.0, orig_ctx: int = 0, p0: float = 0.0,
+               p1: float = 0.0):
+    """lg_rope_table: (rope_dim / 2 frequencies as a CPU tensor, mscale)."""
+    f = torch.empty(max(rope_dim, 0) // 2, dtype=torch.float32)
+    m = C.c_float()
+    check(load().lg_rope_table(scaling, rope_dim, base, factor, orig_ctx, p0, p1, f.data_ptr(), C.byref(m)))
+    return f, m.value
+
+
+def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None, half: bool = False, qw=None, kw=None,
+                        eps: float = 1e-6, mscale: float = 1.0, cache: KvCache = None, want_k: bool = False, q_out=None,
+                        k_out=None):
+    """lg_qk_norm_rope_tokens on q, k, v [nseq, ntok, heads * head_dim] (views of
+    a fused q | k | v row are fine; q or, without a cache, v may be None) and pos
+    [nseq, ntok]: the rotated queries and keys; keys only with want_k or k_out."""
+    rope_dim = head_dim if rope_dim is None else rope_dim
+    p = _pos(pos)
+    kd = k.shape[-1]
+    qd = 0 if q is None else q.shape[-1]
+    if head_dim < 1 or kd % head_dim or qd % head_dim:
+        _refuse(f"rows of {qd} and {kd} values are no heads of {head_dim}")
+    if k_out is None and want_k:
+        k_out = torch.empty((*pos.shape, kd), dtype=torch.float32, device=pos.device)
+    if q_out is None and q is not None:
+        q_out = torch.empty((*pos.shape, qd), dtype=torch.float32, device=pos.device)
+    if cache is not None and (cache.device != pos.device or cache.nseq != pos.shape[0] or v is None):
+        _refuse(f"cache: values and {pos.shape[0]} sequences on {pos.device} wanted")
+    none = (None, 0)
+    _on(pos.device, load().lg_qk_norm_rope_tokens, *(none if q is None else _rows(q, pos, qd, "q")),
+        *(none if q is None else _rows(q_out, pos, qd, "q_out")), *_rows(k, pos, kd, "k"),
+        *(none if k_out is None else _rows(k_out, pos, kd, "k_out")),
+        *(none if cache is None else _rows(v, pos, kd, "v")), _vec(qw, head_dim, pos, "qw"), _vec(kw, head_dim, pos, "kw"),
+        qd // head_dim, kd // head_dim, head_dim, rope_dim, int(half), _vec(freq, rope_dim // 2, pos, "freq"), mscale, eps, p,
+        *pos.shape, None if cache is None else C.byref(cache.desc))
+    return q_out, k_out
+
+
+def kv_values(cache: KvCache, pos0: int = 0, npos: int = None):
+    """lg_kv4_read: the fp16 values [nseq, npos, kv_dim] that rows pos0 .. of a
+    KV4 cache stand for, keys and values."""
+    npos = cache.n_ctx - pos0 if npos is None else npos
+    if npos < 0:
+        _refuse(f"{npos} rows")
+    k, v = (torch.empty((cache.nseq, npos, cache.n_kv_heads * cache.head_dim), dtype=torch.float16, device=cache.device)
+            for _ in range(2))
+    if npos:
+        _on(cache.device, load().lg_kv4_read, C.byref(cache.desc), cache.nseq, pos0, npos, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
 __all__ = ["dequantize_row", "quantize_q8_0", "quantize_q8_K", "matvec", "rmsnorm_quant", "qk_norm_rope_kv",
-           "attention", "swiglu_quant", "Q8_0", "Q8_K", "F32"]
+           "attention", "swiglu_quant", "KvCache", "rope_table", "qk_norm_rope_tokens", "kv_values", "Q8_0", "Q8_K", "F32", "F16", "KV4"]
