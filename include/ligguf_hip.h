@@ -464,6 +464,44 @@ int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q_out, int64
 int lg_kv4_read(const lg_kv_cache* cache, int nseq, int pos0, int npos, uint16_t* k_out, uint16_t* v_out,
                 void* stream);
 
+/* Attention of nseq x ntok query rows over such a cache (its rows, the rows'
+ * own included, are written before): with p = pos[r],
+ *   out[r] = softmax(q[r] K^T / sqrt(head_dim)) V
+ * over the cache rows j <= p of the row's sequence, with window > 0 only those
+ * with j > p - window or j < sinks (sinks >= 0: first positions that stay
+ * visible).  n_heads is a multiple of the cache's n_kv_heads, query head h
+ * reads head h / (n_heads / n_kv_heads).  head_dim 48 (LG_F16 only), 64, 96,
+ * 128 or 256.  max_pos < n_ctx bounds the positions: a row beyond it counts as
+ * one without a token, and its output is zeros.  A row's result does not
+ * depend on what invisible rows hold, infinities and NaN included; a visible
+ * key or query with one makes the row NaN.
+ * fp32 queries and the softmax's weights enter the products as two fp16
+ * parts, about 22 bits.  workspace: lg_attn_cache_workspace_size bytes of
+ * device memory, 16-byte aligned (NULL when that is 0), which nothing else may
+ * use until the call is done: calls that may overlap, replays of captured
+ * ones included, need one each. */
+size_t lg_attn_cache_workspace_size(int nseq, int ntok, int n_heads, int n_kv_heads, int head_dim, int window,
+                                    int sinks, int max_pos);
+int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache* cache, const int* pos, int nseq, int ntok,
+                  int n_heads, int window, int sinks, int max_pos, float* out, int64_t out_stride, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/* Log probabilities of rows of logits (lg_logits_device is one): for each row
+ * r < rows of vocab floats at logits + r * stride (4-byte aligned),
+ *   logprob[r] = log softmax(row)[toks[r]], NaN where toks[r] is no id
+ *   entropy[r] = -sum p log p (nats; terms of p = 0 count as 0)
+ *   top_id, top_logprob [rows][top]: the entries of highest logits, ties by
+ *                the lower id, NaN above all (0 <= top <= 32, top <= vocab)
+ * toks is device memory.  Each output may be NULL (toks and logprob, top_id
+ * and top_logprob go together).  A row with a NaN or +infinity, or with
+ * nothing above -infinity, has NaN probabilities and entropy.  workspace as
+ * for lg_attn_cache.  No counterpart in the reference. */
+#define LG_LOGPROBS_TOP 32
+size_t lg_logprobs_workspace_size(int rows, int vocab, int top);
+int lg_logprobs(const float* logits, int64_t stride, int rows, int vocab, const int* toks, int top, float* logprob,
+                float* entropy, int* top_id, float* top_logprob, void* workspace, size_t workspace_bytes,
+                void* stream);
+
 /* ===================================================================== */
 /* BERT sentence embedding and the vector memory (fast/vdb.cpp)           */
 /* ===================================================================== */

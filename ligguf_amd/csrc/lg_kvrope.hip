@@ -239,6 +239,8 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
         lg_set_error("%s: head_dim %d, rope_dim %d, layout %d", who, head_dim, rope_dim, layout);
         return LG_ERR_ARG;
     }
+    const int64_t rows = (int64_t)nseq * ntok;
+    if (!rows) return LG_OK;
     if (!(eps >= 0.0f) || !pos || (rope_dim && !freq)) {
         lg_set_error("%s: bad argument", who);
         return LG_ERR_ARG;
@@ -260,13 +262,11 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
             return LG_ERR_ARG;
         }
     }
-    const int64_t rows = (int64_t)nseq * ntok;
     const int waves = n_heads + n_kv_heads * (cache ? 2 : 1), all = (waves + 3) / 4;
     if (rows > INT32_MAX / all) {
         lg_set_error("%s: %lld rows of %d heads are too many for one call", who, (long long)rows, waves);
         return LG_ERR_ARG;
     }
-    if (!rows) return LG_OK;
     const int per = rows >= 1024 ? all : 1, nblk = (all + per - 1) / per;
     if (layout == LG_ROPE_HALF)
         k_rope_tokens<true><<<(unsigned)(rows * nblk), 256, 0, (hipStream_t)stream>>>(a, nblk, per);

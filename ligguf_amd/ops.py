@@ -7,6 +7,7 @@ and raises LgError on failure; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -127,6 +128,8 @@ def _rows(t, pos, width, name):
         _refuse(f"{name}: fp32 rows on {pos.device} wanted")
     if t.shape != (*pos.shape, width):
         _refuse(f"{name}: shape {tuple(t.shape)}, {(*pos.shape, width)} wanted")
+    if not t.numel():
+        return None, (width + 3) // 4 * 4
     s = t.stride()
     row = s[1] if t.shape[1] > 1 else s[0] if t.shape[0] > 1 else (width + 3) // 4 * 4
     if (width > 1 and s[2] != 1) or (t.shape[0] > 1 and s[0] != row * t.shape[1]):
@@ -232,5 +235,67 @@ def kv_values(cache: KvCache, pos0: int = 0, npos: int = None):
     return k, v
 
 
+def _work(need, workspace, dev):
+    """(pointer, bytes) of the workspace of a call, a new one unless given."""
+    if workspace is None:
+        if not need:
+            return None, (None, 0)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        _refuse(f"workspace: contiguous memory on {dev} wanted")
+    return workspace, (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max_pos: int = None, out=None, workspace=None):
+    """lg_attn_cache: q [nseq, ntok, n_heads * head_dim] at pos [nseq, ntok] over
+    the cache rows that each position sees.  max_pos, a bound of the positions
+    (n_ctx - 1 by default), sizes the launch."""
+    p = _pos(pos)
+    if cache.device != pos.device or cache.nseq != pos.shape[0]:
+        _refuse(f"cache: {pos.shape[0]} sequences on {pos.device} wanted")
+    max_pos = cache.n_ctx - 1 if max_pos is None else max_pos
+    width = q.shape[-1]
+    heads = width // cache.head_dim
+    if heads * cache.head_dim != width:
+        _refuse(f"rows of {width} values are no heads of {cache.head_dim}")
+    if out is None:
+        out = torch.empty((*pos.shape, width), dtype=torch.float32, device=pos.device)
+    lib = load()
+    need = lib.lg_attn_cache_workspace_size(*pos.shape, heads, cache.n_kv_heads, cache.head_dim, window, sinks, max_pos)
+    workspace, ws = _work(need, workspace, pos.device)
+    _on(pos.device, lib.lg_attn_cache, *_rows(q, pos, width, "q"), C.byref(cache.desc), p, *pos.shape, heads, window, sinks,
+        max_pos, *_rows(out, pos, width, "out"), *ws)
+    return out
+
+
+class Logprobs(NamedTuple):
+    logprob: torch.Tensor        # [rows], None without tokens
+    entropy: torch.Tensor        # [rows]
+    top_id: torch.Tensor         # [rows, top], None for top 0
+    top_logprob: torch.Tensor
+
+
+def logprobs(logits, toks=None, top: int = 0, workspace=None) -> Logprobs:
+    """lg_logprobs of logits [rows, vocab] (dense rows) and int32 toks [rows]."""
+    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        _refuse("logits: dense fp32 rows on the GPU wanted")
+    dev, (rows, vocab) = logits.device, logits.shape
+    if toks is not None and (toks.device != dev or toks.dtype != torch.int32 or toks.shape != (rows,) or not toks.is_contiguous()):
+        _refuse(f"toks: {rows} contiguous int32 on {dev} wanted")
+    if top < 0:
+        _refuse(f"top {top}")
+
+    def new(*shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device=dev)
+    r = Logprobs(new(rows) if toks is not None else None, new(rows), new(rows, top, dtype=torch.int32) if top else None,
+                 new(rows, top) if top else None)
+    lib = load()
+    workspace, ws = _work(lib.lg_logprobs_workspace_size(rows, vocab, top), workspace, dev)
+    _on(dev, lib.lg_logprobs, logits.data_ptr(), max(logits.stride(0), vocab) if rows < 2 else logits.stride(0), rows, vocab,
+        None if toks is None else toks.data_ptr(), top, *(None if t is None else t.data_ptr() for t in r), *ws)
+    return r
+
+
 __all__ = ["dequantize_row", "quantize_q8_0", "quantize_q8_K", "matvec", "rmsnorm_quant", "qk_norm_rope_kv",
-           "attention", "swiglu_quant", "KvCache", "rope_table", "qk_norm_rope_tokens", "kv_values", "Q8_0", "Q8_K", "F32", "F16", "KV4"]
+           "attention", "swiglu_quant", "KvCache", "rope_table", "qk_norm_rope_tokens", "kv_values",
+           "attention_cache", "Logprobs", "logprobs", "Q8_0", "Q8_K", "F32", "F16", "KV4"]

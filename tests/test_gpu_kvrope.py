@@ -252,6 +252,18 @@ def test_other_stream(gpu):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_no_rows(gpu):
+    import torch
+    from ligguf_amd import ops
+    for shape in ((0, 3), (2, 0)):
+        x, pos = torch.zeros(*shape, 128, device=gpu), torch.zeros(shape, dtype=torch.int32, device=gpu)
+        q, k = ops.qk_norm_rope_tokens(x, x, None, pos, torch.zeros(32, device=gpu), 64, want_k=True)
+        assert q.shape == k.shape == x.shape
+    cache = ops.KvCache.empty(ops.F16, 4, 2, 64, 2, gpu)
+    pos = torch.zeros(2, 0, dtype=torch.int32, device=gpu)
+    assert ops.attention_cache(torch.zeros(2, 0, 128, device=gpu), cache, pos).shape == (2, 0, 128)
+
+
 def test_python_refusals(gpu):
     import torch
     from ligguf_amd import ops
