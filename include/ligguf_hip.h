@@ -389,7 +389,7 @@ int lg_swiglu_quant(float* hb, const float* hb2, int n, int qtype, void* out_q, 
  * Nothing is allocated, and no call keeps state for the next. */
 
 /* A layer's cache of nseq sequences in the caller's device memory, for keys
- * and values alike:
+ * and values alike, n_ctx <= 2^30 rows:
  *   LG_F16  [n_ctx][n_kv_heads * head_dim] fp16, as the context's own cache
  *   LG_KV4  [n_kv_heads][n_ctx][head_dim / 2] bytes of 4-bit codes, then
  *           [n_kv_heads][n_ctx][head_dim / 32] pairs (d, m) of fp16: each

@@ -8,7 +8,7 @@
 
 extern "C" int64_t lg_kv_bytes(int type, int n_ctx, int n_kv_heads, int head_dim)
 {
-    if (n_ctx <= 0 || n_kv_heads <= 0 || head_dim <= 0 || head_dim > 256) return -1;
+    if (n_ctx <= 0 || n_ctx > 1 << 30 || n_kv_heads <= 0 || head_dim <= 0 || head_dim > 256) return -1;
     const int64_t n = (int64_t)n_ctx * n_kv_heads;   /* < 2^62; times 512 checked below */
     if (n > ((int64_t)1 << 50)) return -1;
     if (type == LG_F16) return n * head_dim * 2;

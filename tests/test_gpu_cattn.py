@@ -292,3 +292,20 @@ def test_python_refusals(gpu):
                 dict(out=q[:, :2]), dict(out=torch.zeros(2, 3, 258, device=gpu)[..., 1:257])):
         with pytest.raises(L.LgError):
             ops.attention_cache(**{**dict(q=q, cache=cache, pos=pos), **bad})
+
+
+def test_workspace_must_hold_the_partials(gpu):
+    import torch
+    from ligguf_amd import ops
+    lib = L.load()
+    cache = ops.KvCache.empty(ops.F16, 9000, 2, 64, 1, gpu)
+    q, pos = torch.zeros(1, 1, 256, device=gpu), torch.full((1, 1), 8999, dtype=torch.int32, device=gpu)
+    need = lib.lg_attn_cache_workspace_size(1, 1, 4, 2, 64, 0, 0, 8999)
+    assert need > 0
+    ops.attention_cache(q, cache, pos, workspace=torch.empty(need, dtype=torch.uint8, device=gpu))
+    for ws in (torch.empty(need - 1, dtype=torch.uint8, device=gpu), torch.empty(need + 8, dtype=torch.uint8, device=gpu)[8:]):
+        with pytest.raises(L.LgError):
+            ops.attention_cache(q, cache, pos, workspace=ws)
+    c = C.c_void_p
+    assert lib.lg_attn_cache(c(q.data_ptr()), 256, C.byref(cache.desc), c(pos.data_ptr()), 1, 1, 4, 0, 0, 8999,
+                             c(q.data_ptr()), 256, None, 0, None) == -1

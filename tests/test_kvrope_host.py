@@ -21,6 +21,7 @@ def test_cache_bytes():
     assert b(L.F16, 100, 8, 128) == 100 * 8 * 128 * 2
     assert b(L.KV4, 100, 8, 128) == 100 * 8 * (64 + 16)
     assert b(L.KV4, 100, 8, 48) == -1          # no groups of 32
+    assert b(L.F16, (1 << 30) + 1, 1, 64) == -1
     assert b(L.F16, 1 << 30, 8, 128) == (1 << 30) * 2048     # past 32 bits
     for bad in [(L.F32, 1, 1, 64), (L.F16, 0, 1, 64), (L.F16, 1, 0, 64), (L.F16, 1, 1, 0), (L.F16, 1, 1, 257), (99, 1, 1, 64)]:
         assert b(*bad) == -1
