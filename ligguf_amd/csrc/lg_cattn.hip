@@ -162,7 +162,7 @@ struct CaRows {
 };
 
 template <int HD, bool KV4>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_cattn_dec(CAttn a, int nsplit, float* __restrict__ part)
+__global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a, int nsplit, float* __restrict__ part)
 {
     using C = CaDec<HD, KV4>;
     constexpr int KT = C::KT, NU = C::NU, NB = C::NB, NS = C::NS, NT = C::NT;
@@ -363,6 +363,262 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_cattn_dec(CAttn a, i
     }
 }
 
+/* Prompts: 32 columns (query heads of a key head, tokens in order) a wave, NW
+ * waves a workgroup, which share tiles of KT keys in LDS; both products on
+ * 32 x 32 x 16 fp16 MFMA with the operands of k_cattn_dec: lane l feeds row /
+ * column l % 32, k = 8 (l / 32) .. +7, register i of a result is row 8 (i / 4)
+ * + 4 (l / 32) + i % 4 of column l % 32, so registers 8s .. 8s+7 of the scores
+ * are the lane's k of step s of the second product: keys 16s + 4h .. and
+ * 16s + 8 + 4h .. of lane half h.  The next tile is on its way while one
+ * computes (two LDS stages, one barrier a tile). */
+template <int HD, bool KV4>
+struct CaTile {
+    static constexpr int NW = HD <= 128 ? 8 : 4, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;
+    static constexpr int NJ = HD / 16, NT = (HD + 31) / 32;
+    static constexpr int KST = HD + 8;                       /* halves per K row in LDS */
+    static constexpr int VST = NT * 32 + 32;                 /* and per V row: rows 64 bytes on */
+    static constexpr int PW = KV4 ? 16 : 8;                  /* values of a piece that a thread moves */
+    static constexpr int PR = HD / PW, NP = (KT * PR + NTH - 1) / NTH;   /* pieces of a row; of a tile per thread */
+    static constexpr int STAGE = KT * (KST + VST);           /* halves */
+};
+
+template <int HD, bool KV4>
+struct CaPieces {
+    using C = CaTile<HD, KV4>;
+    v4u h[KV4 ? 1 : C::NP];
+    uint2 w[KV4 ? C::NP : 1];
+    uint32_t dm[KV4 ? C::NP : 1];
+
+    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb)
+    {
+#pragma unroll
+        for (int u = 0; u < C::NP; u++) {
+            const int i = min((int)threadIdx.x + u * C::NTH, C::KT * C::PR - 1);
+            const int key = min(kb + i / C::PR, a.max_pos), x = i % C::PR;   /* (rows past it are never visible) */
+            if constexpr (KV4) {
+                w[u] = *(const uint2*)(base + lg_kv4_codes(a.c, g, key) + 8 * x);
+                dm[u] = *(const uint32_t*)(base + lg_kv4_dm(a.c, g, key) + x / 2 * 4);
+            } else
+                h[u] = *(const v4u*)(base + lg_kv16_at(a.c, g, key) + 16 * x);
+        }
+    }
+    /* into rows of ST halves; with `bad`, infinities and NaN as 0 and their keys noted */
+    template <int ST>
+    __device__ __forceinline__ void store(_Float16* dst, uint32_t* bad) const
+    {
+#pragma unroll
+        for (int u = 0; u < C::NP; u++) {
+            const int i = threadIdx.x + u * C::NTH;
+            if ((C::KT * C::PR) % C::NTH == 0 || i < C::KT * C::PR) {
+                _Float16* const q = dst + i / C::PR * ST + i % C::PR * C::PW;
+                v4u x[C::PW / 8];
+                if constexpr (KV4) {
+                    lg_kv4_values(w[u].x, dm[u], (lg_h2*)&x[0]);
+                    lg_kv4_values(w[u].y, dm[u], (lg_h2*)&x[1]);
+                } else
+                    x[0] = h[u];
+                if (bad) {
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < C::PW / 8; e++) any |= ca_drop_bad(x[e]);
+                    if (any) atomicOr(bad + i / C::PR / 32, 1u << (i / C::PR % 32));
+                }
+#pragma unroll
+                for (int e = 0; e < C::PW / 8; e++) *(v4u*)(q + 8 * e) = x[e];
+            }
+        }
+    }
+};
+
+template <int HD, bool KV4>
+__global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void k_cattn_tile(CAttn a, int ncb, int nsplit,
+                                                                                        float* __restrict__ part)
+{
+    using C = CaTile<HD, KV4>;
+    constexpr int KT = C::KT, NK = C::NK, NJ = C::NJ, NT = C::NT;
+    __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
+    __shared__ int s_pos[2 * C::NW];
+    __shared__ uint32_t s_bad[3][2];
+    /* key head fastest; the last columns, which may see most, first */
+    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv;
+    const int seq = blockIdx.x / n_kv % (a.rows / a.ntok), rest = blockIdx.x / n_kv / (a.rows / a.ntok);
+    const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int ncol = a.ntok * a.nrep, idx = cb * 32 * C::NW + 32 * wave + col;
+    const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
+    const int64_t row = (int64_t)seq * a.ntok + tok;
+    int p = a.pos[row];
+    if (idx >= ncol || p > a.max_pos) p = -1;
+    int wmin = p < 0 ? INT32_MAX : p, wmax = p;   /* of the wave */
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        wmin = min(wmin, __shfl_xor(wmin, o));
+        wmax = max(wmax, __shfl_xor(wmax, o));
+    }
+    if (lane == 0) {
+        s_pos[2 * wave] = wmin;
+        s_pos[2 * wave + 1] = wmax;
+    }
+    if (threadIdx.x < 6) s_bad[threadIdx.x / 2][threadIdx.x % 2] = 0;
+    __syncthreads();
+    wmin = __builtin_amdgcn_readfirstlane(wmin);
+    wmax = __builtin_amdgcn_readfirstlane(wmax);
+    int pmin = INT32_MAX, pmax = -1;              /* of the workgroup */
+#pragma unroll
+    for (int w = 0; w < C::NW; w++) {
+        pmin = min(pmin, s_pos[2 * w]);
+        pmax = max(pmax, s_pos[2 * w + 1]);
+    }
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
+
+    typedef float v16f __attribute__((ext_vector_type(16)));
+    v16f o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) o[t] = (v16f){};
+    float l = 0.0f, mx = -INFINITY;
+    if (pmax >= 0) {
+        const CaTiles tiles(a, pmin, pmax, KT);
+        const int t0 = (int)((int64_t)tiles.n * sp / nsplit), t1 = (int)((int64_t)tiles.n * (sp + 1) / nsplit);
+        const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
+        const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
+        /* tiles with keys that some row of the workgroup (wave) does not see */
+        auto partly = [&](int kb, int lo, int hi) {
+            return kb + KT - 1 > lo || (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
+        };
+        CaPieces<HD, KV4> P;
+        v8h qh[NJ], ql[NJ];
+        float sc;
+        {
+            float x[NJ][8], big = 0.0f;
+            const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * h;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const v4f y = idx < ncol ? *(const v4f*)(q + 16 * j + e) : (v4f){};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        x[j][e + i] = y[i];
+                        big = fmaxf(big, fabsf(y[i]));
+                    }
+                }
+            big = fmaxf(big, lg_partner<5>(big));
+            const int ex = __builtin_amdgcn_frexp_expf(big);
+            sc = ldexpf(a.scale2, ex - 14);
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) ca_split2(ldexpf(x[j][e], 14 - ex), ldexpf(x[j][e + 1], 14 - ex), qh[j], ql[j], e);
+        }
+        float m = -0x1p40f, cc = __builtin_fmaf(-m, sc, 14.0f);
+        for (int it = t0 - 1; it < t1; it++) {
+            const bool more = it + 1 < t1;
+            const int kb = tiles.at(max(it, t0)) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
+            const int cur = (it - t0) & 1, nxt = cur ^ 1, slot = (it - t0 + 3) % 3;
+            _Float16* const sK = s_kv + cur * C::STAGE;
+            _Float16* const sV = sK + KT * C::KST;
+            _Float16* const nK = s_kv + nxt * C::STAGE;
+            const bool on = it >= t0 && kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
+            if (more) P.load(a, kc, g, kn);
+            v16f s[NK];
+            if (on) {
+#pragma unroll
+                for (int n = 0; n < NK; n++) s[n] = (v16f){};
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int n = 0; n < NK; n++) {
+                        const v8h k = *(const v8h*)(sK + (32 * n + col) * C::KST + 16 * j + 8 * h);
+                        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[j], s[n], 0, 0, 0);
+                        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[j], s[n], 0, 0, 0);
+                    }
+            }
+            if (more) {
+                P.template store<C::KST>(nK, nullptr);
+                P.load(a, vc, g, kn);
+            }
+            if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
+            if (on) {
+                if (partly(kb, wmin, wmax)) {
+#pragma unroll
+                    for (int n = 0; n < NK; n++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (!ca_sees(a, p, kb + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3))) s[n][i] = -INFINITY;
+                }
+                float mn = s[0][0];
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) mn = fmaxf(mn, s[n][i]);
+                if (__builtin_amdgcn_ballot_w64(mn > m)) {
+                    mn = fmaxf(mn, lg_partner<5>(mn));
+                    mn = fmaxf(mn, m);
+                    const float cn = __builtin_fmaf(-mn, sc, 14.0f), al = __builtin_amdgcn_exp2f(cn - cc);
+                    m = mn;
+                    cc = cn;
+                    l *= al;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) o[t] *= al;
+                }
+#pragma unroll
+                for (int st = 0; st < 2 * NK; st++) {
+                    float w[8];
+                    v8h ph, pl;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st / 2][8 * (st & 1) + i], sc, cc));
+                    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) ca_split2(w[i], w[i + 1], ph, pl, i);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const _Float16* const v = sV + (16 * st + 4 * h + (lane & 15) / 4) * C::VST + 32 * t + (lane & 16) + 4 * (lane & 3);
+                        const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 8 * C::VST);
+                        const v8h x = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph, o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl, o[t], 0, 0, 0);
+                    }
+                }
+                /* infinities and NaN of keys that only some rows see: added by
+                 * itself to those that do, whatever the (positive) weight */
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+                    for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][n]); keys; keys &= keys - 1) {
+                        const int key = kb + 32 * n + __builtin_ctz(keys);
+                        if (ca_sees(a, p, key))
+#pragma unroll
+                            for (int t = 0; t < NT; t++)
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    const int d = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+                                    const float x = HD % 32 == 0 || d < HD ? ca_value(a.c, vc, g, key, d) : 0.0f;
+                                    if (!(fabsf(x) <= FLT_MAX)) o[t][i] += x;
+                                }
+                    }
+            }
+            if (more) P.template store<C::VST>(nK + KT * C::KST, partly(kn, pmin, pmax) ? s_bad[(slot + 1) % 3] : nullptr);
+            __syncthreads();
+        }
+        l += lg_partner<5>(l);
+        mx = l == 0.0f ? -INFINITY : m * sc;
+    }
+    if (idx >= ncol) return;
+    const int64_t at = ((int64_t)sp * a.rows + row) * a.n_heads + head;
+    float* const dst = part ? part + at * HD : a.out + row * a.os + (size_t)head * HD;
+    const float f = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * t + 2 * i + 4 * h;
+            const v4f y = {o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
+            if (HD % 32 == 0 || d < HD) *(v4f*)(dst + d) = p < 0 ? (v4f){} : y * f;
+        }
+    if (part && h == 0) *(float2*)(part + (int64_t)nsplit * a.rows * a.n_heads * HD + 2 * at) = make_float2(mx, l);
+}
+
 /* the splits' parts of a row's head: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M);
  * a thread per four dims */
 __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const float* __restrict__ part)
@@ -393,6 +649,7 @@ __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const 
 /* How a call is cut, from its sizes alone. */
 struct CaPlan {
     bool dec;     /* up to 16 columns a key head */
+    int ncb;      /* else: blocks of columns of a sequence's key head */
     int nsplit;
     size_t ws;
 };
@@ -403,82 +660,18 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
     const int64_t cols = ntok * (n_heads / n_kv);
     p.dec = cols <= 16;
     p.nsplit = 1;
-    if (p.dec) {
-        int64_t keys = (int64_t)max_pos + 1;
-        if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
+    int64_t keys = (int64_t)max_pos + 1;
+    if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
+    if (!p.dec) {
+        const int64_t width = hd <= 128 ? 256 : 128;
+        p.ncb = (int)((cols + width - 1) / width);
+        p.nsplit = (int)std::max<int64_t>(1, std::min(256 / (nseq * n_kv * p.ncb), keys / 512));
+    } else {
         /* two workgroups a CU, each with at least a tile for each wave */
         p.nsplit = (int)std::max<int64_t>(1, std::min(512 / (nseq * n_kv), (keys + 255) / 256));
     }
     if (p.nsplit > 1) p.ws = (size_t)p.nsplit * nseq * ntok * n_heads * (hd + 2) * sizeof(float);
     return p;
-}
-
-/* One wave per row and head: 64 keys a step, one a lane, their scores from
- * whole cache rows, a running maximum and sum, then each visible key's value
- * row times its weight with the dims over the lanes. */
-__global__ __launch_bounds__(256) void k_cattn_row(CAttn a)
-{
-    __shared__ __attribute__((aligned(16))) float s_q[4][256];
-    __shared__ float s_p[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = a.c.hd;
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    if (item >= (int64_t)a.rows * a.n_heads) return;
-    const int row = (int)(item / a.n_heads), head = (int)(item % a.n_heads), g = head / a.nrep;
-    const int p = a.pos[row];
-    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -FLT_MAX, l = 0.0f;
-    for (int d = lane; d < hd; d += 64) s_q[wave][d] = a.q[row * a.qs + head * hd + d] * a.scale2;
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const size_t seq = (size_t)(row / a.ntok) * a.c.seq;
-    if (p >= 0 && p <= a.max_pos) {
-        const int lo = a.window > 0 ? max(0, p - a.window + 1) / 64 : 0;
-        const int first = min((min(a.sinks, p + 1) + 63) / 64, lo);
-        for (int i = 0; i < first + p / 64 - lo + 1; i++) {
-            const int kb = 64 * (i < first ? i : lo + i - first), key = kb + lane;
-            const bool vis = ca_sees(a, p, key);
-            float s = -INFINITY;
-            if (vis) {
-                s = 0.0f;
-                for (int d = 0; d < hd; d += 8) {
-                    lg_h2 k[4];
-                    if (a.c.type == LG_F16) *(uint4*)k = *(const uint4*)(a.c.k + seq + lg_kv16_at(a.c, g, key) + 2 * d);
-                    else
-                        lg_kv4_values(*(const uint32_t*)(a.c.k + seq + lg_kv4_codes(a.c, g, key) + d / 2),
-                                      *(const uint32_t*)(a.c.k + seq + lg_kv4_dm(a.c, g, key) + d / 32 * 4), k);
-                    for (int e = 0; e < 4; e++)
-                        s = __builtin_fmaf(s_q[wave][d + 2 * e], (float)k[e][0], __builtin_fmaf(s_q[wave][d + 2 * e + 1], (float)k[e][1], s));
-                }
-            }
-            const float mn = fmaxf(m, lg_group_max<64>(s)), w = vis ? exp2f(s - mn) : 0.0f, al = exp2f(m - mn);
-            m = mn;
-            l = __builtin_fmaf(l, al, lg_group_sum<64>(w));
-            for (int e = 0; e < 4; e++) o[e] *= al;
-            s_p[wave][lane] = w;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            for (uint64_t bits = __builtin_amdgcn_ballot_w64(vis); bits; bits &= bits - 1) {
-                const int j = __builtin_ctzll(bits);
-                const float w1 = s_p[wave][j];
-                for (int e = 0, d = lane; d < hd; e++, d += 64) {
-                    float v;
-                    if (a.c.type == LG_F16) v = lg_h2f(*(const uint16_t*)(a.c.v + seq + lg_kv16_at(a.c, g, kb + j) + 2 * d));
-                    else {
-                        lg_h2 x[4];
-                        lg_kv4_values(*(const uint32_t*)(a.c.v + seq + lg_kv4_codes(a.c, g, kb + j) + d / 8 * 4),
-                                      *(const uint32_t*)(a.c.v + seq + lg_kv4_dm(a.c, g, kb + j) + d / 32 * 4), x);
-                        const lg_h2 y = d & 4 ? (d & 2 ? x[3] : x[2]) : (d & 2 ? x[1] : x[0]);
-                        v = (float)(d & 1 ? y[1] : y[0]);
-                    }
-                    o[e] = __builtin_fmaf(w1, v, o[e]);
-                }
-            }
-            __builtin_amdgcn_wave_barrier();
-        }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   /* (no visible key) */
-    for (int e = 0, d = lane; d < hd; e++, d += 64) a.out[row * a.os + head * hd + d] = o[e] * inv;
 }
 
 extern "C" size_t lg_attn_cache_workspace_size(int nseq, int ntok, int n_heads, int n_kv_heads, int head_dim, int window,
@@ -488,16 +681,22 @@ extern "C" size_t lg_attn_cache_workspace_size(int nseq, int ntok, int n_heads, 
     return ca_plan(nseq, ntok, n_heads, n_kv_heads, head_dim, window, sinks, max_pos).ws;
 }
 
-template <int HD>
-static void ca_dec(const CAttn& a, const CaPlan& p, int nseq, float* part, hipStream_t s)
+template <int HD, bool KV4>
+static void ca_launch(const CAttn& a, const CaPlan& p, int nseq, float* part, hipStream_t s)
 {
-    const unsigned n = (unsigned)((int64_t)nseq * a.c.n_kv * p.nsplit);
+    const int64_t n = (int64_t)nseq * a.c.n_kv * p.nsplit;
+    if (p.dec)
+        k_cattn_dec<HD, KV4><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, part);
+    else
+        k_cattn_tile<HD, KV4><<<(unsigned)(n * p.ncb), CaTile<HD, KV4>::NTH, 0, s>>>(a, p.ncb, p.nsplit, part);
+}
+
+template <int HD>
+static void ca_type(const CAttn& a, const CaPlan& p, int nseq, float* part, hipStream_t s)
+{
     if constexpr (HD != 48)
-        if (a.c.type == LG_KV4) {
-            k_cattn_dec<HD, true><<<n, 256, 0, s>>>(a, p.nsplit, part);
-            return;
-        }
-    k_cattn_dec<HD, false><<<n, 256, 0, s>>>(a, p.nsplit, part);
+        if (a.c.type == LG_KV4) return ca_launch<HD, true>(a, p, nseq, part, s);
+    ca_launch<HD, false>(a, p, nseq, part, s);
 }
 
 extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache* cache, const int* pos, int nseq,
@@ -545,15 +744,13 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     }
     hipStream_t s = (hipStream_t)stream;
     float* const part = p.ws ? (float*)workspace : nullptr;
-    if (p.dec) switch (hd) {
-        case 48: ca_dec<48>(a, p, nseq, part, s); break;
-        case 64: ca_dec<64>(a, p, nseq, part, s); break;
-        case 96: ca_dec<96>(a, p, nseq, part, s); break;
-        case 128: ca_dec<128>(a, p, nseq, part, s); break;
-        default: ca_dec<256>(a, p, nseq, part, s); break;
-        }
-    else
-        k_cattn_row<<<(unsigned)((rows * n_heads + 3) / 4), 256, 0, s>>>(a);
+    switch (hd) {
+    case 48: ca_type<48>(a, p, nseq, part, s); break;
+    case 64: ca_type<64>(a, p, nseq, part, s); break;
+    case 96: ca_type<96>(a, p, nseq, part, s); break;
+    case 128: ca_type<128>(a, p, nseq, part, s); break;
+    default: ca_type<256>(a, p, nseq, part, s); break;
+    }
     if (part) k_cattn_merge<<<(unsigned)((rows * n_heads * (hd / 4) + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
     return lg_check_launch(who);
 }
