@@ -108,37 +108,49 @@ def swiglu_quant(hb: torch.Tensor, hb2: torch.Tensor, qtype: int = Q8_K):
 # --------------------------------------------------------------------------
 # many tokens and long contexts
 # --------------------------------------------------------------------------
+# A serving loop makes these calls once per layer and token: each costs the host a few
+# microseconds beside the launches themselves, so the checks below read a tensor's fields once.
+_FP32, _INT32 = torch.float32, torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream(i).cuda_stream without the Stream object
+
+
 def _refuse(msg):
     raise LgError(f"LG_ERR_ARG: {msg}")
 
 
-def _on(dev, fn, *args):
-    """fn(*args, stream) on dev and its current stream."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+def _on(i, fn, *args):
+    """fn(*args, stream) on device i and its current stream."""
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        check(rc)
 
 
 def _rows(t, pos, width, name):
     """(pointer, floats from row to row) of fp32 rows [nseq, ntok, width]; the
     last axis is dense and the first two are one run of rows."""
-    if t.dtype != torch.float32 or t.device != pos.device:
-        _refuse(f"{name}: fp32 rows on {pos.device} wanted")
-    if t.shape != (*pos.shape, width):
-        _refuse(f"{name}: shape {tuple(t.shape)}, {(*pos.shape, width)} wanted")
+    nseq, ntok = pos.shape
+    if t.dtype is not _FP32 or t.device != pos.device or t.shape != (nseq, ntok, width):
+        _refuse(f"{name}: fp32 [{nseq}, {ntok}, {width}] on {pos.device} wanted, {t.dtype} {tuple(t.shape)} on {t.device} given")
+    s0, s1, s2 = t.stride()
+    if ntok > 1:
+        row = s1
+    elif nseq > 1:
+        row = s0
+    else:
+        row = (width + 3) // 4 * 4
     if not t.numel():
         return None, (width + 3) // 4 * 4
-    s = t.stride()
-    row = s[1] if t.shape[1] > 1 else s[0] if t.shape[0] > 1 else (width + 3) // 4 * 4
-    if (width > 1 and s[2] != 1) or (t.shape[0] > 1 and s[0] != row * t.shape[1]):
-        _refuse(f"{name}: rows of strides {s} are not one run")
+    if (s2 != 1 and width > 1) or (nseq > 1 and s0 != row * ntok):
+        _refuse(f"{name}: rows of strides {t.stride()} are not one run")
     return t.data_ptr(), row
 
 
 def _pos(pos):
-    if not pos.is_cuda or pos.dtype != torch.int32 or pos.dim() != 2 or not pos.is_contiguous():
+    if pos.dtype is not _INT32 or not pos.is_cuda or pos.dim() != 2 or not pos.is_contiguous():
         _refuse("pos: contiguous int32 [nseq, ntok] on the GPU wanted")
     return pos.data_ptr()
 
@@ -146,7 +158,7 @@ def _pos(pos):
 def _vec(t, n, like, name):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.device != like.device or not t.is_contiguous() or t.numel() < n:
+    if t.dtype is not _FP32 or t.device != like.device or not t.is_contiguous() or t.numel() < n:
         _refuse(f"{name}: {n} contiguous fp32 values on {like.device} wanted")
     return t.data_ptr()
 
@@ -158,21 +170,23 @@ class KvCache:
 
     def __init__(self, k, v, n_kv_heads: int, head_dim: int, type: int = F16, n_ctx: int = None):
         if n_ctx is None:
-            if type != F16:
-                _refuse("n_ctx is needed for a cache in 4 bits")
+            if type != F16 or k.dim() != 3:
+                _refuse("n_ctx is needed for a cache that is not fp16 [nseq, n_ctx, kv_dim]")
             n_ctx = k.shape[1]
         need = load().lg_kv_bytes(type, n_ctx, n_kv_heads, head_dim)
-        want = torch.float16 if type == F16 else torch.uint8
-        if need < 0 or (type not in (F16, KV4)):
+        if need < 0:
             _refuse(f"no cache of type {type}, {n_ctx} rows, {n_kv_heads} heads of {head_dim}")
-        for t in (k, v):
-            if not t.is_cuda or t.device != k.device or t.dtype != want or t.shape != k.shape or not t.is_contiguous():
-                _refuse(f"k and v: contiguous {want} tensors of one shape on one GPU wanted")
-        size = k.numel() // k.shape[0] * k.element_size() if k.dim() > 1 and k.shape[0] else -1
+        want = torch.float16 if type == F16 else torch.uint8
+        dev, shape = k.device, k.shape
+        if (k.dtype is not want or v.dtype is not want or not k.is_cuda or v.device != dev or v.shape != shape or not k.is_contiguous()
+                or not v.is_contiguous()):
+            _refuse(f"k and v: contiguous {want} tensors of one shape on one GPU wanted")
+        nseq = shape[0] if len(shape) > 1 else 0
+        size = k.nbytes // nseq if nseq else -1
         if size < need or (type == F16 and size != need):
-            _refuse(f"k and v: {need} bytes a sequence wanted, shape {tuple(k.shape)} given")
-        self.k, self.v, self.type, self.n_ctx, self.nseq = k, v, type, n_ctx, k.shape[0]
-        self.n_kv_heads, self.head_dim, self.device = n_kv_heads, head_dim, k.device
+            _refuse(f"k and v: {need} bytes a sequence wanted, shape {tuple(shape)} given")
+        self.k, self.v, self.type, self.n_ctx, self.nseq = k, v, type, n_ctx, nseq
+        self.n_kv_heads, self.head_dim, self.device = n_kv_heads, head_dim, dev
         self.desc = L.LgKvCache(k.data_ptr(), v.data_ptr(), type, n_ctx, n_kv_heads, head_dim, size)
 
     @classmethod
@@ -201,24 +215,25 @@ def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None,
     a fused q | k | v row are fine; q or, without a cache, v may be None) and pos
     [nseq, ntok]: the rotated queries and keys; keys only with want_k or k_out."""
     rope_dim = head_dim if rope_dim is None else rope_dim
-    p = _pos(pos)
+    p, dev = _pos(pos), pos.device
+    nseq, ntok = pos.shape
     kd = k.shape[-1]
     qd = 0 if q is None else q.shape[-1]
     if head_dim < 1 or kd % head_dim or qd % head_dim:
         _refuse(f"rows of {qd} and {kd} values are no heads of {head_dim}")
     if k_out is None and want_k:
-        k_out = torch.empty((*pos.shape, kd), dtype=torch.float32, device=pos.device)
+        k_out = k.new_empty((nseq, ntok, kd))
     if q_out is None and q is not None:
-        q_out = torch.empty((*pos.shape, qd), dtype=torch.float32, device=pos.device)
-    if cache is not None and (cache.device != pos.device or cache.nseq != pos.shape[0] or v is None):
-        _refuse(f"cache: values and {pos.shape[0]} sequences on {pos.device} wanted")
+        q_out = q.new_empty((nseq, ntok, qd))
+    if cache is not None and (cache.device != dev or cache.nseq != nseq or v is None):
+        _refuse(f"cache: values and {nseq} sequences on {dev} wanted")
     none = (None, 0)
-    _on(pos.device, load().lg_qk_norm_rope_tokens, *(none if q is None else _rows(q, pos, qd, "q")),
+    _on(dev.index, load().lg_qk_norm_rope_tokens, *(none if q is None else _rows(q, pos, qd, "q")),
         *(none if q is None else _rows(q_out, pos, qd, "q_out")), *_rows(k, pos, kd, "k"),
         *(none if k_out is None else _rows(k_out, pos, kd, "k_out")),
         *(none if cache is None else _rows(v, pos, kd, "v")), _vec(qw, head_dim, pos, "qw"), _vec(kw, head_dim, pos, "kw"),
         qd // head_dim, kd // head_dim, head_dim, rope_dim, int(half), _vec(freq, rope_dim // 2, pos, "freq"), mscale, eps, p,
-        *pos.shape, None if cache is None else C.byref(cache.desc))
+        nseq, ntok, None if cache is None else C.byref(cache.desc))
     return q_out, k_out
 
 
@@ -228,10 +243,11 @@ def kv_values(cache: KvCache, pos0: int = 0, npos: int = None):
     npos = cache.n_ctx - pos0 if npos is None else npos
     if npos < 0:
         _refuse(f"{npos} rows")
-    k, v = (torch.empty((cache.nseq, npos, cache.n_kv_heads * cache.head_dim), dtype=torch.float16, device=cache.device)
-            for _ in range(2))
+    shape = (cache.nseq, npos, cache.n_kv_heads * cache.head_dim)
+    k = torch.empty(shape, dtype=torch.float16, device=cache.device)
+    v = torch.empty_like(k)
     if npos:
-        _on(cache.device, load().lg_kv4_read, C.byref(cache.desc), cache.nseq, pos0, npos, k.data_ptr(), v.data_ptr())
+        _on(cache.device.index, load().lg_kv4_read, C.byref(cache.desc), cache.nseq, pos0, npos, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -250,21 +266,23 @@ def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max
     """lg_attn_cache: q [nseq, ntok, n_heads * head_dim] at pos [nseq, ntok] over
     the cache rows that each position sees.  max_pos, a bound of the positions
     (n_ctx - 1 by default), sizes the launch."""
-    p = _pos(pos)
-    if cache.device != pos.device or cache.nseq != pos.shape[0]:
-        _refuse(f"cache: {pos.shape[0]} sequences on {pos.device} wanted")
+    p, dev = _pos(pos), pos.device
+    nseq, ntok = pos.shape
+    if cache.device != dev or cache.nseq != nseq:
+        _refuse(f"cache: {nseq} sequences on {dev} wanted")
     max_pos = cache.n_ctx - 1 if max_pos is None else max_pos
-    width = q.shape[-1]
-    heads = width // cache.head_dim
-    if heads * cache.head_dim != width:
-        _refuse(f"rows of {width} values are no heads of {cache.head_dim}")
+    width, hd = q.shape[-1], cache.head_dim
+    heads = width // hd
+    if heads * hd != width:
+        _refuse(f"rows of {width} values are no heads of {hd}")
+    rows = _rows(q, pos, width, "q")
     if out is None:
-        out = torch.empty((*pos.shape, width), dtype=torch.float32, device=pos.device)
+        out = q.new_empty((nseq, ntok, width))
     lib = load()
-    need = lib.lg_attn_cache_workspace_size(*pos.shape, heads, cache.n_kv_heads, cache.head_dim, window, sinks, max_pos)
-    workspace, ws = _work(need, workspace, pos.device)
-    _on(pos.device, lib.lg_attn_cache, *_rows(q, pos, width, "q"), C.byref(cache.desc), p, *pos.shape, heads, window, sinks,
-        max_pos, *_rows(out, pos, width, "out"), *ws)
+    workspace, ws = _work(lib.lg_attn_cache_workspace_size(nseq, ntok, heads, cache.n_kv_heads, hd, window, sinks, max_pos), workspace,
+                          dev)
+    _on(dev.index, lib.lg_attn_cache, *rows, C.byref(cache.desc), p, nseq, ntok, heads, window, sinks, max_pos,
+        *_rows(out, pos, width, "out"), *ws)
     return out
 
 
@@ -277,23 +295,23 @@ class Logprobs(NamedTuple):
 
 def logprobs(logits, toks=None, top: int = 0, workspace=None) -> Logprobs:
     """lg_logprobs of logits [rows, vocab] (dense rows) and int32 toks [rows]."""
-    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    if logits.dtype is not _FP32 or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         _refuse("logits: dense fp32 rows on the GPU wanted")
     dev, (rows, vocab) = logits.device, logits.shape
-    if toks is not None and (toks.device != dev or toks.dtype != torch.int32 or toks.shape != (rows,) or not toks.is_contiguous()):
+    if toks is not None and (toks.dtype is not _INT32 or toks.device != dev or toks.shape != (rows,) or not toks.is_contiguous()):
         _refuse(f"toks: {rows} contiguous int32 on {dev} wanted")
     if top < 0:
         _refuse(f"top {top}")
-
-    def new(*shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=dev)
-    r = Logprobs(new(rows) if toks is not None else None, new(rows), new(rows, top, dtype=torch.int32) if top else None,
-                 new(rows, top) if top else None)
+    entropy = logits.new_empty((rows,))
+    lp = None if toks is None else logits.new_empty((rows,))
+    top_lp = logits.new_empty((rows, top)) if top else None
+    top_id = torch.empty_like(top_lp, dtype=_INT32) if top else None
     lib = load()
     workspace, ws = _work(lib.lg_logprobs_workspace_size(rows, vocab, top), workspace, dev)
-    _on(dev, lib.lg_logprobs, logits.data_ptr(), max(logits.stride(0), vocab) if rows < 2 else logits.stride(0), rows, vocab,
-        None if toks is None else toks.data_ptr(), top, *(None if t is None else t.data_ptr() for t in r), *ws)
-    return r
+    _on(dev.index, lib.lg_logprobs, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
+        None if toks is None else toks.data_ptr(), top, None if toks is None else lp.data_ptr(), entropy.data_ptr(),
+        top_id.data_ptr() if top else None, top_lp.data_ptr() if top else None, *ws)
+    return Logprobs(lp, entropy, top_id, top_lp)
 
 
 __all__ = ["dequantize_row", "quantize_q8_0", "quantize_q8_K", "matvec", "rmsnorm_quant", "qk_norm_rope_kv",
