@@ -7,6 +7,9 @@
 #include <algorithm>
 
 #include "lg_kv.h"
+#ifndef CA_W
+#define CA_W 2
+#endif
 
 struct CAttn {
     const float* q;
@@ -23,6 +26,7 @@ __device__ __forceinline__ bool ca_sees(const CAttn& a, int p, int key)
     return key <= p && (a.window <= 0 || key > p - a.window || key < a.sinks);
 }
 
+typedef float lg_f2 __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -32,11 +36,12 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
  * fp16(x - hi); the products of both with fp16 values are exact in fp32 */
 __device__ __forceinline__ void ca_split2(float x0, float x1, v8h& hi, v8h& lo, int i)
 {
-    const lg_h2 x = {(_Float16)x0, (_Float16)x1};
+    const lg_h2 x = __builtin_convertvector(((lg_f2){x0, x1}), lg_h2);
+    const lg_h2 y = __builtin_convertvector(((lg_f2){__builtin_fmaf((float)x[0], -1.0f, x0), __builtin_fmaf((float)x[1], -1.0f, x1)}), lg_h2);
     hi[i] = x[0];
     hi[i + 1] = x[1];
-    lo[i] = (_Float16)(x0 - (float)x[0]);
-    lo[i + 1] = (_Float16)(x1 - (float)x[1]);
+    lo[i] = y[0];
+    lo[i + 1] = y[1];
 }
 
 /* the wave's LDS writes before its other lanes' reads */
@@ -68,16 +73,27 @@ __device__ __forceinline__ bool ca_drop_bad(v4u& w)
     return any != 0;
 }
 
-/* one value of a cached value row */
-__device__ __forceinline__ float ca_value(const LgKv& c, const uint8_t* v, int g, int key, int d)
+/* a mask of lanes as one of their rows l % 16 */
+__device__ __forceinline__ uint64_t ca_row16(uint64_t b) { return (b | b >> 16 | b >> 32 | b >> 48) & 0xFFFF; }
+
+/* four values of a cached value row, from dim d (a multiple of 4) on */
+__device__ __forceinline__ v4f ca_values(const LgKv& c, const uint8_t* v, int g, int key, int d)
 {
-    if (c.type == LG_F16) return lg_h2f(*(const uint16_t*)(v + lg_kv16_at(c, g, key) + 2 * d));
     lg_h2 x[4];
-    lg_kv4_values(*(const uint32_t*)(v + lg_kv4_codes(c, g, key) + d / 8 * 4),
-                  *(const uint32_t*)(v + lg_kv4_dm(c, g, key) + d / 32 * 4), x);
-    const lg_h2 y = d & 4 ? (d & 2 ? x[3] : x[2]) : (d & 2 ? x[1] : x[0]);
-    return (float)(d & 1 ? y[1] : y[0]);
+    if (c.type == LG_F16) *(uint2*)x = *(const uint2*)(v + lg_kv16_at(c, g, key) + 2 * d);
+    else {
+        lg_kv4_values(*(const uint32_t*)(v + lg_kv4_codes(c, g, key) + d / 8 * 4),
+                      *(const uint32_t*)(v + lg_kv4_dm(c, g, key) + d / 32 * 4), x);
+        if (d & 4) {
+            x[0] = x[2];
+            x[1] = x[3];
+        }
+    }
+    return (v4f){(float)x[0][0], (float)x[0][1], (float)x[1][0], (float)x[1][1]};
 }
+
+/* o plus those of x that are infinite or NaN */
+__device__ __forceinline__ float ca_add_bad(float o, float x) { return fabsf(x) <= FLT_MAX ? o : o + x; }
 
 /* The keys that rows of positions pmin .. pmax may see, in tiles of KT: those
  * that hold sinks, then those of the windows (one run where they meet). */
@@ -87,10 +103,24 @@ struct CaTiles {
     {
         lo = a.window > 0 ? max(0, pmin - a.window + 1) / kt : 0;
         first = min((min(a.sinks, pmax + 1) + kt - 1) / kt, lo);
-        n = first + pmax / kt - lo + 1;
+        n = pmax < 0 ? 0 : first + pmax / kt - lo + 1;
+    }
+    /* split sp's run of them: `chunk` tiles or, where that leaves some, equal parts */
+    __device__ __forceinline__ void chunk(int sp, int nsplit, int chunk, int* t0, int* t1) const
+    {
+        const int64_t len = max(chunk, (n + nsplit - 1) / nsplit);
+        *t0 = (int)min(sp * len, (int64_t)n);
+        *t1 = (int)min(*t0 + len, (int64_t)n);
     }
     __device__ __forceinline__ int at(int i) const { return i < first ? i : lo + i - first; }
 };
+
+/* Partials of a split call: [split][row][head] sums, then (maximum, sum of
+ * weights) of each; a part without keys has weight 0 and no sums. */
+__device__ __forceinline__ float2& ca_part_ml(const CAttn& a, int nsplit, float* part, int hd, int64_t at)
+{
+    return ((float2*)(part + (int64_t)nsplit * a.rows * a.n_heads * hd))[at];
+}
 
 /* One token's query heads of a key head, or a few tokens' (up to 16 columns):
  * split over the keys, every wave with tiles of KT keys of its own.
@@ -129,20 +159,22 @@ struct CaRows {
     v4u h[KV4 ? 1 : C::NU][KV4 ? 1 : C::NS];
     uint32_t w[KV4 ? C::NU : 1][KV4 ? C::NS : 1], dm[KV4 ? C::NU : 1][C::ND];
 
-    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb, int r, int c)
+    /* the tile's address is the wave's, a lane's part of it fits 32 bits (rows of at most 2^25 bytes); at: the lane's rows in the tile */
+    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb, const uint32_t at[C::NU], int c)
     {
+        const uint8_t* const p0 = base + (KV4 ? lg_kv4_codes(a.c, g, kb) : lg_kv16_at(a.c, g, kb));
+        const uint8_t* const q0 = base + (KV4 ? lg_kv4_dm(a.c, g, kb) : 0);
 #pragma unroll
         for (int u = 0; u < C::NU; u++) {
-            const int key = min(kb + 16 * u + r, a.max_pos);   /* (rows past it are never visible) */
             if constexpr (KV4) {
-                const uint8_t* const p = base + lg_kv4_codes(a.c, g, key) + (C::RUN ? c * (HD / 8) : 4 * c);
+                const uint8_t* const p = p0 + at[u] * (uint32_t)(HD / 2) + (C::RUN ? c * (HD / 8) : 4 * c);
 #pragma unroll
                 for (int s = 0; s < C::NS; s++) w[u][s] = *(const uint32_t*)(p + s * (C::RUN ? 4 : 16));
-                const uint8_t* const q = base + lg_kv4_dm(a.c, g, key) + (HD == 96 ? 0 : HD == 64 ? c / 2 * 4 : c * C::ND * 4);
+                const uint8_t* const q = q0 + at[u] * (uint32_t)(HD / 8) + (HD == 96 ? 0 : HD == 64 ? c / 2 * 4 : c * C::ND * 4);
 #pragma unroll
                 for (int i = 0; i < C::ND; i++) dm[u][i] = *(const uint32_t*)(q + 4 * i);
             } else {
-                const uint8_t* const p = base + lg_kv16_at(a.c, g, key) + 16 * c;
+                const uint8_t* const p = p0 + at[u] * (uint32_t)(a.c.n_kv * HD * 2) + 16 * c;
 #pragma unroll
                 for (int s = 0; s < C::NS; s++)
                     h[u][s] = HD % 32 == 0 || 32 * s + 8 * c < HD ? *(const v4u*)(p + 64 * s) : (v4u){};
@@ -161,19 +193,32 @@ struct CaRows {
     }
 };
 
-template <int HD, bool KV4>
-__global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a, int nsplit, float* __restrict__ part)
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? CA_W : 1)) void k_cattn_dec(CAttn a, int nsplit, int chunk,
+                                                                           float* __restrict__ part)
 {
     using C = CaDec<HD, KV4>;
     constexpr int KT = C::KT, NU = C::NU, NB = C::NB, NS = C::NS, NT = C::NT;
-    __shared__ __attribute__((aligned(16))) uint8_t s_raw[4 * C::WAVE];
-    __shared__ float s_ml[4][16][2];
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * C::WAVE];
+    __shared__ float s_ml[NW][16][2];
     const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, sp = blockIdx.x / n_kv % nsplit, seq = blockIdx.x / n_kv / nsplit;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, c = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, c = lane >> 4;
     const int tok = col / a.nrep, ncol = a.ntok * a.nrep;
     const int64_t row = (int64_t)seq * a.ntok + min(tok, a.ntok - 1);
     const int head = g * a.nrep + col % a.nrep;
     int p = a.pos[row];
+    /* the column's query, on its way before the first keys: loads come back in order */
+    v4f x[2 * NS];
+    {
+        const float* const q = a.q + row * a.qs + (size_t)head * HD;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const int d = C::dim(s, c);
+            const bool in = col < ncol && d < HD;
+            x[2 * s] = in ? *(const v4f*)(q + d) : (v4f){};
+            x[2 * s + 1] = in ? *(const v4f*)(q + d + 4) : (v4f){};
+        }
+    }
     if (col >= ncol || p > a.max_pos) p = -1;
     int pmin = p < 0 ? INT32_MAX : p, pmax = p;
 #pragma unroll
@@ -184,54 +229,61 @@ __global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a,
     pmin = __builtin_amdgcn_readfirstlane(pmin);
     pmax = __builtin_amdgcn_readfirstlane(pmax);
 
+    const CaTiles tiles(a, pmin, pmax, KT);
+    int t0, t1;
+    tiles.chunk(sp, nsplit, chunk, &t0, &t1);
+    if (part && t0 >= t1) {   /* (workgroup-uniform) */
+        if ((int)threadIdx.x < ncol)
+            ca_part_ml(a, nsplit, part, HD, ((int64_t)sp * a.rows + (int64_t)seq * a.ntok + threadIdx.x / a.nrep) * a.n_heads +
+                                               g * a.nrep + threadIdx.x % a.nrep) = make_float2(-INFINITY, 0.0f);
+        return;
+    }
     v4f o[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) o[t] = (v4f){};
     float l = 0.0f, mx = -INFINITY;   /* the column's maximum in units of a power of two; l over this lane's keys */
-    if (pmax >= 0) {
-        const CaTiles tiles(a, pmin, pmax, KT);
-        const int t0 = (int)((int64_t)tiles.n * sp / nsplit), t1 = (int)((int64_t)tiles.n * (sp + 1) / nsplit);
+    if (t0 + wave < t1) {
         const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
         const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
         _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
         CaRows<HD, KV4> K, V;
-        int it = t0 + wave;
-        if (it < t1) {
-            K.load(a, kc, g, tiles.at(it) * KT, col, c);
-            V.load(a, vc, g, tiles.at(it) * KT, col, c);
-        }
-        /* the column's query in two parts */
-        v8h qh[NS], ql[NS];
-        float sc;
-        {
-            float x[NS][8], big = 0.0f;
-            const float* const q = a.q + row * a.qs + (size_t)head * HD;
+        uint32_t at[NU];
+        /* keys that some column does not see (wave-uniform) */
+        auto partly = [&](int kb) { return kb + KT - 1 > pmin || (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks); };
+        /* the lane's rows of the tile at kb.  Those that none of the columns at
+         * one position sees give way to one that they do, so that whatever
+         * they hold takes no part; where positions differ, see `bad` below. */
+        auto rows_of = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const int d = C::dim(s, c);
-                const bool in = col < ncol && d < HD;
+            for (int u = 0; u < NU; u++) at[u] = min(16 * u + col, a.max_pos - kb);
+            if (pmin == pmax && partly(kb)) {
+                const int some = kb < a.sinks || a.window <= 0 ? 0 : max(0, pmax - a.window + 1 - kb);
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const v4f y = in ? *(const v4f*)(q + d + e) : (v4f){};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        x[s][e + i] = y[i];
-                        big = fmaxf(big, fabsf(y[i]));
-                    }
-                }
+                for (int u = 0; u < NU; u++)
+                    if (!ca_sees(a, pmax, kb + 16 * u + col)) at[u] = some;
             }
-            big = fmaxf(big, lg_partner<4>(big));
-            big = fmaxf(big, lg_partner<5>(big));
-            const int ex = __builtin_amdgcn_frexp_expf(big);   /* big < 2^ex */
-            sc = ldexpf(a.scale2, ex - 14);
+        };
+        int it = t0 + wave, kb = tiles.at(it) * KT;
+        rows_of(kb);
+        K.load(a, kc, g, kb, at, c);
+        V.load(a, vc, g, kb, at, c);
+        /* the query in two parts, while the first keys come */
+        v8h qh[NS], ql[NS];
+        float big = 0.0f;
 #pragma unroll
-            for (int s = 0; s < NS; s++)
+        for (int i = 0; i < 2 * NS; i++)
+            big = fmaxf(fmaxf(big, fmaxf(fabsf(x[i][0]), fabsf(x[i][1]))), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
+        big = fmaxf(big, lg_partner<4>(big));
+        big = fmaxf(big, lg_partner<5>(big));
+        const int ex = __builtin_amdgcn_frexp_expf(big);   /* big < 2^ex */
+        const float sc = ldexpf(a.scale2, ex - 14);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) ca_split2(ldexpf(x[s][e], 14 - ex), ldexpf(x[s][e + 1], 14 - ex), qh[s], ql[s], e);
-        }
+        for (int j = 0; j < NS; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j], ql[j], e);
         float m = -0x1p40f, cc = __builtin_fmaf(-m, sc, 14.0f);   /* below any score; cc: 14 less the maximum */
-        for (; it < t1; it += 4) {
-            const int kb = tiles.at(it) * KT;
+        for (; it < t1; it += NW) {
             v4f s[NU];
 #pragma unroll
             for (int u = 0; u < NU; u++) {
@@ -243,10 +295,12 @@ __global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a,
                     s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], s[u], 0, 0, 0);
                 }
             }
-            const int kn = it + 4 < t1 ? tiles.at(it + 4) * KT : -1;
-            if (kn >= 0) K.load(a, kc, g, kn, col, c);
-            /* keys that some column does not see (wave-uniform) */
-            const bool part_seen = kb + KT - 1 > pmin || (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks);
+            const int kn = it + NW < t1 ? tiles.at(it + NW) * KT : -1;
+            if (kn >= 0) {
+                rows_of(kn);
+                K.load(a, kc, g, kn, at, c);
+            }
+            const bool part_seen = partly(kb);
             if (part_seen) {
 #pragma unroll
                 for (int u = 0; u < NU; u++)
@@ -270,18 +324,19 @@ __global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a,
 #pragma unroll
                 for (int t = 0; t < NT; t++) o[t] *= al;
             }
+            uint64_t bad = 0;   /* keys of the tile */
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                uint64_t bad[2] = {};
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < NS; j++) {
-                        v4u x = V.get(2 * b + u, j);
-                        if (part_seen) bad[u] |= __builtin_amdgcn_ballot_w64(ca_drop_bad(x));
-                        if (HD % 32 == 0 || C::dim(j, c) < HD) *(v4u*)(sV + (16 * u + col) * C::VST + C::dim(j, c)) = x;
+                        v4u y = V.get(2 * b + u, j);
+                        if (part_seen && pmin != pmax)
+                            bad |= ca_row16(__builtin_amdgcn_ballot_w64(ca_drop_bad(y))) << (32 * b + 16 * u);
+                        if (HD % 32 == 0 || C::dim(j, c) < HD) *(v4u*)(sV + (16 * u + col) * C::VST + C::dim(j, c)) = y;
                     }
-                if (b == NB - 1 && kn >= 0) V.load(a, vc, g, kn, col, c);
+                if (b == NB - 1 && kn >= 0) V.load(a, vc, g, kn, at, c);
                 v8h ph, pl;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -297,34 +352,31 @@ __global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a,
                 for (int t = 0; t < NT; t++) {
                     const _Float16* const v = sV + (4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
                     const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
-                    const v8h x = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph, o[t], 0, 0, 0);
-                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl, o[t], 0, 0, 0);
+                    const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
                 }
                 ca_wave_sync();   /* (the reads before the next block's writes) */
-                /* infinities and NaN of keys that only some columns see: added
-                 * by itself to those that do, whatever the (positive) weight */
+            }
+            /* infinities and NaN of keys that only some columns see: added by
+             * itself to those that do, whatever the (positive) weight */
+            for (; bad; bad &= bad - 1) {
+                const int key = kb + __builtin_ctzll(bad);
+                if (ca_sees(a, p, key))
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-                    for (uint32_t keys = (uint32_t)(bad[u] | bad[u] >> 16 | bad[u] >> 32 | bad[u] >> 48) & 0xFFFFu; keys;
-                         keys &= keys - 1) {
-                        const int key = kb + 32 * b + 16 * u + __builtin_ctz(keys);
-                        if (ca_sees(a, p, key))
+                    for (int t = 0; t < NT; t++) {
+                        const v4f y = ca_values(a.c, vc, g, key, 16 * t + 4 * c);
 #pragma unroll
-                            for (int t = 0; t < NT; t++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const float x = ca_value(a.c, vc, g, key, 16 * t + 4 * c + i);
-                                    if (!(fabsf(x) <= FLT_MAX)) o[t][i] += x;
-                                }
+                        for (int i = 0; i < 4; i++) o[t][i] = ca_add_bad(o[t][i], y[i]);
                     }
             }
+            kb = kn;
         }
         l += lg_partner<4>(l);
         l += lg_partner<5>(l);
         mx = l == 0.0f ? -INFINITY : m * sc;
     }
-    /* the four waves' parts of each column together, by way of LDS */
+    /* the waves' parts of each column together, by way of LDS */
     float* const sO = (float*)(s_raw + wave * C::WAVE);
 #pragma unroll
     for (int t = 0; t < NT; t++) *(v4f*)(sO + col * C::OST + 16 * t + 4 * c) = o[t];
@@ -333,15 +385,15 @@ __global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a,
         s_ml[wave][col][1] = l;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < ncol * (HD / 4); i += 256) {
+    for (int i = threadIdx.x; i < ncol * (HD / 4); i += 64 * NW) {
         const int k = i / (HD / 4), d = i % (HD / 4) * 4;
         float M = s_ml[0][k][0];
 #pragma unroll
-        for (int w = 1; w < 4; w++) M = fmaxf(M, s_ml[w][k][0]);
+        for (int w = 1; w < NW; w++) M = fmaxf(M, s_ml[w][k][0]);
         v4f y = {};
         float L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             /* (a wave without keys has l = 0 and all zeros) */
             const float lw = s_ml[w][k][1], f = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][k][0] - M);
             const v4f x = *(const v4f*)((const float*)(s_raw + w * C::WAVE) + k * C::OST + d);
@@ -354,7 +406,7 @@ __global__ __launch_bounds__(256, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a,
         if (part) {
             const int64_t at = ((int64_t)sp * a.rows + r) * a.n_heads + hh;
             *(v4f*)(part + at * HD + d) = y;
-            if (d == 0) *(float2*)(part + (int64_t)nsplit * a.rows * a.n_heads * HD + 2 * at) = make_float2(M, L);
+            if (d == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(M, L);
         } else {
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             const int pk = a.pos[r];
@@ -479,7 +531,8 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
     float l = 0.0f, mx = -INFINITY;
     if (pmax >= 0) {
         const CaTiles tiles(a, pmin, pmax, KT);
-        const int t0 = (int)((int64_t)tiles.n * sp / nsplit), t1 = (int)((int64_t)tiles.n * (sp + 1) / nsplit);
+        int t0, t1;
+        tiles.chunk(sp, nsplit, 0, &t0, &t1);
         const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
         const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
         /* tiles with keys that some row of the workgroup (wave) does not see */
@@ -591,10 +644,12 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
 #pragma unroll
                             for (int t = 0; t < NT; t++)
 #pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    const int d = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-                                    const float x = HD % 32 == 0 || d < HD ? ca_value(a.c, vc, g, key, d) : 0.0f;
-                                    if (!(fabsf(x) <= FLT_MAX)) o[t][i] += x;
+                                for (int i = 0; i < 16; i += 4) {
+                                    const int d = 32 * t + 2 * i + 4 * h;
+                                    if (HD % 32 != 0 && d >= HD) continue;
+                                    const v4f x = ca_values(a.c, vc, g, key, d);
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) o[t][i + e] = ca_add_bad(o[t][i + e], x[e]);
                                 }
                     }
             }
@@ -616,45 +671,68 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             const v4f y = {o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
             if (HD % 32 == 0 || d < HD) *(v4f*)(dst + d) = p < 0 ? (v4f){} : y * f;
         }
-    if (part && h == 0) *(float2*)(part + (int64_t)nsplit * a.rows * a.n_heads * HD + 2 * at) = make_float2(mx, l);
+    if (part && h == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(mx, l);
 }
 
-/* the splits' parts of a row's head: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M);
- * a thread per four dims */
+/* the splits' parts of a row's head: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M),
+ * a thread per four dims.  G threads share them where there are many parts and
+ * few rows: one thread alone waits for one load after the other (64 parts of 32
+ * heads: 34 us; 3.x with eight). */
+template <int G>
 __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const float* __restrict__ part)
 {
-    const int hd = a.c.hd, dq = hd / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.rows * a.n_heads;
-    if (i >= n * dq) return;
-    const int64_t at = i / dq, row = at / a.n_heads;
-    const int d = (int)(i % dq) * 4, head = (int)(at % a.n_heads), p = a.pos[row];
+    __shared__ v4f s_y[G > 1 ? 256 : 1];
+    __shared__ float s_l[G > 1 ? 256 : 1];
+    const int hd = a.c.hd, dq = hd / 4, per = 256 / G;
+    const int64_t i = (int64_t)blockIdx.x * per + threadIdx.x % per, n = (int64_t)a.rows * a.n_heads;
+    const int64_t at = min(i / dq, n - 1), row = at / a.n_heads;
+    const int d = (int)(i % dq) * 4, head = (int)(at % a.n_heads), p = a.pos[row], grp = threadIdx.x / per;
     const float2* const ml = (const float2*)(part + nsplit * n * hd);
     v4f y = {};
     float L = 0.0f;
     if (p >= 0 && p <= a.max_pos) {
         float M = -INFINITY;
+#pragma unroll 4
         for (int s = 0; s < nsplit; s++) M = fmaxf(M, ml[s * n + at].x);
-        for (int s = 0; s < nsplit; s++) {
+#pragma unroll 2
+        for (int s = grp; s < nsplit; s += G) {
             const float2 x = ml[s * n + at];
-            const float f = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - M);
-            const v4f v = *(const v4f*)(part + (s * n + at) * hd + d);
+            const bool some = x.y != 0.0f;
+            const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
+            const v4f v = some ? *(const v4f*)(part + (s * n + at) * hd + d) : (v4f){};
             L = __builtin_fmaf(x.y, f, L);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
         }
     }
-    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = y * (L == 0.0f ? 0.0f : 1.0f / L);
+    if constexpr (G > 1) {
+        s_y[threadIdx.x] = y;
+        s_l[threadIdx.x] = L;
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int k = 1; k < G; k++) {
+            y += s_y[threadIdx.x + k * per];
+            L += s_l[threadIdx.x + k * per];
+        }
+    }
+    if (i < n * dq) *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = y * (L == 0.0f ? 0.0f : 1.0f / L);
 }
 
 /* How a call is cut, from its sizes alone. */
 struct CaPlan {
     bool dec;     /* up to 16 columns a key head */
     int ncb;      /* else: blocks of columns of a sequence's key head */
-    int nsplit;
+    bool wide;    /* dec: eight waves a workgroup */
+    int nsplit, chunk;   /* parts of the keys, tiles in a part */
     size_t ws;
 };
 
-static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos)
+/* keys a wave takes at a time (CaDec) */
+static int CA_KT(int hd, bool kv4) { return kv4 && hd <= 128 ? 64 : 32; }
+
+static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos,
+                      bool kv4)
 {
     CaPlan p = {};
     const int64_t cols = ntok * (n_heads / n_kv);
@@ -667,8 +745,20 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         p.ncb = (int)((cols + width - 1) / width);
         p.nsplit = (int)std::max<int64_t>(1, std::min(256 / (nseq * n_kv * p.ncb), keys / 512));
     } else {
-        /* two workgroups a CU, each with at least a tile for each wave */
-        p.nsplit = (int)std::max<int64_t>(1, std::min(512 / (nseq * n_kv), (keys + 255) / 256));
+#ifndef CA_SLOTS
+#define CA_SLOTS (kv4 ? 256 : 512)
+#define CA_MIN 256
+#endif
+        const int64_t groups = nseq * n_kv;
+        const int kt = CA_KT(hd, kv4);
+        p.wide = hd <= 128 && keys <= 1024 && groups <= 256;
+        if (!p.wide) {
+            /* two workgroups a CU, each with at least a tile or two for each wave; chunks short enough to even
+             * out ragged lengths */
+            p.nsplit = (int)std::max<int64_t>({1, std::min(CA_SLOTS / groups, (keys + CA_MIN - 1) / CA_MIN),
+                                               std::min<int64_t>(keys / (kv4 ? 2048 : 1024), 16384 / groups)});
+            p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
+        }
     }
     if (p.nsplit > 1) p.ws = (size_t)p.nsplit * nseq * ntok * n_heads * (hd + 2) * sizeof(float);
     return p;
@@ -678,15 +768,21 @@ extern "C" size_t lg_attn_cache_workspace_size(int nseq, int ntok, int n_heads, 
                                                int sinks, int max_pos)
 {
     if (nseq <= 0 || ntok <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_pos < 0) return 0;
-    return ca_plan(nseq, ntok, n_heads, n_kv_heads, head_dim, window, sinks, max_pos).ws;
+    return std::max(ca_plan(nseq, ntok, n_heads, n_kv_heads, head_dim, window, sinks, max_pos, false).ws,
+                    ca_plan(nseq, ntok, n_heads, n_kv_heads, head_dim, window, sinks, max_pos, true).ws);
 }
 
 template <int HD, bool KV4>
 static void ca_launch(const CAttn& a, const CaPlan& p, int nseq, float* part, hipStream_t s)
 {
     const int64_t n = (int64_t)nseq * a.c.n_kv * p.nsplit;
+    if constexpr (HD <= 128)
+        if (p.dec && p.wide) {
+            k_cattn_dec<HD, KV4, 8><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
+            return;
+        }
     if (p.dec)
-        k_cattn_dec<HD, KV4><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, part);
+        k_cattn_dec<HD, KV4, 4><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
     else
         k_cattn_tile<HD, KV4><<<(unsigned)(n * p.ncb), CaTile<HD, KV4>::NTH, 0, s>>>(a, p.ncb, p.nsplit, part);
 }
@@ -737,7 +833,7 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     a.rows = (int)rows;
     a.nrep = n_heads / a.c.n_kv;
     a.scale2 = 1.44269504088896341f / sqrtf((float)hd);
-    const CaPlan p = ca_plan(nseq, ntok, n_heads, a.c.n_kv, hd, window, sinks, max_pos);
+    const CaPlan p = ca_plan(nseq, ntok, n_heads, a.c.n_kv, hd, window, sinks, max_pos, a.c.type == LG_KV4);
     if (p.ws && (!workspace || !lg_al16(workspace) || workspace_bytes < p.ws)) {
         lg_set_error("%s: workspace of %zu bytes, 16-byte aligned, %zu needed", who, workspace_bytes, p.ws);
         return LG_ERR_ARG;
@@ -751,6 +847,12 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     case 128: ca_type<128>(a, p, nseq, part, s); break;
     default: ca_type<256>(a, p, nseq, part, s); break;
     }
-    if (part) k_cattn_merge<<<(unsigned)((rows * n_heads * (hd / 4) + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
+    if (part) {
+        const int64_t n = rows * n_heads * (hd / 4);   /* threads of a group */
+        if (p.nsplit > 8)
+            k_cattn_merge<8><<<(unsigned)((n + 31) / 32), 256, 0, s>>>(a, p.nsplit, part);
+        else
+            k_cattn_merge<1><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
+    }
     return lg_check_launch(who);
 }

@@ -33,18 +33,30 @@ __device__ __forceinline__ size_t lg_kv4_dm(const LgKv& c, int g, int pos)
     return (size_t)c.n_kv * c.n_ctx * (c.hd / 2) + ((size_t)g * c.n_ctx + pos) * (c.hd / 8);
 }
 
-/* the eight fp16 values of a word of codes: 2j, 2j + 1 in v[j].  c | 0x6400 is
- * 1024 + c in fp16, exact, as is the difference; c d + m is one fused fp16
- * multiply-add, the one rounding that the format has. */
+/* the eight fp16 values of a word of codes: 2j, 2j + 1 in v[j].  A code under
+ * the exponent of 1024 is 1024 + c (in bits 0..3) or 1024 + 16 c (4..7); taking
+ * the 1024 off, for the latter as x / 16 - 64, is exact.  c d + m is one fused
+ * fp16 multiply-add, the one rounding that the format has.  The constants are
+ * kept in registers: v_and_or_b32 takes no literal, and as literals they cost
+ * two operations and a shift more per pair (19 a word instead of 13). */
 __device__ __forceinline__ void lg_kv4_values(uint32_t w, uint32_t dm, lg_h2 v[4])
 {
+    uint32_t m0 = 0x000F000Fu, m1 = 0x00F000F0u, one = 0x64006400u;
+    __asm__("" : "+v"(m0));
+    __asm__("" : "+v"(m1));
+    __asm__("" : "+s"(one));
     const lg_h2 x = __builtin_bit_cast(lg_h2, dm), d = {x[0], x[0]}, m = {x[1], x[1]};
-    const lg_h2 off = {(_Float16)1024.0f, (_Float16)1024.0f};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const lg_h2 c = __builtin_bit_cast(lg_h2, ((w >> (4 * j)) & 0x000F000Fu) | 0x64006400u) - off;
-        v[j] = __builtin_elementwise_fma(c, d, m);
-    }
+    const lg_h2 off = {(_Float16)-1024.0f, (_Float16)-1024.0f}, six = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const lg_h2 off16 = {(_Float16)-64.0f, (_Float16)-64.0f};
+    const uint32_t u = w >> 8;
+    const lg_h2 c0 = __builtin_bit_cast(lg_h2, (w & m0) | one) + off;
+    const lg_h2 c1 = __builtin_elementwise_fma(__builtin_bit_cast(lg_h2, (w & m1) | one), six, off16);
+    const lg_h2 c2 = __builtin_bit_cast(lg_h2, (u & m0) | one) + off;
+    const lg_h2 c3 = __builtin_elementwise_fma(__builtin_bit_cast(lg_h2, (u & m1) | one), six, off16);
+    v[0] = __builtin_elementwise_fma(c0, d, m);
+    v[1] = __builtin_elementwise_fma(c1, d, m);
+    v[2] = __builtin_elementwise_fma(c2, d, m);
+    v[3] = __builtin_elementwise_fma(c3, d, m);
 }
 
 /* the codes of eight values of a group of 32 that four neighbouring lanes
