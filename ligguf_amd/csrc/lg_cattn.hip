@@ -7,9 +7,6 @@
 #include <algorithm>
 
 #include "lg_kv.h"
-#ifndef CA_W
-#define CA_W 2
-#endif
 
 struct CAttn {
     const float* q;
@@ -77,10 +74,11 @@ __device__ __forceinline__ bool ca_drop_bad(v4u& w)
 __device__ __forceinline__ uint64_t ca_row16(uint64_t b) { return (b | b >> 16 | b >> 32 | b >> 48) & 0xFFFF; }
 
 /* four values of a cached value row, from dim d (a multiple of 4) on */
+template <bool KV4>
 __device__ __forceinline__ v4f ca_values(const LgKv& c, const uint8_t* v, int g, int key, int d)
 {
     lg_h2 x[4];
-    if (c.type == LG_F16) *(uint2*)x = *(const uint2*)(v + lg_kv16_at(c, g, key) + 2 * d);
+    if constexpr (!KV4) *(uint2*)x = *(const uint2*)(v + lg_kv16_at(c, g, key) + 2 * d);
     else {
         lg_kv4_values(*(const uint32_t*)(v + lg_kv4_codes(c, g, key) + d / 8 * 4),
                       *(const uint32_t*)(v + lg_kv4_dm(c, g, key) + d / 32 * 4), x);
@@ -194,7 +192,7 @@ struct CaRows {
 };
 
 template <int HD, bool KV4, int NW>
-__global__ __launch_bounds__(64 * NW, (HD <= 128 ? CA_W : 1)) void k_cattn_dec(CAttn a, int nsplit, int chunk,
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a, int nsplit, int chunk,
                                                                            float* __restrict__ part)
 {
     using C = CaDec<HD, KV4>;
@@ -365,7 +363,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? CA_W : 1)) void k_cattn_dec(C
                 if (ca_sees(a, p, key))
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        const v4f y = ca_values(a.c, vc, g, key, 16 * t + 4 * c);
+                        const v4f y = ca_values<KV4>(a.c, vc, g, key, 16 * t + 4 * c);
 #pragma unroll
                         for (int i = 0; i < 4; i++) o[t][i] = ca_add_bad(o[t][i], y[i]);
                     }
@@ -441,17 +439,21 @@ struct CaPieces {
     uint2 w[KV4 ? C::NP : 1];
     uint32_t dm[KV4 ? C::NP : 1];
 
+    /* (the tile's address is the wave's, a thread's part of it fits 32 bits) */
     __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb)
     {
+        const uint8_t* const p = base + (KV4 ? lg_kv4_codes(a.c, g, kb) : lg_kv16_at(a.c, g, kb));
+        const uint8_t* const q = base + (KV4 ? lg_kv4_dm(a.c, g, kb) : 0);
+        const int last = a.max_pos - kb;   /* (rows past it are never visible) */
 #pragma unroll
         for (int u = 0; u < C::NP; u++) {
             const int i = min((int)threadIdx.x + u * C::NTH, C::KT * C::PR - 1);
-            const int key = min(kb + i / C::PR, a.max_pos), x = i % C::PR;   /* (rows past it are never visible) */
+            const uint32_t key = min(i / C::PR, last), x = i % C::PR;
             if constexpr (KV4) {
-                w[u] = *(const uint2*)(base + lg_kv4_codes(a.c, g, key) + 8 * x);
-                dm[u] = *(const uint32_t*)(base + lg_kv4_dm(a.c, g, key) + x / 2 * 4);
+                w[u] = *(const uint2*)(p + (key * (HD / 2) + 8 * x));
+                dm[u] = *(const uint32_t*)(q + (key * (HD / 8) + x / 2 * 4));
             } else
-                h[u] = *(const v4u*)(base + lg_kv16_at(a.c, g, key) + 16 * x);
+                h[u] = *(const v4u*)(p + (key * (uint32_t)(a.c.n_kv * HD * 2) + 16 * x));
         }
     }
     /* into rows of ST halves; with `bad`, infinities and NaN as 0 and their keys noted */
@@ -495,7 +497,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
     const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv;
     const int seq = blockIdx.x / n_kv % (a.rows / a.ntok), rest = blockIdx.x / n_kv / (a.rows / a.ntok);
     const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int ncol = a.ntok * a.nrep, idx = cb * 32 * C::NW + 32 * wave + col;
     const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
     const int64_t row = (int64_t)seq * a.ntok + tok;
@@ -576,6 +578,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             if (more) P.load(a, kc, g, kn);
             v16f s[NK];
             if (on) {
+                __builtin_amdgcn_s_setprio(1);   /* its products ahead of the other wave's softmax: 700 x 9000 251 -> 243 us */
 #pragma unroll
                 for (int n = 0; n < NK; n++) s[n] = (v16f){};
 #pragma unroll
@@ -587,6 +590,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                         s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[j], s[n], 0, 0, 0);
                     }
             }
+            __builtin_amdgcn_s_setprio(0);
             if (more) {
                 P.template store<C::KST>(nK, nullptr);
                 P.load(a, vc, g, kn);
@@ -647,7 +651,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                                 for (int i = 0; i < 16; i += 4) {
                                     const int d = 32 * t + 2 * i + 4 * h;
                                     if (HD % 32 != 0 && d >= HD) continue;
-                                    const v4f x = ca_values(a.c, vc, g, key, d);
+                                    const v4f x = ca_values<KV4>(a.c, vc, g, key, d);
 #pragma unroll
                                     for (int e = 0; e < 4; e++) o[t][i + e] = ca_add_bad(o[t][i + e], x[e]);
                                 }
@@ -745,17 +749,13 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         p.ncb = (int)((cols + width - 1) / width);
         p.nsplit = (int)std::max<int64_t>(1, std::min(256 / (nseq * n_kv * p.ncb), keys / 512));
     } else {
-#ifndef CA_SLOTS
-#define CA_SLOTS (kv4 ? 256 : 512)
-#define CA_MIN 256
-#endif
         const int64_t groups = nseq * n_kv;
         const int kt = CA_KT(hd, kv4);
         p.wide = hd <= 128 && keys <= 1024 && groups <= 256;
         if (!p.wide) {
             /* two workgroups a CU, each with at least a tile or two for each wave; chunks short enough to even
              * out ragged lengths */
-            p.nsplit = (int)std::max<int64_t>({1, std::min(CA_SLOTS / groups, (keys + CA_MIN - 1) / CA_MIN),
+            p.nsplit = (int)std::max<int64_t>({1, std::min((kv4 ? 256 : 512) / groups, (keys + 255) / 256),
                                                std::min<int64_t>(keys / (kv4 ? 2048 : 1024), 16384 / groups)});
             p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
         }
