@@ -114,107 +114,194 @@ __device__ __forceinline__ float2 lg_turn(int pos, float freq, float mscale)
     return make_float2((float)c * mscale, (float)s * mscale);
 }
 
-/* One workgroup per token and block of heads, one wave per head: queries,
- * then keys, then values.  A lane holds pairs p = lane, lane + 64 of its head:
- * the two values that turn together, or past rope_dim two neighbours that stay
- * -- so a pair never leaves its lane in either layout.  Rows for the 4-bit
- * cache go through LDS to eight consecutive values a lane. */
-template <bool HALF>
+typedef float v2f __attribute__((ext_vector_type(2), aligned(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+/* A workgroup takes a token's heads from `blk * per` rounds on: queries, then
+ * keys, then values; in a round each of its four waves takes 64 / G heads, G
+ * lanes a head.  A lane holds N neighbouring pairs p = N i .. of its head (and
+ * those 64 on, in the one-pair form): the two values that turn together, or
+ * past rope_dim two neighbours that stay -- so a pair never leaves its lane in
+ * either layout, and the norm's sum is the only exchange.  N = 2 needs the
+ * pairs to come in twos (head_dim % 4 == 0, rope_dim % 4 == 0): 16 bytes a
+ * lane.  N = 1 takes every other shape.  Bound by its bytes: 6000 tokens of
+ * 32 + 8 heads of 128, 246 MB, 46 us, 5.3 TB/s (73 us with one pair a lane; 56
+ * with two rounds loaded at a time, whose registers halve the waves).  Rows for the 4-bit cache
+ * go through LDS to eight consecutive values a lane. */
+template <bool HALF, int N, int G>
 __global__ __launch_bounds__(256) void k_rope_tokens(RopeArgs a, int nblk, int per)
 {
+    constexpr int HPW = 64 / G, J = N == 2 ? 1 : 2;   /* heads of a wave, runs of pairs of a lane */
     __shared__ float2 s_cs[128];
     __shared__ __attribute__((aligned(16))) float s_row[4][256];
     const int row = blockIdx.x / nblk, blk = blockIdx.x % nblk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane % G;
     const int pos = a.pos[row];
-    const bool on = pos >= 0 && (!a.c.type || pos < a.c.n_ctx);   /* (workgroup-uniform) */
     const int np = a.rope / 2, hd = a.hd, seq = row / a.ntok;
-    if (on && threadIdx.x < np) s_cs[threadIdx.x] = lg_turn(pos, a.freq[threadIdx.x], a.mscale);
-    __syncthreads();
     const int n_all = a.n_heads + a.n_kv * (a.c.type ? 2 : 1);
+    const bool on = pos >= 0 && (!a.c.type || pos < a.c.n_ctx);   /* (workgroup-uniform) */
+
+    struct Head {
+        int kind, g;   /* 0 query, 1 key, 2 value, 3 none */
+        float e[J][2 * N];
+    };
+    auto head_of = [&](int h, Head& x) {
+        x.kind = h < a.n_heads ? 0 : h < a.n_heads + a.n_kv ? 1 : h < n_all ? 2 : 3;
+        x.g = x.kind == 0 ? h : x.kind == 1 ? h - a.n_heads : h - a.n_heads - a.n_kv;
+    };
+    /* element e of the lane's run j: pair N (li + G j) + e / 2; HALF keeps the first
+     * values of its pairs together, then the second ones */
+    auto at = [&](int j, int e, bool value) {
+        const int p = N * (li + G * j), half = HALF && !value && p < np;
+        return half ? (e < N ? p + e : p + np + e - N) : 2 * p + e;
+    };
+    auto turns = [&](int j, bool value) { return !value && N * (li + G * j) < np; };
+    auto in = [&](int j) { return N * (li + G * j) < hd / 2; };
+    auto ld = [&](const float* p, int j, bool value, float* e) {
+        if constexpr (N == 2) {
+            if (HALF) {
+                *(v2f*)e = *(const v2f*)(p + at(j, 0, value));
+                *(v2f*)(e + 2) = *(const v2f*)(p + at(j, 2, value));
+            } else
+                *(v4f*)e = *(const v4f*)(p + at(j, 0, value));
+        } else {
+            e[0] = p[at(j, 0, value)];
+            e[1] = p[at(j, 1, value)];
+        }
+    };
+    auto st = [&](float* p, int j, bool value, const float* e) {
+        if constexpr (N == 2) {
+            if (HALF) {
+                *(v2f*)(p + at(j, 0, value)) = *(const v2f*)e;
+                *(v2f*)(p + at(j, 2, value)) = *(const v2f*)(e + 2);
+            } else
+                *(v4f*)(p + at(j, 0, value)) = *(const v4f*)e;
+        } else {
+            p[at(j, 0, value)] = e[0];
+            p[at(j, 1, value)] = e[1];
+        }
+    };
+
     for (int i = 0; i < per; i++) {
-        const int h = (blk * per + i) * 4 + wave;   /* (wave-uniform) */
-        if (h >= n_all) return;
-        const int kind = h < a.n_heads ? 0 : h < a.n_heads + a.n_kv ? 1 : 2;
-        const int g = kind == 0 ? h : kind == 1 ? h - a.n_heads : h - a.n_heads - a.n_kv;
-        const float* const x = kind == 0 ? a.q + row * a.qs : kind == 1 ? a.k + row * a.ks : a.v + row * a.vs;
-        float* const y = kind == 0 ? a.qo + row * a.qos : kind == 1 && a.ko ? a.ko + row * a.kos : nullptr;
-        const float* const w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
-        const int turning = kind == 2 ? 0 : np;
-        float e[2][2] = {};
-        int at[2][2];
+        const int h0 = ((blk * per + i) * 4 + wave) * HPW;
+        Head x;
+        head_of(h0 + lane / G, x);
+        const int kind = x.kind, g = x.g;
+        {
+            const float* const p = kind == 0 ? a.q + row * a.qs : kind == 1 ? a.k + row * a.ks : a.v + row * a.vs;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int p = lane + 64 * j;
-            const bool turn = HALF && p < np && kind != 2;
-            at[j][0] = turn ? p : 2 * p;
-            at[j][1] = turn ? p + np : 2 * p + 1;
-            if (on && p < hd / 2) {
-                e[j][0] = x[(size_t)g * hd + at[j][0]];
-                e[j][1] = x[(size_t)g * hd + at[j][1]];
+            for (int j = 0; j < J; j++) {
+#pragma unroll
+                for (int e = 0; e < 2 * N; e++) x.e[j][e] = 0.0f;
+                if (on && kind < 3 && in(j)) ld(p + (size_t)g * hd, j, kind == 2, x.e[j]);
             }
         }
-        if (w && on) {
+        if (i == 0) {   /* (the first loads are on their way) */
+            if (on && (int)threadIdx.x < np) s_cs[threadIdx.x] = lg_turn(pos, a.freq[threadIdx.x], a.mscale);
+            __syncthreads();
+        }
+        const bool value = kind == 2;
+        const float* const w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
+        if (a.qw || a.kw) {   /* (all lanes take part in the sums) */
             float ss = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 2; j++) ss += lg_fma2(e[j][0], e[j][0], e[j][1], e[j][1]);
-            const float sc = 1.0f / sqrtf(lg_group_sum<64>(ss) / (float)hd + a.eps);
+            for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (lane + 64 * j < hd / 2) {
-                    e[j][0] = e[j][0] * sc * w[at[j][0]];
-                    e[j][1] = e[j][1] * sc * w[at[j][1]];
+                for (int e = 0; e < 2 * N; e++) ss = __builtin_fmaf(x.e[j][e], x.e[j][e], ss);
+            const float sc = 1.0f / sqrtf(lg_group_sum<G>(ss) / (float)hd + a.eps);
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                if (w && in(j)) {
+                    float f[2 * N];
+                    ld(w, j, value, f);
+#pragma unroll
+                    for (int e = 0; e < 2 * N; e++) x.e[j][e] = on ? x.e[j][e] * sc * f[e] : 0.0f;
                 }
         }
+        float* const y = kind == 0 ? a.qo + row * a.qos : kind == 1 && a.ko ? a.ko + row * a.kos : nullptr;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int p = lane + 64 * j;
-            if (on && p < turning) {
-                const float2 t = s_cs[p];
-                const float x0 = e[j][0], x1 = e[j][1];
-                e[j][0] = lg_fma2(x0, t.x, -x1, t.y);
-                e[j][1] = lg_fma2(x0, t.y, x1, t.x);
+        for (int j = 0; j < J; j++) {
+            float* const e = x.e[j];
+            if (on && turns(j, value)) {
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    const float2 t = s_cs[N * (li + G * j) + k];
+                    float &v0 = e[HALF ? k : 2 * k], &v1 = e[HALF ? k + N : 2 * k + 1];
+                    const float x0 = v0, x1 = v1;
+                    v0 = lg_fma2(x0, t.x, -x1, t.y);
+                    v1 = lg_fma2(x0, t.y, x1, t.x);
+                }
             }
-            if (y && p < hd / 2) {
-                y[(size_t)g * hd + at[j][0]] = e[j][0];
-                y[(size_t)g * hd + at[j][1]] = e[j][1];
-            }
+            if (kind < 2 && y && in(j)) st(y + (size_t)g * hd, j, value, e);
         }
-        if (kind == 0 || !a.c.type || !on) continue;
-        uint8_t* const cache = (kind == 1 ? a.c.k : a.c.v) + (size_t)seq * a.c.seq;
+        if (!a.c.type || !on) continue;
         if (a.c.type == LG_F16) {
-            uint16_t* const r = (uint16_t*)(cache + lg_kv16_at(a.c, g, pos));
+            if (kind == 1 || kind == 2) {
+                uint16_t* const r = (uint16_t*)((value ? a.c.v : a.c.k) + (size_t)seq * a.c.seq + lg_kv16_at(a.c, g, pos));
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (lane + 64 * j < hd / 2) {
-                    r[at[j][0]] = lg_f2h(e[j][0]);
-                    r[at[j][1]] = lg_f2h(e[j][1]);
-                }
-        } else {
+                for (int j = 0; j < J; j++)
+                    if (in(j)) {
+                        const float* const e = x.e[j];
+                        if constexpr (N == 2) {
+                            const uint32_t w0 = (uint32_t)lg_f2h(e[0]) | (uint32_t)lg_f2h(e[1]) << 16;
+                            const uint32_t w1 = (uint32_t)lg_f2h(e[2]) | (uint32_t)lg_f2h(e[3]) << 16;
+                            if (HALF) {
+                                *(uint32_t*)(r + at(j, 0, value)) = w0;
+                                *(uint32_t*)(r + at(j, 2, value)) = w1;
+                            } else
+                                *(uint2*)(r + at(j, 0, value)) = make_uint2(w0, w1);
+                        } else {
+                            r[at(j, 0, value)] = lg_f2h(e[0]);
+                            r[at(j, 1, value)] = lg_f2h(e[1]);
+                        }
+                    }
+            }
+        } else if (__builtin_amdgcn_ballot_w64(kind == 1 || kind == 2)) {
             float* const s = s_row[wave];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (lane + 64 * j < hd / 2) {
-                    s[at[j][0]] = e[j][0];
-                    s[at[j][1]] = e[j][1];
-                }
+            for (int j = 0; j < J; j++)
+                if (in(j)) st(s + lane / G * hd, j, value, x.e[j]);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const int hw = hd / 8, k = lane / hw;   /* the wave's head that this lane has a word of, four lanes a group */
+            Head z;
+            head_of(h0 + k, z);
             float v[8] = {};
-            if (lane < hd / 8) {
-                *(float4*)v = *(const float4*)(s + 8 * lane);
-                *(float4*)(v + 4) = *(const float4*)(s + 8 * lane + 4);
+            if (k < HPW) {
+                *(v4f*)v = *(const v4f*)(s + 8 * lane);
+                *(v4f*)(v + 4) = *(const v4f*)(s + 8 * lane + 4);
             }
             uint32_t dm;
             const uint32_t code = lg_kv4_encode(v, &dm);
-            if (lane < hd / 8) {
-                ((uint32_t*)(cache + lg_kv4_codes(a.c, g, pos)))[lane] = code;
-                if (lane % 4 == 0) ((uint32_t*)(cache + lg_kv4_dm(a.c, g, pos)))[lane / 4] = dm;
+            if (k < HPW && (z.kind == 1 || z.kind == 2)) {
+                uint8_t* const c = (z.kind == 2 ? a.c.v : a.c.k) + (size_t)seq * a.c.seq;
+                const int wd = lane % hw;
+                ((uint32_t*)(c + lg_kv4_codes(a.c, z.g, pos)))[wd] = code;
+                if (wd % 4 == 0) ((uint32_t*)(c + lg_kv4_dm(a.c, z.g, pos)))[wd / 4] = dm;
             }
-            __builtin_amdgcn_wave_barrier();   /* the row's reads before the next head's writes */
+            __builtin_amdgcn_wave_barrier();   /* the row's reads before the next round's writes */
         }
     }
+}
+
+template <bool HALF, int N, int G>
+static void rope_launch(const RopeArgs& a, int64_t rows, int all, hipStream_t s)
+{
+    /* rounds of four waves' heads.  Many rows: a workgroup takes all of a token's, so that its angles (in double) are
+     * worked out once; few: one round each, for more of them at a time */
+    const int rounds = (all + 4 * (64 / G) - 1) / (4 * (64 / G));
+    const int nblk = rows >= 512 ? 1 : rounds;
+    k_rope_tokens<HALF, N, G><<<(unsigned)(rows * nblk), 256, 0, s>>>(a, nblk, nblk == 1 ? rounds : 1);
+}
+
+template <bool HALF>
+static void rope_shape(const RopeArgs& a, int64_t rows, int all, hipStream_t s)
+{
+    if (a.hd % 4 || a.rope % 4 || (a.qw && !lg_al16(a.qw)) || (a.kw && !lg_al16(a.kw))) rope_launch<HALF, 1, 64>(a, rows, all, s);
+    else if (a.hd <= 64) rope_launch<HALF, 2, 16>(a, rows, all, s);
+    else if (a.hd <= 128) rope_launch<HALF, 2, 32>(a, rows, all, s);
+    else rope_launch<HALF, 2, 64>(a, rows, all, s);
 }
 
 static bool rows_bad(const void* p, int64_t stride, int64_t least)
@@ -262,33 +349,32 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
             return LG_ERR_ARG;
         }
     }
-    const int waves = n_heads + n_kv_heads * (cache ? 2 : 1), all = (waves + 3) / 4;
-    if (rows > INT32_MAX / all) {
+    const int waves = n_heads + n_kv_heads * (cache ? 2 : 1);
+    if (rows > INT32_MAX / waves) {
         lg_set_error("%s: %lld rows of %d heads are too many for one call", who, (long long)rows, waves);
         return LG_ERR_ARG;
     }
-    const int per = rows >= 1024 ? all : 1, nblk = (all + per - 1) / per;
-    if (layout == LG_ROPE_HALF)
-        k_rope_tokens<true><<<(unsigned)(rows * nblk), 256, 0, (hipStream_t)stream>>>(a, nblk, per);
-    else
-        k_rope_tokens<false><<<(unsigned)(rows * nblk), 256, 0, (hipStream_t)stream>>>(a, nblk, per);
+    if (layout == LG_ROPE_HALF) rope_shape<true>(a, rows, waves, (hipStream_t)stream);
+    else rope_shape<false>(a, rows, waves, (hipStream_t)stream);
     return lg_check_launch(who);
 }
 
-/* one thread per word of eight codes; keys, then values */
+/* one thread per word of eight codes; keys, then values.  I: 32 bits where the words of a sequence are fewer
+ * (64-bit divisions cost more than the reads) */
+template <typename I>
 __global__ __launch_bounds__(256) void k_kv4_read(LgKv c, int pos0, int npos, uint16_t* __restrict__ ko,
                                                   uint16_t* __restrict__ vo)
 {
-    const int hw = c.hd / 8;                       /* words of a head's row */
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)npos * c.n_kv * hw) return;
-    const int wd = (int)(i % hw), g = (int)(i / hw % c.n_kv), p = (int)(i / hw / c.n_kv), seq = blockIdx.y;
+    const I hw = c.hd / 8, i = (I)blockIdx.x * 256 + threadIdx.x;   /* words of a head's row */
+    if (i >= (I)npos * c.n_kv * hw) return;
+    const I r = i / hw;
+    const int wd = (int)(i - r * hw), p = (int)(r / (I)c.n_kv), g = (int)(r - p * (I)c.n_kv), seq = blockIdx.y;
     const uint8_t* const b = (blockIdx.z ? c.v : c.k) + (size_t)seq * c.seq;
     const uint32_t w = ((const uint32_t*)(b + lg_kv4_codes(c, g, pos0 + p)))[wd];
     const uint32_t dm = ((const uint32_t*)(b + lg_kv4_dm(c, g, pos0 + p)))[wd / 4];
     lg_h2 v[4];
     lg_kv4_values(w, dm, v);
-    uint16_t* const o = (blockIdx.z ? vo : ko) + (((size_t)seq * npos + p) * c.n_kv + g) * c.hd + 8 * wd;
+    uint16_t* const o = (blockIdx.z ? vo : ko) + (size_t)seq * npos * c.n_kv * c.hd + 8 * (size_t)i;
     *(uint4*)o = *(const uint4*)v;
 }
 
@@ -317,6 +403,8 @@ extern "C" int lg_kv4_read(const lg_kv_cache* cache, int nseq, int pos0, int npo
         return LG_ERR_ARG;
     }
     if (!n || !nseq) return LG_OK;
-    k_kv4_read<<<dim3((unsigned)n, nseq, 2), 256, 0, (hipStream_t)stream>>>(c, pos0, npos, k_out, v_out);
+    const dim3 grid((unsigned)n, nseq, 2);
+    if (n <= INT32_MAX / 256) k_kv4_read<uint32_t><<<grid, 256, 0, (hipStream_t)stream>>>(c, pos0, npos, k_out, v_out);
+    else k_kv4_read<uint64_t><<<grid, 256, 0, (hipStream_t)stream>>>(c, pos0, npos, k_out, v_out);
     return lg_check_launch(who);
 }

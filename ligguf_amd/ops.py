@@ -129,21 +129,15 @@ def _on(i, fn, *args):
         check(rc)
 
 
-def _rows(t, pos, width, name):
-    """(pointer, floats from row to row) of fp32 rows [nseq, ntok, width]; the
-    last axis is dense and the first two are one run of rows."""
-    nseq, ntok = pos.shape
-    if t.dtype is not _FP32 or t.device != pos.device or t.shape != (nseq, ntok, width):
-        _refuse(f"{name}: fp32 [{nseq}, {ntok}, {width}] on {pos.device} wanted, {t.dtype} {tuple(t.shape)} on {t.device} given")
+def _rows(t, i, nseq, ntok, width, name):
+    """(pointer, floats from row to row) of fp32 rows [nseq, ntok, width] on
+    device i; the last axis is dense and the first two are one run of rows."""
+    if t.dtype is not _FP32 or t.get_device() != i or t.shape != (nseq, ntok, width):
+        _refuse(f"{name}: fp32 [{nseq}, {ntok}, {width}] on GPU {i} wanted, {t.dtype} {tuple(t.shape)} on {t.device} given")
     s0, s1, s2 = t.stride()
-    if ntok > 1:
-        row = s1
-    elif nseq > 1:
-        row = s0
-    else:
-        row = (width + 3) // 4 * 4
-    if not t.numel():
+    if not (nseq and ntok and width):
         return None, (width + 3) // 4 * 4
+    row = s1 if ntok > 1 else s0 if nseq > 1 else (width + 3) // 4 * 4
     if (s2 != 1 and width > 1) or (nseq > 1 and s0 != row * ntok):
         _refuse(f"{name}: rows of strides {t.stride()} are not one run")
     return t.data_ptr(), row
@@ -155,11 +149,11 @@ def _pos(pos):
     return pos.data_ptr()
 
 
-def _vec(t, n, like, name):
+def _vec(t, n, i, name):
     if t is None:
         return None
-    if t.dtype is not _FP32 or t.device != like.device or not t.is_contiguous() or t.numel() < n:
-        _refuse(f"{name}: {n} contiguous fp32 values on {like.device} wanted")
+    if t.dtype is not _FP32 or t.get_device() != i or not t.is_contiguous() or t.numel() < n:
+        _refuse(f"{name}: {n} contiguous fp32 values on GPU {i} wanted")
     return t.data_ptr()
 
 
@@ -177,8 +171,8 @@ class KvCache:
         if need < 0:
             _refuse(f"no cache of type {type}, {n_ctx} rows, {n_kv_heads} heads of {head_dim}")
         want = torch.float16 if type == F16 else torch.uint8
-        dev, shape = k.device, k.shape
-        if (k.dtype is not want or v.dtype is not want or not k.is_cuda or v.device != dev or v.shape != shape or not k.is_contiguous()
+        i, shape = k.get_device(), k.shape
+        if (k.dtype is not want or v.dtype is not want or i < 0 or v.get_device() != i or v.shape != shape or not k.is_contiguous()
                 or not v.is_contiguous()):
             _refuse(f"k and v: contiguous {want} tensors of one shape on one GPU wanted")
         nseq = shape[0] if len(shape) > 1 else 0
@@ -186,7 +180,7 @@ class KvCache:
         if size < need or (type == F16 and size != need):
             _refuse(f"k and v: {need} bytes a sequence wanted, shape {tuple(shape)} given")
         self.k, self.v, self.type, self.n_ctx, self.nseq = k, v, type, n_ctx, nseq
-        self.n_kv_heads, self.head_dim, self.device = n_kv_heads, head_dim, dev
+        self.n_kv_heads, self.head_dim, self.index = n_kv_heads, head_dim, i
         self.desc = L.LgKvCache(k.data_ptr(), v.data_ptr(), type, n_ctx, n_kv_heads, head_dim, size)
 
     @classmethod
@@ -215,25 +209,33 @@ def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None,
     a fused q | k | v row are fine; q or, without a cache, v may be None) and pos
     [nseq, ntok]: the rotated queries and keys; keys only with want_k or k_out."""
     rope_dim = head_dim if rope_dim is None else rope_dim
-    p, dev = _pos(pos), pos.device
+    p, i = _pos(pos), pos.get_device()
     nseq, ntok = pos.shape
     kd = k.shape[-1]
     qd = 0 if q is None else q.shape[-1]
     if head_dim < 1 or kd % head_dim or qd % head_dim:
         _refuse(f"rows of {qd} and {kd} values are no heads of {head_dim}")
+    at = (i, nseq, ntok)
+    if q is None:
+        q_out, rq, rqo = None, (None, 0), (None, 0)
+    else:
+        rq = _rows(q, *at, qd, "q")
+        if q_out is None:
+            q_out = q.new_empty((nseq, ntok, qd))
+        rqo = _rows(q_out, *at, qd, "q_out")
+    rk = _rows(k, *at, kd, "k")
     if k_out is None and want_k:
         k_out = k.new_empty((nseq, ntok, kd))
-    if q_out is None and q is not None:
-        q_out = q.new_empty((nseq, ntok, qd))
-    if cache is not None and (cache.device != dev or cache.nseq != nseq or v is None):
-        _refuse(f"cache: values and {nseq} sequences on {dev} wanted")
-    none = (None, 0)
-    _on(dev.index, load().lg_qk_norm_rope_tokens, *(none if q is None else _rows(q, pos, qd, "q")),
-        *(none if q is None else _rows(q_out, pos, qd, "q_out")), *_rows(k, pos, kd, "k"),
-        *(none if k_out is None else _rows(k_out, pos, kd, "k_out")),
-        *(none if cache is None else _rows(v, pos, kd, "v")), _vec(qw, head_dim, pos, "qw"), _vec(kw, head_dim, pos, "kw"),
-        qd // head_dim, kd // head_dim, head_dim, rope_dim, int(half), _vec(freq, rope_dim // 2, pos, "freq"), mscale, eps, p,
-        nseq, ntok, None if cache is None else C.byref(cache.desc))
+    rko = (None, 0) if k_out is None else _rows(k_out, *at, kd, "k_out")
+    if cache is None:
+        rv, desc = (None, 0), None
+    else:
+        if cache.index != i or cache.nseq != nseq or v is None:
+            _refuse(f"cache: values and {nseq} sequences on GPU {i} wanted")
+        rv, desc = _rows(v, *at, kd, "v"), C.byref(cache.desc)
+    _on(i, load().lg_qk_norm_rope_tokens, *rq, *rqo, *rk, *rko, *rv, _vec(qw, head_dim, i, "qw"), _vec(kw, head_dim, i, "kw"),
+        qd // head_dim, kd // head_dim, head_dim, rope_dim, 1 if half else 0, _vec(freq, rope_dim // 2, i, "freq"), mscale, eps, p,
+        nseq, ntok, desc)
     return q_out, k_out
 
 
@@ -244,21 +246,21 @@ def kv_values(cache: KvCache, pos0: int = 0, npos: int = None):
     if npos < 0:
         _refuse(f"{npos} rows")
     shape = (cache.nseq, npos, cache.n_kv_heads * cache.head_dim)
-    k = torch.empty(shape, dtype=torch.float16, device=cache.device)
+    k = cache.k.new_empty(shape, dtype=torch.float16)
     v = torch.empty_like(k)
     if npos:
-        _on(cache.device.index, load().lg_kv4_read, C.byref(cache.desc), cache.nseq, pos0, npos, k.data_ptr(), v.data_ptr())
+        _on(cache.index, load().lg_kv4_read, C.byref(cache.desc), cache.nseq, pos0, npos, k.data_ptr(), v.data_ptr())
     return k, v
 
 
-def _work(need, workspace, dev):
-    """(pointer, bytes) of the workspace of a call, a new one unless given."""
+def _work(need, workspace, like):
+    """The workspace of a call beside `like`, a new one unless given, and its (pointer, bytes)."""
     if workspace is None:
         if not need:
             return None, (None, 0)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or not workspace.is_contiguous():
-        _refuse(f"workspace: contiguous memory on {dev} wanted")
+        workspace = like.new_empty((need + 3) // 4)
+    elif workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+        _refuse(f"workspace: contiguous memory on {like.device} wanted")
     return workspace, (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
@@ -266,23 +268,22 @@ def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max
     """lg_attn_cache: q [nseq, ntok, n_heads * head_dim] at pos [nseq, ntok] over
     the cache rows that each position sees.  max_pos, a bound of the positions
     (n_ctx - 1 by default), sizes the launch."""
-    p, dev = _pos(pos), pos.device
+    p, i = _pos(pos), pos.get_device()
     nseq, ntok = pos.shape
-    if cache.device != dev or cache.nseq != nseq:
-        _refuse(f"cache: {nseq} sequences on {dev} wanted")
+    if cache.index != i or cache.nseq != nseq:
+        _refuse(f"cache: {nseq} sequences on GPU {i} wanted")
     max_pos = cache.n_ctx - 1 if max_pos is None else max_pos
     width, hd = q.shape[-1], cache.head_dim
     heads = width // hd
     if heads * hd != width:
         _refuse(f"rows of {width} values are no heads of {hd}")
-    rows = _rows(q, pos, width, "q")
+    rows = _rows(q, i, nseq, ntok, width, "q")
     if out is None:
         out = q.new_empty((nseq, ntok, width))
     lib = load()
-    workspace, ws = _work(lib.lg_attn_cache_workspace_size(nseq, ntok, heads, cache.n_kv_heads, hd, window, sinks, max_pos), workspace,
-                          dev)
-    _on(dev.index, lib.lg_attn_cache, *rows, C.byref(cache.desc), p, nseq, ntok, heads, window, sinks, max_pos,
-        *_rows(out, pos, width, "out"), *ws)
+    workspace, ws = _work(lib.lg_attn_cache_workspace_size(nseq, ntok, heads, cache.n_kv_heads, hd, window, sinks, max_pos), workspace, q)
+    _on(i, lib.lg_attn_cache, *rows, C.byref(cache.desc), p, nseq, ntok, heads, window, sinks, max_pos,
+        *_rows(out, i, nseq, ntok, width, "out"), *ws)
     return out
 
 
@@ -297,19 +298,21 @@ def logprobs(logits, toks=None, top: int = 0, workspace=None) -> Logprobs:
     """lg_logprobs of logits [rows, vocab] (dense rows) and int32 toks [rows]."""
     if logits.dtype is not _FP32 or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         _refuse("logits: dense fp32 rows on the GPU wanted")
-    dev, (rows, vocab) = logits.device, logits.shape
-    if toks is not None and (toks.dtype is not _INT32 or toks.device != dev or toks.shape != (rows,) or not toks.is_contiguous()):
-        _refuse(f"toks: {rows} contiguous int32 on {dev} wanted")
+    i, (rows, vocab) = logits.get_device(), logits.shape
+    if toks is not None and (toks.dtype is not _INT32 or toks.get_device() != i or toks.shape != (rows,) or not toks.is_contiguous()):
+        _refuse(f"toks: {rows} contiguous int32 on {logits.device} wanted")
     if top < 0:
         _refuse(f"top {top}")
-    entropy = logits.new_empty((rows,))
-    lp = None if toks is None else logits.new_empty((rows,))
-    top_lp = logits.new_empty((rows, top)) if top else None
-    top_id = torch.empty_like(top_lp, dtype=_INT32) if top else None
+    new = logits.new_empty
+    entropy = new(rows)
+    lp, pt, pl = (None, None, None) if toks is None else (t := new(rows), toks.data_ptr(), t.data_ptr())
+    top_id = top_lp = None
+    if top:
+        top_lp = new((rows, top))
+        top_id = torch.empty_like(top_lp, dtype=_INT32)
     lib = load()
-    workspace, ws = _work(lib.lg_logprobs_workspace_size(rows, vocab, top), workspace, dev)
-    _on(dev.index, lib.lg_logprobs, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-        None if toks is None else toks.data_ptr(), top, None if toks is None else lp.data_ptr(), entropy.data_ptr(),
+    workspace, ws = _work(lib.lg_logprobs_workspace_size(rows, vocab, top), workspace, logits)
+    _on(i, lib.lg_logprobs, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, pt, top, pl, entropy.data_ptr(),
         top_id.data_ptr() if top else None, top_lp.data_ptr() if top else None, *ws)
     return Logprobs(lp, entropy, top_id, top_lp)
 
