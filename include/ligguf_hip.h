@@ -494,13 +494,11 @@ int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache* cache, co
  *                the lower id, NaN above all (0 <= top <= 32, top <= vocab)
  * toks is device memory.  Each output may be NULL (toks and logprob, top_id
  * and top_logprob go together).  A row with a NaN or +infinity, or with
- * nothing above -infinity, has NaN probabilities and entropy.  workspace as
- * for lg_attn_cache.  No counterpart in the reference. */
+ * nothing above -infinity, has NaN probabilities and entropy.  No
+ * counterpart in the reference. */
 #define LG_LOGPROBS_TOP 32
-size_t lg_logprobs_workspace_size(int rows, int vocab, int top);
 int lg_logprobs(const float* logits, int64_t stride, int rows, int vocab, const int* toks, int top, float* logprob,
-                float* entropy, int* top_id, float* top_logprob, void* workspace, size_t workspace_bytes,
-                void* stream);
+                float* entropy, int* top_id, float* top_logprob, void* stream);
 
 /* ===================================================================== */
 /* BERT sentence embedding and the vector memory (fast/vdb.cpp)           */

@@ -21,9 +21,8 @@ __device__ __forceinline__ float lp_value(uint64_t key)
     return u == 0xFFFFFFFFu ? NAN : __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 
-constexpr int LP_T = 256;       /* threads */
 constexpr int LP_CAP = 1024;    /* candidates that LDS holds */
-constexpr int LP_COLS = 64;     /* lanes whose values are looked through for them */
+constexpr int LP_COLS = 64;     /* threads whose values are looked through for them */
 constexpr float LP_LOG2E = 1.44269504088896341f;
 
 /* a row as quads of 16 aligned bytes: quad q holds ids 4q - sh .. +3, the
@@ -49,13 +48,17 @@ struct LpRow {
 
 struct LpShared {
     uint64_t list[LP_CAP];
-    float red[8], top[LP_T];
-    uint32_t hist[256];
+    float4 sums[16];            /* a wave's m, z, h and its largest value */
+    __attribute__((aligned(16))) uint32_t top[256];
+    uint32_t hist[256], bound;
     uint64_t prefix;
     int n, nsel, need, sel[LP_COLS];
 };
 
-/* f(value, id) for the values of quads q0 + lane column `col` of every LP_T */
+/* a value's place among the reals as an unsigned number; lp_key's upper half */
+__device__ __forceinline__ uint32_t lp_ord(float x) { return (uint32_t)(lp_key(x, 0) >> 32); }
+
+/* f(value, id) for the values of quad q */
 template <typename F>
 __device__ __forceinline__ void lp_quad(const LpRow& r, int q, F f)
 {
@@ -68,60 +71,70 @@ __device__ __forceinline__ void lp_quad(const LpRow& r, int q, F f)
 
 /* the `top` largest keys of s.list[0 .. n), in order, each by the number of
  * larger ones (keys are unique); n >= top */
-template <typename F>
+template <int T, typename F>
 __device__ __forceinline__ void lp_emit(const LpShared& s, int n, int top, F f)
 {
-    for (int i = threadIdx.x; i < n; i += LP_T) {
+    for (int i = threadIdx.x; i < n; i += T) {
         const uint64_t k = s.list[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; j++) rank += s.list[j] > k ? 1 : 0;
         if (rank < top) f(rank, k);
     }
 }
 
-/* The top keys of quads [q0, q1) into s.list, returns how many (top or a few
- * more).  mine: the largest value of this thread's quads q0 + threadIdx.x,
- * + LP_T, ...  At least `top` values reach T, the top-th largest of the
- * threads' own maxima, and all that do lie in the quads of threads whose
- * maximum does: only those few threads' quads are read again.  Where that
- * says little -- many maxima equal to T, fewer maxima than `top`, NaN (any) --
+/* The keys of the row's nq quads that may be among the `top` largest into s.list;
+ * returns how many (top at least).  The workgroup's 256 maxima in s.top, of
+ * disjoint values, are published; mine: this thread's own, of its quads
+ * off + threadIdx.x, + T, ...  A bound that `top` of the 256 reach is found by
+ * halving over the upper 16 bits of their order -- a few values more than
+ * asked reach it -- and all that do lie in the quads of the threads whose
+ * maximum does, so only those are read again.  Where that says little (many
+ * maxima reach the bound, fewer than `top` are above -infinity, NaN: `any`)
  * the top-th key is found digit by digit, a pass over the quads for each of
  * its eight bytes. */
-__device__ __forceinline__ int lp_top(LpShared& s, const LpRow& r, int q0, int q1, int top, float mine, bool any)
+template <int T>
+__device__ __forceinline__ int lp_top(LpShared& s, const LpRow& r, int nq, int off, int top, uint32_t mine, bool any)
 {
     const int t = threadIdx.x;
-    s.top[t] = mine;
-    if (t == 0) {
-        s.n = 0;
-        s.nsel = 0;
+    if (t < 64) {
+        const uint4 v = *(const uint4*)(s.top + 4 * t);
+        uint32_t bound = 0;
+#pragma unroll
+        for (int b = 31; b >= 16; b--) {
+            const uint32_t c = bound | 1u << b;
+            const int n = __popcll(__builtin_amdgcn_ballot_w64(v.x >= c)) + __popcll(__builtin_amdgcn_ballot_w64(v.y >= c)) +
+                          __popcll(__builtin_amdgcn_ballot_w64(v.z >= c)) + __popcll(__builtin_amdgcn_ballot_w64(v.w >= c));
+            if (n >= top) bound = c;
+        }
+        if (t == 0) {
+            s.bound = bound;
+            s.n = 0;
+            s.nsel = 0;
+        }
     }
     __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < LP_T; j += 4) {
-        const float4 v = *(const float4*)(s.top + j);
-        rank += (v.x > mine || (v.x == mine && j < t)) + (v.y > mine || (v.y == mine && j + 1 < t)) +
-                (v.z > mine || (v.z == mine && j + 2 < t)) + (v.w > mine || (v.w == mine && j + 3 < t));
-    }
-    if (rank == top - 1) s.red[0] = mine;
-    __syncthreads();
-    const float T = s.red[0];
-    if (mine >= T && T > -INFINITY) {
+    const uint32_t bound = s.bound;
+    const bool use = !any && bound > 0x007FFFFFu;   /* (that of -infinity) */
+    if (use && mine >= bound) {
         const int i = atomicAdd(&s.nsel, 1);   /* (in whatever order: the list is ranked) */
         if (i < LP_COLS) s.sel[i] = t;
     }
     __syncthreads();
-    const int nsel = s.nsel, per = (q1 - q0 + LP_T - 1) / LP_T;
-    if (!any && nsel && nsel <= LP_COLS) {
-        for (int i = t; i < nsel * per; i += LP_T) {
-            const int q = q0 + s.sel[i / per] + i % per * LP_T;
-            if (q < q1)
-                lp_quad(r, q, [&](float x, int id) {
-                    if (x >= T) {
-                        const int at = atomicAdd(&s.n, 1);
-                        if (at < LP_CAP) s.list[at] = lp_key(x, id);
-                    }
-                });
+    const int nsel = s.nsel, per = (nq + T - 1) / T;
+    if (use && nsel <= LP_COLS) {
+        auto add = [&](float x, int id) {
+            const uint64_t k = lp_key(x, id);
+            if ((uint32_t)(k >> 32) >= bound) {
+                const int at = atomicAdd(&s.n, 1);
+                if (at < LP_CAP) s.list[at] = k;
+            }
+        };
+        for (int i = t; i < nsel * per; i += T) {
+            const int q = off + s.sel[i / per] + i % per * T;
+            if (q < nq) lp_quad(r, q, add);
         }
+        if (off && t == T - 1) lp_quad(r, 0, add);
         __syncthreads();
         if (s.n <= LP_CAP) return s.n;
     }
@@ -130,10 +143,10 @@ __device__ __forceinline__ int lp_top(LpShared& s, const LpRow& r, int q0, int q
         s.need = top;
     }
     for (int d = 7; d >= 0; d--) {
-        s.hist[t] = 0;
+        if (t < 256) s.hist[t] = 0;
         __syncthreads();
         const uint64_t prefix = s.prefix;
-        for (int q = q0 + t; q < q1; q += LP_T)
+        for (int q = t; q < nq; q += T)
             lp_quad(r, q, [&](float x, int id) {
                 const uint64_t k = lp_key(x, id);
                 if (d == 7 || k >> (8 * d + 8) == prefix) atomicAdd(&s.hist[k >> (8 * d) & 255], 1u);
@@ -163,7 +176,7 @@ __device__ __forceinline__ int lp_top(LpShared& s, const LpRow& r, int q0, int q
     const uint64_t last = s.prefix;
     if (t == 0) s.n = 0;
     __syncthreads();
-    for (int q = q0 + t; q < q1; q += LP_T)
+    for (int q = t; q < nq; q += T)
         lp_quad(r, q, [&](float x, int id) {
             const uint64_t k = lp_key(x, id);
             if (k >= last) s.list[atomicAdd(&s.n, 1)] = k;   /* exactly top of them */
@@ -175,12 +188,10 @@ __device__ __forceinline__ int lp_top(LpShared& s, const LpRow& r, int q0, int q
 struct LpArgs {
     const float* logits;
     int64_t stride;
-    int rows, vocab, top, nsplit;
+    int vocab, top;
     const int* toks;
     float *logprob, *entropy, *top_logprob;
     int* top_id;
-    float4* sums;     /* [rows][nsplit]: m, z, h */
-    uint64_t* keys;   /* [rows][nsplit][top], descending */
 };
 
 /* a row's scalars from its m, z = sum e^(x - m), h = sum e^(x - m) (x - m);
@@ -198,35 +209,40 @@ __device__ __forceinline__ float lp_scalars(const LpArgs& a, int row, float m, f
     return lz;
 }
 
-__device__ __forceinline__ void lp_put(const LpArgs& a, int row, int rank, uint64_t key, float m, float lz)
+__device__ __forceinline__ float lp_first(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
+
+/* (m, z, h) over the wave: the first lane's, since the compiler fuses a
+ * product here into the first addition and the lanes' sums then differ in the
+ * last bit -- and which thread writes an entry differs from run to run */
+__device__ __forceinline__ void lp_wave(float& m, float& z, float& h)
 {
-    a.top_id[(int64_t)row * a.top + rank] = (int)~(uint32_t)key;
-    a.top_logprob[(int64_t)row * a.top + rank] = lp_value(key) - m - lz;
+    const float M = lg_group_max<64>(m), d = fmaxf(m - M, -1e30f), al = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+    h = lp_first(lg_group_sum<64>(al * __builtin_fmaf(z, d, h)));
+    z = lp_first(lg_group_sum<64>(z * al));
+    m = lp_first(M);
 }
 
-/* One read of the logits: a workgroup takes a row or a part of one, a thread
+/* One read of the logits: a workgroup takes a row, a thread
  * 16 values at a time with a maximum, a sum and a weighted sum of its own.
  * e^x as 2^(x log2 e) with the maximum taken off before the product, so that
  * the largest term is 1 to the last bit and log z has no error of log2 e's
  * rounding times the maximum. */
-__global__ __launch_bounds__(LP_T) void k_logp(LpArgs a)
+template <int T>
+__global__ __launch_bounds__(T) void k_logp(LpArgs a)
 {
     __shared__ LpShared s;
-    const int row = blockIdx.x / a.nsplit, sp = blockIdx.x % a.nsplit;
+    const int row = blockIdx.x, t = threadIdx.x;
     const LpRow r(a.logits + row * a.stride, a.vocab);
-    const int64_t nq = r.quads();
-    const int q0 = (int)(nq * sp / a.nsplit), q1 = (int)(nq * (sp + 1) / a.nsplit);
+    const int nq = r.quads();
     float m = -FLT_MAX, z = 0.0f, h = 0.0f, mine = -INFINITY;
-    for (int q = q0 + threadIdx.x; q < q1; q += 4 * LP_T) {
+    auto take = [&](const float4 (&v)[4]) __attribute__((always_inline)) {
         float x[16];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int at = q + j * LP_T;
-            const float4 v = at < q1 ? r.load(at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            x[4 * j] = v.x;
-            x[4 * j + 1] = v.y;
-            x[4 * j + 2] = v.z;
-            x[4 * j + 3] = v.w;
+            x[4 * j] = v[j].x;
+            x[4 * j + 1] = v[j].y;
+            x[4 * j + 2] = v[j].z;
+            x[4 * j + 3] = v[j].w;
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) mine = fmaxf(mine, x[i]);
@@ -243,78 +259,69 @@ __global__ __launch_bounds__(LP_T) void k_logp(LpArgs a)
         }
         z += zs;
         h += hs;
+    };
+    /* whole blocks of 4 T quads, the next one on its way; what is left, quad by
+     * quad; the first quad of a row that is not aligned, which no thread counts
+     * among its own */
+    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const int off = r.sh ? 1 : 0, full = (a.vocab + r.sh) / 4;
+    int q = off;
+    float4 v[4];
+    if (q + 4 * T <= full) {
+        const float4* const p = (const float4*)(r.x - r.sh) + t;
+        float4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = p[q + j * T];
+        for (; q + 4 * T <= full; q += 4 * T) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = w[j];
+            if (q + 8 * T <= full)
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = p[q + (4 + j) * T];
+            take(v);
+        }
     }
-    float M = lg_group_max<64>(m);
-    if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = M;
+    for (; q < nq; q += 4 * T) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int at = q + t + j * T;
+            v[j] = at < nq ? r.load(at) : none;
+        }
+        take(v);
+    }
+    const uint32_t ord = lp_ord(mine);
+    if (off) {
+        v[0] = t == 0 ? r.load(0) : none;
+        v[1] = v[2] = v[3] = none;
+        take(v);
+    }
+    {   /* of T / 256 neighbours */
+        uint32_t o = ord;
+        if constexpr (T >= 512) o = max(o, (uint32_t)lg_partner<0>((int)o));
+        if constexpr (T >= 1024) o = max(o, (uint32_t)lg_partner<1>((int)o));
+        if (t % (T / 256) == 0) s.top[t / (T / 256)] = o;
+    }
+    lp_wave(m, z, h);
+    if (t % 64 == 0) s.sums[t / 64] = make_float4(m, z, h, 0.0f);
     __syncthreads();
-    M = fmaxf(fmaxf(s.red[0], s.red[1]), fmaxf(s.red[2], s.red[3]));
-    const float d0 = fmaxf(m - M, -1e30f), al = __builtin_amdgcn_exp2f(d0 * LP_LOG2E);
-    h = lg_block_sum(al * __builtin_fmaf(z, d0, h), s.red);
-    z = lg_block_sum(z * al, s.red);
-    __syncthreads();
-    const bool whole = a.nsplit == 1;
-    float lz = 0.0f;
-    if (whole) lz = lp_scalars(a, row, M, z, h);
-    else if (threadIdx.x == 0) a.sums[blockIdx.x] = make_float4(M, z, h, 0.0f);
+    {
+        const float4 v = t % 64 < T / 64 ? s.sums[t % 64] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
+        m = v.x;
+        z = v.y;
+        h = v.z;
+        lp_wave(m, z, h);
+    }
+    const float lz = lp_scalars(a, row, m, z, h);
     if (!a.top) return;
-    const int n = lp_top(s, r, q0, q1, a.top, mine, z != z);
-    lp_emit(s, n, a.top, [&](int rank, uint64_t k) {
-        if (whole) lp_put(a, row, rank, k, M, lz);
-        else a.keys[(int64_t)blockIdx.x * a.top + rank] = k;
+    const int n = lp_top<T>(s, r, nq, off, a.top, ord, z != z);
+    lp_emit<T>(s, n, a.top, [&](int rank, uint64_t k) {
+        a.top_id[(int64_t)row * a.top + rank] = (int)~(uint32_t)k;
+        a.top_logprob[(int64_t)row * a.top + rank] = lp_value(k) - m - lz;
     });
 }
 
-/* The parts of a row.  Every part has `top` keys in order, so at least `top` keys reach the largest of
- * the parts' last ones, and the least of the parts' (ceil(top / parts))-th
- * ones: the larger bound leaves few to rank. */
-__global__ __launch_bounds__(LP_T) void k_logp_join(LpArgs a)
-{
-    __shared__ LpShared s;
-    const int row = blockIdx.x, t = threadIdx.x, ns = a.nsplit, top = a.top;
-    const float4* const p = a.sums + (int64_t)row * ns;
-    float M = -FLT_MAX, z = 0.0f, h = 0.0f;
-    for (int i = 0; i < ns; i++) M = fmaxf(M, p[i].x);
-    for (int i = 0; i < ns; i++) {
-        const float d0 = fmaxf(p[i].x - M, -1e30f), al = __builtin_amdgcn_exp2f(d0 * LP_LOG2E);
-        h += al * __builtin_fmaf(p[i].y, d0, p[i].z);
-        z = __builtin_fmaf(p[i].y, al, z);
-    }
-    const float lz = lp_scalars(a, row, M, z, h);
-    if (!top) return;
-    const uint64_t* const keys = a.keys + (int64_t)row * ns * top;
-    const int deep = (top + ns - 1) / ns - 1;
-    uint64_t b0 = 0, b1 = ~0ull;
-    for (int i = 0; i < ns; i++) {
-        const uint64_t x = keys[i * top + top - 1], y = keys[i * top + deep];
-        b0 = x > b0 ? x : b0;
-        b1 = y < b1 ? y : b1;
-    }
-    const uint64_t bound = b0 > b1 ? b0 : b1;
-    if (t == 0) s.n = 0;
-    __syncthreads();
-    for (int i = t; i < ns * top; i += LP_T)
-        if (keys[i] >= bound) s.list[atomicAdd(&s.n, 1)] = keys[i];
-    __syncthreads();
-    lp_emit(s, s.n, top, [&](int rank, uint64_t k) { lp_put(a, row, rank, k, M, lz); });
-}
-
-/* parts of a row: some eight workgroups a CU in all, parts of at least 4096
- * logits, and no more keys than the join's list holds */
-static int lp_split(int64_t rows, int vocab)
-{
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2048 / rows, vocab / 4096, LP_CAP / LG_LOGPROBS_TOP}));
-}
-
-extern "C" size_t lg_logprobs_workspace_size(int rows, int vocab, int top)
-{
-    if (rows <= 0 || vocab <= 0 || top < 0) return 0;
-    const int ns = lp_split(rows, vocab);
-    return ns > 1 ? (size_t)rows * ns * (16 + 8 * (size_t)top) : 0;
-}
-
 extern "C" int lg_logprobs(const float* logits, int64_t stride, int rows, int vocab, const int* toks, int top,
-                           float* logprob, float* entropy, int* top_id, float* top_logprob, void* workspace,
-                           size_t workspace_bytes, void* stream)
+                           float* logprob, float* entropy, int* top_id, float* top_logprob, void* stream)
 {
     const char* who = "lg_logprobs";
     if ((rows && !logits) || ((uintptr_t)logits & 3) || rows < 0 || vocab <= 0 || vocab > INT32_MAX - 16 || stride < vocab ||
@@ -327,18 +334,14 @@ extern "C" int lg_logprobs(const float* logits, int64_t stride, int rows, int vo
         lg_set_error("%s: tokens and their log probabilities, ids and log probabilities of the top go together", who);
         return LG_ERR_ARG;
     }
-    LpArgs a = {logits, stride, rows, vocab, top, lp_split(rows, vocab), toks, logprob, entropy, top_logprob, top_id,
-                nullptr, nullptr};
-    const size_t need = lg_logprobs_workspace_size(rows, vocab, top);
-    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) {
-        lg_set_error("%s: workspace of %zu bytes, 16-byte aligned, %zu needed", who, workspace_bytes, need);
-        return LG_ERR_ARG;
-    }
-    if (need) {
-        a.sums = (float4*)workspace;
-        a.keys = (uint64_t*)(a.sums + (size_t)rows * a.nsplit);
-    }
-    k_logp<<<(unsigned)rows * a.nsplit, LP_T, 0, (hipStream_t)stream>>>(a);
-    if (a.nsplit > 1) k_logp_join<<<rows, LP_T, 0, (hipStream_t)stream>>>(a);
+    const LpArgs a = {logits, stride, vocab, top, toks, logprob, entropy, top_logprob, top_id};
+    /* A workgroup has a row to itself.  1024 threads, and two of them a CU; of
+     * many short rows more at a time, with 256 threads each: 700 rows of 4000,
+     * top 20, 6 us against 14, of 32000 21 against 23, of 50000 32 against 30;
+     * 256 of 16000 11 against 8.  Rows in parts of 4096 logits and a second
+     * launch to join them were faster for one row of 151936 only (11 us against
+     * 16, without the host's time for that launch; 32000 logits 9 against 8). */
+    if (rows > 512 && vocab <= 32768) k_logp<256><<<rows, 256, 0, (hipStream_t)stream>>>(a);
+    else k_logp<1024><<<rows, 1024, 0, (hipStream_t)stream>>>(a);
     return lg_check_launch(who);
 }

@@ -128,9 +128,7 @@ SIGNATURES = {
     "lg_attn_cache_workspace_size": (C.c_size_t, [C.c_int] * 8),
     "lg_attn_cache": (C.c_int, [_vp, C.c_int64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
                                 C.c_int64, _vp, C.c_size_t, _vp]),
-    "lg_logprobs_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
-    "lg_logprobs": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_size_t,
-                              _vp]),
+    "lg_logprobs": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp]),
     "lg_bert_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "lg_bert_destroy": (C.c_int, [_vp]),
     "lg_bert_last_error": (C.c_char_p, [_vp]),

@@ -294,7 +294,7 @@ class Logprobs(NamedTuple):
     top_logprob: torch.Tensor
 
 
-def logprobs(logits, toks=None, top: int = 0, workspace=None) -> Logprobs:
+def logprobs(logits, toks=None, top: int = 0) -> Logprobs:
     """lg_logprobs of logits [rows, vocab] (dense rows) and int32 toks [rows]."""
     if logits.dtype is not _FP32 or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         _refuse("logits: dense fp32 rows on the GPU wanted")
@@ -310,10 +310,8 @@ def logprobs(logits, toks=None, top: int = 0, workspace=None) -> Logprobs:
     if top:
         top_lp = new((rows, top))
         top_id = torch.empty_like(top_lp, dtype=_INT32)
-    lib = load()
-    workspace, ws = _work(lib.lg_logprobs_workspace_size(rows, vocab, top), workspace, logits)
-    _on(i, lib.lg_logprobs, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, pt, top, pl, entropy.data_ptr(),
-        top_id.data_ptr() if top else None, top_lp.data_ptr() if top else None, *ws)
+    _on(i, load().lg_logprobs, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, pt, top, pl, entropy.data_ptr(),
+        top_id.data_ptr() if top else None, top_lp.data_ptr() if top else None)
     return Logprobs(lp, entropy, top_id, top_lp)
 
 

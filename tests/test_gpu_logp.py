@@ -57,7 +57,8 @@ def check(gpu, x, toks, top, wide=None):
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 31), (2, 64), (1, 1000), (5, 1023), (2, 2049), (1, 32000), (40, 5000),
-                                        (3, 50257), (1, 151936), (300, 4097), (700, 600)])
+                                        (3, 50257), (1, 151936), (300, 4097), (700, 600), (3, 16389),
+                                        (520, 9001), (2, 40001)])
 @pytest.mark.parametrize("top", [0, 1, 5, 20, 32])
 def test_rows(gpu, rows, vocab, top):
     print(f"logprobs: {rows} x {vocab} top {top}", flush=True)
@@ -157,6 +158,17 @@ def test_captured_calls(gpu, rows, vocab):
         want = ops.logprobs(x, toks, top=7)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(r, want))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 31000), (60, 3000), (2, 151936), (300, 5000)])
+def test_same_results_every_time(gpu, rows, vocab):
+    """Which thread writes an entry depends on the order of LDS atomics; what it writes does not."""
+    import torch
+    from ligguf_amd import ops
+    x, toks = torch.randn(rows, vocab, device=gpu), torch.zeros(rows, dtype=torch.int32, device=gpu)
+    a = ops.logprobs(x, toks, top=20)
+    for _ in range(20):
+        assert all(torch.equal(p, q) for p, q in zip(ops.logprobs(x, toks, top=20), a))
 
 
 def test_python_refusals(gpu):

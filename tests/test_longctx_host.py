@@ -33,8 +33,8 @@ def test_no_rows_is_no_work():
     assert attn(nseq=0) == 0 and attn(ntok=0) == 0 and logp(rows=0) == 0
 
 
-def logp(x=P, stride=100, rows=2, vocab=100, toks=P, top=3, lp=P, ent=P, ids=P, tl=P, ws=P, wb=1 << 30):
-    return L.load().lg_logprobs(x, stride, rows, vocab, toks, top, lp, ent, ids, tl, ws, wb, None)
+def logp(x=P, stride=100, rows=2, vocab=100, toks=P, top=3, lp=P, ent=P, ids=P, tl=P):
+    return L.load().lg_logprobs(x, stride, rows, vocab, toks, top, lp, ent, ids, tl, None)
 
 
 @pytest.mark.parametrize("kw", [
