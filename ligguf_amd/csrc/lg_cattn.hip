@@ -545,36 +545,44 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
         v8h qh[NJ], ql[NJ];
         float sc;
         {
-            float x[NJ][8], big = 0.0f;
+            /* queries, first keys and first values on their way together */
+            v4f x[2 * NJ];
             const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * h;
 #pragma unroll
-            for (int j = 0; j < NJ; j++)
+            for (int j = 0; j < 2 * NJ; j++) x[j] = idx < ncol ? *(const v4f*)(q + 16 * (j / 2) + 4 * (j % 2)) : (v4f){};
+            CaPieces<HD, KV4> V0;
+            const int k0 = tiles.at(t0) * KT;
+            if (t0 < t1) {
+                P.load(a, kc, g, k0);
+                V0.load(a, vc, g, k0);
+            }
+            float big = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const v4f y = idx < ncol ? *(const v4f*)(q + 16 * j + e) : (v4f){};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        x[j][e + i] = y[i];
-                        big = fmaxf(big, fabsf(y[i]));
-                    }
-                }
+            for (int j = 0; j < 2 * NJ; j++)
+                big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
             big = fmaxf(big, lg_partner<5>(big));
             const int ex = __builtin_amdgcn_frexp_expf(big);
             sc = ldexpf(a.scale2, ex - 14);
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) ca_split2(ldexpf(x[j][e], 14 - ex), ldexpf(x[j][e + 1], 14 - ex), qh[j], ql[j], e);
+                for (int e = 0; e < 8; e += 2)
+                    ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j], ql[j], e);
+            if (t0 < t1) {
+                P.template store<C::KST>(s_kv, nullptr);
+                V0.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax) ? s_bad[0] : nullptr);
+            }
         }
+        __syncthreads();
         float m = -0x1p40f, cc = __builtin_fmaf(-m, sc, 14.0f);
-        for (int it = t0 - 1; it < t1; it++) {
+        for (int it = t0; it < t1; it++) {
             const bool more = it + 1 < t1;
-            const int kb = tiles.at(max(it, t0)) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
-            const int cur = (it - t0) & 1, nxt = cur ^ 1, slot = (it - t0 + 3) % 3;
+            const int kb = tiles.at(it) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
+            const int cur = (it - t0) & 1, nxt = cur ^ 1, slot = (it - t0) % 3;
             _Float16* const sK = s_kv + cur * C::STAGE;
             _Float16* const sV = sK + KT * C::KST;
             _Float16* const nK = s_kv + nxt * C::STAGE;
-            const bool on = it >= t0 && kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
+            const bool on = kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
             if (more) P.load(a, kc, g, kn);
             v16f s[NK];
             if (on) {
