@@ -541,7 +541,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
         auto partly = [&](int kb, int lo, int hi) {
             return kb + KT - 1 > lo || (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
         };
-        CaPieces<HD, KV4> P;
+        CaPieces<HD, KV4> P, V;
         v8h qh[NJ], ql[NJ];
         float sc;
         {
@@ -550,11 +550,10 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * h;
 #pragma unroll
             for (int j = 0; j < 2 * NJ; j++) x[j] = idx < ncol ? *(const v4f*)(q + 16 * (j / 2) + 4 * (j % 2)) : (v4f){};
-            CaPieces<HD, KV4> V0;
             const int k0 = tiles.at(t0) * KT;
             if (t0 < t1) {
                 P.load(a, kc, g, k0);
-                V0.load(a, vc, g, k0);
+                V.load(a, vc, g, k0);
             }
             float big = 0.0f;
 #pragma unroll
@@ -570,7 +569,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                     ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j], ql[j], e);
             if (t0 < t1) {
                 P.template store<C::KST>(s_kv, nullptr);
-                V0.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax) ? s_bad[0] : nullptr);
+                V.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax) ? s_bad[0] : nullptr);
             }
         }
         __syncthreads();
@@ -583,7 +582,10 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             _Float16* const sV = sK + KT * C::KST;
             _Float16* const nK = s_kv + nxt * C::STAGE;
             const bool on = kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
-            if (more) P.load(a, kc, g, kn);
+            if (more) {
+                P.load(a, kc, g, kn);
+                V.load(a, vc, g, kn);
+            }
             v16f s[NK];
             if (on) {
                 __builtin_amdgcn_s_setprio(1);   /* its products ahead of the other wave's softmax: 700 x 9000 251 -> 243 us */
@@ -601,7 +603,6 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             __builtin_amdgcn_s_setprio(0);
             if (more) {
                 P.template store<C::KST>(nK, nullptr);
-                P.load(a, vc, g, kn);
             }
             if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
             if (on) {
@@ -665,7 +666,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                                 }
                     }
             }
-            if (more) P.template store<C::VST>(nK + KT * C::KST, partly(kn, pmin, pmax) ? s_bad[(slot + 1) % 3] : nullptr);
+            if (more) V.template store<C::VST>(nK + KT * C::KST, partly(kn, pmin, pmax) ? s_bad[(slot + 1) % 3] : nullptr);
             __syncthreads();
         }
         l += lg_partner<5>(l);
