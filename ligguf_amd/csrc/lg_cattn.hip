@@ -113,6 +113,8 @@ struct CaTiles {
     __device__ __forceinline__ int at(int i) const { return i < first ? i : lo + i - first; }
 };
 
+constexpr int CA_PARTS = 512;   /* at most */
+
 /* Partials of a split call: [split][row][head] sums, then (maximum, sum of
  * weights) of each; a part without keys has weight 0 and no sums. */
 __device__ __forceinline__ float2& ca_part_ml(const CAttn& a, int nsplit, float* part, int hd, int64_t at)
@@ -687,49 +689,81 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
     if (part && h == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(mx, l);
 }
 
-/* the splits' parts of a row's head: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M),
- * a thread per four dims.  G threads share them where there are many parts and
- * few rows: one thread alone waits for one load after the other (64 parts of 32
- * heads: 34 us; 3.x with eight). */
-template <int G>
+/* the splits' parts of a row's head: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M) */
+/* few parts: a thread per four dims */
 __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const float* __restrict__ part)
 {
-    __shared__ v4f s_y[G > 1 ? 256 : 1];
-    __shared__ float s_l[G > 1 ? 256 : 1];
-    const int hd = a.c.hd, dq = hd / 4, per = 256 / G;
-    const int64_t i = (int64_t)blockIdx.x * per + threadIdx.x % per, n = (int64_t)a.rows * a.n_heads;
-    const int64_t at = min(i / dq, n - 1), row = at / a.n_heads;
-    const int d = (int)(i % dq) * 4, head = (int)(at % a.n_heads), p = a.pos[row], grp = threadIdx.x / per;
+    const int hd = a.c.hd, dq = hd / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.rows * a.n_heads;
+    if (i >= n * dq) return;
+    const int64_t at = i / dq, row = at / a.n_heads;
+    const int d = (int)(i % dq) * 4, head = (int)(at % a.n_heads), p = a.pos[row];
     const float2* const ml = (const float2*)(part + nsplit * n * hd);
     v4f y = {};
     float L = 0.0f;
     if (p >= 0 && p <= a.max_pos) {
         float M = -INFINITY;
-#pragma unroll 4
         for (int s = 0; s < nsplit; s++) M = fmaxf(M, ml[s * n + at].x);
-#pragma unroll 2
-        for (int s = grp; s < nsplit; s += G) {
+        for (int s = 0; s < nsplit; s++) {
             const float2 x = ml[s * n + at];
-            const bool some = x.y != 0.0f;
-            const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
-            const v4f v = some ? *(const v4f*)(part + (s * n + at) * hd + d) : (v4f){};
+            if (x.y == 0.0f) continue;   /* (no keys, no sums written) */
+            const float f = __builtin_amdgcn_exp2f(x.x - M);
+            const v4f v = *(const v4f*)(part + (s * n + at) * hd + d);
             L = __builtin_fmaf(x.y, f, L);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
         }
     }
-    if constexpr (G > 1) {
-        s_y[threadIdx.x] = y;
-        s_l[threadIdx.x] = L;
-        __syncthreads();
-        if (grp) return;
+    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = y * (L == 0.0f ? 0.0f : 1.0f / L);
+}
+
+/* many parts of few rows: a workgroup per row's head, the weights by one wave,
+ * the sums by groups of hd / 4 threads -- a thread that walks over the parts
+ * waits for one load after the other (64 parts of 32 heads: 34 us) */
+__global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, const float* __restrict__ part)
+{
+    __shared__ float s_f[CA_PARTS], s_l;
+    __shared__ v4f s_y[256];
+    const int hd = a.c.hd, dq = hd / 4, grp = threadIdx.x / dq, ng = 256 / dq, d = threadIdx.x % dq * 4;
+    const int64_t at = blockIdx.x, n = (int64_t)a.rows * a.n_heads, row = at / a.n_heads;
+    const int head = (int)(at % a.n_heads), p = a.pos[row];
+    const float2* const ml = (const float2*)(part + nsplit * n * hd);
+    if (threadIdx.x < 64) {
+        float2 x[CA_PARTS / 64];
+        float M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int k = 1; k < G; k++) {
-            y += s_y[threadIdx.x + k * per];
-            L += s_l[threadIdx.x + k * per];
+        for (int k = 0; k < CA_PARTS / 64; k++) {
+            const int s = threadIdx.x + 64 * k;
+            x[k] = s < nsplit ? ml[s * n + at] : make_float2(-INFINITY, 0.0f);
+            M = fmaxf(M, x[k].x);
         }
+        M = lg_group_max<64>(M);
+#pragma unroll
+        for (int k = 0; k < CA_PARTS / 64; k++) {
+            const float f = x[k].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[k].x - M);
+            s_f[threadIdx.x + 64 * k] = f;
+            L = __builtin_fmaf(x[k].y, f, L);
+        }
+        L = lg_group_sum<64>(L);
+        if (threadIdx.x == 0) s_l = L;
     }
-    if (i < n * dq) *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = y * (L == 0.0f ? 0.0f : 1.0f / L);
+    __syncthreads();
+    v4f y = {};
+    if (grp < ng) {
+#pragma unroll 4
+        for (int s = grp; s < nsplit; s += ng) {
+            const float f = s_f[s];
+            const v4f v = f != 0.0f ? *(const v4f*)(part + (s * n + at) * hd + d) : (v4f){};   /* (no keys, no sums written) */
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
+        }
+        s_y[threadIdx.x] = y;
+    }
+    __syncthreads();
+    if (grp) return;
+    for (int k = 1; k < ng; k++) y += s_y[threadIdx.x + k * dq];
+    const float L = s_l;
+    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = p < 0 || p > a.max_pos || L == 0.0f ? (v4f){} : y * (1.0f / L);
 }
 
 /* How a call is cut, from its sizes alone. */
@@ -764,8 +798,8 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         if (!p.wide) {
             /* two workgroups a CU, each with at least a tile or two for each wave; chunks short enough to even
              * out ragged lengths */
-            p.nsplit = (int)std::max<int64_t>({1, std::min((kv4 ? 256 : 512) / groups, (keys + 255) / 256),
-                                               std::min<int64_t>(keys / (kv4 ? 2048 : 1024), 16384 / groups)});
+            p.nsplit = (int)std::max<int64_t>({1, std::min<int64_t>(512 / groups, (keys + 255) / 256),
+                                               std::min<int64_t>({keys / (kv4 ? 2048 : 1024), 16384 / groups, CA_PARTS})});
             p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
         }
     }
@@ -857,11 +891,10 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     default: ca_type<256>(a, p, nseq, part, s); break;
     }
     if (part) {
-        const int64_t n = rows * n_heads * (hd / 4);   /* threads of a group */
         if (p.nsplit > 8)
-            k_cattn_merge<8><<<(unsigned)((n + 31) / 32), 256, 0, s>>>(a, p.nsplit, part);
+            k_cattn_merge_wide<<<(unsigned)(rows * n_heads), 256, 0, s>>>(a, p.nsplit, part);
         else
-            k_cattn_merge<1><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
+            k_cattn_merge<<<(unsigned)((rows * n_heads * (hd / 4) + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
     }
     return lg_check_launch(who);
 }
