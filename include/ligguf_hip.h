@@ -480,8 +480,8 @@ int lg_kv4_read(const lg_kv_cache* cache, int nseq, int pos0, int npos, uint16_t
  * device memory, 16-byte aligned (NULL when that is 0), which nothing else may
  * use until the call is done: calls that may overlap, replays of captured
  * ones included, need one each. */
-size_t lg_attn_cache_workspace_size(int nseq, int ntok, int n_heads, int n_kv_heads, int head_dim, int window,
-                                    int sinks, int max_pos);
+size_t lg_attn_cache_workspace_size(const lg_kv_cache* cache, int nseq, int ntok, int n_heads, int window, int sinks,
+                                    int max_pos);
 int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache* cache, const int* pos, int nseq, int ntok,
                   int n_heads, int window, int sinks, int max_pos, float* out, int64_t out_stride, void* workspace,
                   size_t workspace_bytes, void* stream);

@@ -775,9 +775,6 @@ struct CaPlan {
     size_t ws;
 };
 
-/* keys a wave takes at a time (CaDec) */
-static int CA_KT(int hd, bool kv4) { return kv4 && hd <= 128 ? 64 : 32; }
-
 static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos,
                       bool kv4)
 {
@@ -792,12 +789,19 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         p.ncb = (int)((cols + width - 1) / width);
         p.nsplit = (int)std::max<int64_t>(1, std::min(256 / (nseq * n_kv * p.ncb), keys / 512));
     } else {
+        /* Short contexts: eight waves and no second launch.  32 heads of 128, 8
+         * key heads, us of the GPU, one launch / split and joined: fp16 512 keys
+         * 11.3 / 11.0 (and the host's 3 for a launch), 1024 18.3 / 12.4, but of 32
+         * sequences 26 / 29; 4 bits 512 8.4 / 9.9, 1024 11.7 / 11.4.
+         * Else two workgroups a CU, each with some 256 keys at least; and
+         * chunks short enough to even out ragged lengths: 24 sequences of up
+         * to 12000 fp16 rows 133 us with 1024 keys, 148 with 2048, 186 with the
+         * lengths halved; 40 of up to 8208 rows in 4 bits 148 with 512, 117
+         * with 1024, 106 with 2048, 121 with 4096. */
         const int64_t groups = nseq * n_kv;
-        const int kt = CA_KT(hd, kv4);
-        p.wide = hd <= 128 && keys <= 1024 && groups <= 256;
+        const int kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec) */
+        p.wide = hd <= 128 && groups <= 256 && keys <= (kv4 || groups >= 128 ? 1024 : 512);
         if (!p.wide) {
-            /* two workgroups a CU, each with at least a tile or two for each wave; chunks short enough to even
-             * out ragged lengths */
             p.nsplit = (int)std::max<int64_t>({1, std::min<int64_t>(512 / groups, (keys + 255) / 256),
                                                std::min<int64_t>({keys / (kv4 ? 2048 : 1024), 16384 / groups, CA_PARTS})});
             p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
@@ -807,12 +811,13 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
     return p;
 }
 
-extern "C" size_t lg_attn_cache_workspace_size(int nseq, int ntok, int n_heads, int n_kv_heads, int head_dim, int window,
-                                               int sinks, int max_pos)
+extern "C" size_t lg_attn_cache_workspace_size(const lg_kv_cache* cache, int nseq, int ntok, int n_heads, int window, int sinks,
+                                               int max_pos)
 {
-    if (nseq <= 0 || ntok <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_pos < 0) return 0;
-    return std::max(ca_plan(nseq, ntok, n_heads, n_kv_heads, head_dim, window, sinks, max_pos, false).ws,
-                    ca_plan(nseq, ntok, n_heads, n_kv_heads, head_dim, window, sinks, max_pos, true).ws);
+    if (!cache || cache->n_kv_heads <= 0 || cache->head_dim <= 0 || nseq <= 0 || ntok <= 0 || n_heads <= 0 || window < 0 ||
+        sinks < 0 || max_pos < 0)
+        return 0;
+    return ca_plan(nseq, ntok, n_heads, cache->n_kv_heads, cache->head_dim, window, sinks, max_pos, cache->type == LG_KV4).ws;
 }
 
 template <int HD, bool KV4>

@@ -125,7 +125,7 @@ SIGNATURES = {
                                          _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_float,
                                          C.c_float, _vp, C.c_int, C.c_int, _vp, _vp]),
     "lg_kv4_read": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]),
-    "lg_attn_cache_workspace_size": (C.c_size_t, [C.c_int] * 8),
+    "lg_attn_cache_workspace_size": (C.c_size_t, [_vp] + [C.c_int] * 6),
     "lg_attn_cache": (C.c_int, [_vp, C.c_int64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
                                 C.c_int64, _vp, C.c_size_t, _vp]),
     "lg_logprobs": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp]),

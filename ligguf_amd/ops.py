@@ -280,9 +280,9 @@ def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max
     rows = _rows(q, i, nseq, ntok, width, "q")
     if out is None:
         out = q.new_empty((nseq, ntok, width))
-    lib = load()
-    workspace, ws = _work(lib.lg_attn_cache_workspace_size(nseq, ntok, heads, cache.n_kv_heads, hd, window, sinks, max_pos), workspace, q)
-    _on(i, lib.lg_attn_cache, *rows, C.byref(cache.desc), p, nseq, ntok, heads, window, sinks, max_pos,
+    lib, desc = load(), C.byref(cache.desc)
+    workspace, ws = _work(lib.lg_attn_cache_workspace_size(desc, nseq, ntok, heads, window, sinks, max_pos), workspace, q)
+    _on(i, lib.lg_attn_cache, *rows, desc, p, nseq, ntok, heads, window, sinks, max_pos,
         *_rows(out, i, nseq, ntok, width, "out"), *ws)
     return out
 

@@ -300,7 +300,7 @@ def test_workspace_must_hold_the_partials(gpu):
     lib = L.load()
     cache = ops.KvCache.empty(ops.F16, 9000, 2, 64, 1, gpu)
     q, pos = torch.zeros(1, 1, 256, device=gpu), torch.full((1, 1), 8999, dtype=torch.int32, device=gpu)
-    need = lib.lg_attn_cache_workspace_size(1, 1, 4, 2, 64, 0, 0, 8999)
+    need = lib.lg_attn_cache_workspace_size(C.byref(cache.desc), 1, 1, 4, 0, 0, 8999)
     assert need > 0
     ops.attention_cache(q, cache, pos, workspace=torch.empty(need, dtype=torch.uint8, device=gpu))
     for ws in (torch.empty(need - 1, dtype=torch.uint8, device=gpu), torch.empty(need + 8, dtype=torch.uint8, device=gpu)[8:]):

@@ -29,6 +29,18 @@ def test_attention_refuses_an_unknown_cache_type():
     assert L.load().lg_attn_cache(P, 256, None, P, 1, 1, 4, 0, 0, 31, P, 256, P, 1 << 20, None) == -1
 
 
+def test_attention_refuses_a_workspace_too_small():
+    c = cache(n_ctx=9000)
+    need = L.load().lg_attn_cache_workspace_size(C.byref(c), 1, 1, 4, 0, 0, 8999)
+    assert need > 0
+    for ws, wb in ((None, need), (P, need - 1), (P + 8, need)):
+        assert attn(c=c, max_pos=8999, ws=ws, wb=wb) == -1
+    # sizes that no call takes need none
+    for a in ((0, 1, 4, 0, 0, 8999), (1, -1, 4, 0, 0, 8999), (1, 1, 0, 0, 0, 8999), (1, 1, 4, -1, 0, 8999), (1, 1, 4, 0, 0, -1)):
+        assert L.load().lg_attn_cache_workspace_size(C.byref(c), *a) == 0
+    assert L.load().lg_attn_cache_workspace_size(None, 1, 1, 4, 0, 0, 8999) == 0
+
+
 def test_no_rows_is_no_work():
     assert attn(nseq=0) == 0 and attn(ntok=0) == 0 and logp(rows=0) == 0
 
