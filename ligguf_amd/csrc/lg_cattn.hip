@@ -34,7 +34,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void ca_split2(float x0, float x1, v8h& hi, v8h& lo, int i)
 {
     const lg_h2 x = __builtin_convertvector(((lg_f2){x0, x1}), lg_h2);
-    const lg_h2 y = __builtin_convertvector(((lg_f2){__builtin_fmaf((float)x[0], -1.0f, x0), __builtin_fmaf((float)x[1], -1.0f, x1)}), lg_h2);
+    const lg_h2 y = __builtin_convertvector(((lg_f2){x0 - (float)x[0], x1 - (float)x[1]}), lg_h2);
     hi[i] = x[0];
     hi[i + 1] = x[1];
     lo[i] = y[0];
@@ -787,7 +787,22 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
     if (!p.dec) {
         const int64_t width = hd <= 128 ? 256 : 128;
         p.ncb = (int)((cols + width - 1) / width);
-        p.nsplit = (int)std::max<int64_t>(1, std::min(256 / (nseq * n_kv * p.ncb), keys / 512));
+        /* Parts of the keys: whole rounds of 256 workgroups (one a CU), each as
+         * long as its tiles and, measured, some four more for its start and end;
+         * joined parts are written and read once, about 14 MB in a tile's
+         * time.  700 rows over 9000 keys (88 workgroups, us): 1 part 428, 2
+         * 234, 3 321, 4 259, 5 220, 6 280, 8 232. */
+        const int64_t wgs = nseq * n_kv * p.ncb, kt = hd <= 128 ? 64 : 32;
+        const double tiles = (double)((window > 0 ? keys : std::max<int64_t>(1, keys - ntok / 2)) + kt - 1) / kt;
+        double best = 0.0;
+        for (int ns = 1; ns <= 64 && (ns == 1 || tiles / ns >= 4.0); ns++) {
+            double cost = (double)((wgs * ns + 255) / 256) * (tiles / ns + 4.0);
+            if (ns > 1) cost += 1.5 + 8e-6 / 14.0 * ns * (double)(nseq * ntok) * n_heads * hd;
+            if (ns == 1 || cost < best) {
+                best = cost;
+                p.nsplit = ns;
+            }
+        }
     } else {
         /* Short contexts: eight waves and no second launch.  32 heads of 128, 8
          * key heads, us of the GPU, one launch / split and joined: fp16 512 keys

@@ -21,7 +21,7 @@ import numpy as np
 from . import encode
 from .gguf import GARRAY, GFLOAT32, GSTRING, GUINT32, read_gguf, write_gguf
 from .lib import (ARCH_LLAMA, ARCH_QWEN3, BLOCK, F32, Q1_0, Q1_G, Q4_K, Q6_K, Q8_0, LgLayerDesc, LgModelDesc,
-                  LgWeight, check, load, row_size)
+                  LgError, LgWeight, check, load, row_size)
 
 
 @dataclass(frozen=True)
@@ -289,6 +289,7 @@ class Engine:
         self.lib = load()
         self.ctx = C.c_void_p()
         check(self.lib.lg_create(device, C.byref(self.ctx)))
+        self.device = device
         self.vocab = 0
         self.cfg = None
 
@@ -321,6 +322,25 @@ class Engine:
             return out
         check(self.lib.lg_decode_step(self.ctx, tok, pos, None), self.ctx)
         return None
+
+    def logprobs(self, tok: int, top: int = 0):
+        """lg_logprobs of the last step's logits, on the device: log probability
+        of token tok, entropy, and the `top` alternatives as (id, log
+        probability).  Device memory from torch."""
+        import torch
+
+        from . import ops
+        if not self.vocab:
+            raise LgError("LG_ERR_STATE: no model loaded")
+        check(self.lib.lg_sync(self.ctx), self.ctx)      # the step runs on the context's stream
+        n = self.vocab
+        view = type("Logits", (), {"__cuda_array_interface__": {
+            "shape": (1, n), "typestr": "<f4", "data": (self.lib.lg_logits_device(self.ctx), False), "version": 2}})()
+        dev = torch.device("cuda", self.device)
+        with torch.cuda.device(dev):
+            r = ops.logprobs(torch.as_tensor(view, device=dev), torch.tensor([tok], dtype=torch.int32, device=dev), top=top)
+            alts = list(zip(r.top_id[0].tolist(), r.top_logprob[0].tolist())) if top else []
+            return float(r.logprob[0]), float(r.entropy[0]), alts
 
     def decode_traced(self, tok: int, pos: int):
         """lg_decode_step with lg_trace_acts_next_step: (logits, [4L+1][stride]

@@ -194,6 +194,51 @@ def test_visible_key_nan_makes_its_rows_nan(gpu):
         assert np.isnan(got[0, :, :2]).all() and np.isfinite(got[0, :, 2:]).all()
 
 
+@pytest.mark.parametrize("ctype", TYPES)
+@pytest.mark.parametrize("ntok", [1, 4, 40])
+def test_queries_of_rows_without_a_token(gpu, ctype, ntok):
+    """NaN and infinities in the queries of idle rows stay there, and their outputs are zeros."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(4)
+    for n_ctx in (200, 2500):
+        cache, _ = make(gpu, ctype, 3, n_ctx, 2, 64, g)
+        q = torch.randn(3, ntok, 256, device=gpu)
+        pos = torch.from_numpy(g.integers(0, n_ctx, (3, ntok)).astype(np.int32)).to(gpu)
+        pos[1] = -1
+        pos[2, 0] = n_ctx
+        want = ops.attention_cache(q, cache, pos)
+        q[1] = float("nan")
+        q[2, 0] = float("inf")
+        got = ops.attention_cache(q, cache, pos)
+        assert torch.equal(got, want) and not got[1].any() and not got[2, 0].any()
+
+
+def test_visible_infinity_in_a_value(gpu):
+    """Where every row sees it, and far from any edge: its dim of every row that does is not finite,
+    the other dims are as without it."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(6)
+    for ntok in (1, 40):
+        cache, _ = make(gpu, L.F16, 1, 600, 1, 64, g)
+        q, pos = torch.randn(1, ntok, 128, device=gpu), torch.arange(600 - ntok, 600, dtype=torch.int32, device=gpu).view(1, -1)
+        want = ops.attention_cache(q, cache, pos)
+        cache.v[0, 70, 9] = float("inf")
+        got = ops.attention_cache(q, cache, pos)
+        bad = torch.zeros(64, dtype=torch.bool, device=gpu)
+        bad[9] = True
+        got, want = got.view(ntok, 2, 64), want.view(ntok, 2, 64)
+        assert not torch.isfinite(got[..., bad]).any() and torch.equal(got[..., ~bad], want[..., ~bad])
+
+
+def test_prompts_over_many_column_blocks_and_parts(gpu):
+    """Several blocks of columns, the last one cut, whole and with the keys in parts."""
+    check(gpu, L.F16, 4, 2, 64, 1, 333, 340, 0, 0, np.arange(7, 340))
+    check(gpu, L.KV4, 8, 1, 64, 1, 70, 5000, 0, 0, np.arange(4930, 5000))
+    check(gpu, L.F16, 2, 1, 256, 1, 150, 1300, 700, 5, np.arange(1150, 1300))
+
+
 def test_strided_rows_and_what_lies_between(gpu):
     import torch
     from ligguf_amd import ops

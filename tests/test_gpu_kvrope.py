@@ -252,6 +252,26 @@ def test_other_stream(gpu):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_one_norm_only_and_weights_on_any_boundary(gpu):
+    import torch
+    from ligguf_amd import ops
+    g = torch.Generator(device=gpu).manual_seed(8)
+    q, k = torch.randn(2, 7, 4 * 64, generator=g, device=gpu), torch.randn(2, 7, 2 * 64, generator=g, device=gpu)
+    w = torch.randn(65, generator=g, device=gpu)
+    pos = torch.arange(14, dtype=torch.int32, device=gpu).view(2, 7)
+    freq = ops.rope_table(64, 1e4)[0].to(gpu)
+    plain = ops.qk_norm_rope_tokens(q, k, None, pos, freq, 64, want_k=True)
+    both = ops.qk_norm_rope_tokens(q, k, None, pos, freq, 64, qw=w[:64].contiguous(), kw=w[1:].clone(), want_k=True)
+    a = ops.qk_norm_rope_tokens(q, k, None, pos, freq, 64, qw=w[:64], want_k=True)
+    b = ops.qk_norm_rope_tokens(q, k, None, pos, freq, 64, kw=w[1:].clone(), want_k=True)
+    assert torch.equal(a[0], both[0]) and torch.equal(a[1], plain[1])
+    assert torch.equal(b[0], plain[0]) and torch.equal(b[1], both[1])
+    # weights four bytes off a 16-byte boundary take the one-pair form: sums in another order
+    off = ops.qk_norm_rope_tokens(q, k, None, pos, freq, 64, qw=w[:64], kw=w[1:], want_k=True)
+    for x, y in zip(off, both):
+        assert float((x - y).abs().max()) <= 40 * U * float(y.abs().max())
+
+
 def test_no_rows(gpu):
     import torch
     from ligguf_amd import ops
