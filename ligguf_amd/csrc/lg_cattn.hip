@@ -805,19 +805,22 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         }
     } else {
         /* Short contexts: eight waves and no second launch.  32 heads of 128, 8
-         * key heads, us of the GPU, one launch / split and joined: fp16 512 keys
-         * 11.3 / 11.0 (and the host's 3 for a launch), 1024 18.3 / 12.4, but of 32
-         * sequences 26 / 29; 4 bits 512 8.4 / 9.9, 1024 11.7 / 11.4.
-         * Else two workgroups a CU, each with some 256 keys at least; and
-         * chunks short enough to even out ragged lengths: 24 sequences of up
-         * to 12000 fp16 rows 133 us with 1024 keys, 148 with 2048, 186 with the
-         * lengths halved; 40 of up to 8208 rows in 4 bits 148 with 512, 117
-         * with 1024, 106 with 2048, 121 with 4096. */
+         * key heads, us of the GPU, one launch / parts and their join (which
+         * cost an eager caller 4 more): fp16 256 keys 8.0 / 8.5, 512 11.3 / 8.6,
+         * 768 14.7 / 8.9, but of 32 sequences 512 15 / 19, 1024 25 / 29; 4 bits
+         * 512 8.4 / 9.4, 768 9.5 / 9.7, 1024 11.7 / 9.6, of 32 sequences 13.5
+         * / 17.
+         * Else two workgroups a CU, of 64 keys at least in fp16 (512 keys
+         * 8.6 us, with 128 9.5, with 256 11.0) and 256 in 4 bits (6000 keys
+         * 11.0 us, with 64 12.2); and chunks short enough to even out ragged
+         * lengths: 24 sequences of up to 12000 fp16 rows 133 us with 1024 keys,
+         * 148 with 2048, 186 with half a length; 40 of up to 8208 rows in 4
+         * bits 148 with 512, 117 with 1024, 106 with 2048, 121 with 4096. */
         const int64_t groups = nseq * n_kv;
-        const int kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec) */
-        p.wide = hd <= 128 && groups <= 256 && keys <= (kv4 || groups >= 128 ? 1024 : 512);
+        const int kt = kv4 && hd <= 128 ? 64 : 32, least = kv4 ? 256 : 64;   /* (CaDec::KT) */
+        p.wide = hd <= 128 && groups <= 256 && keys <= (groups >= 128 ? 1024 : kv4 ? 768 : 512);
         if (!p.wide) {
-            p.nsplit = (int)std::max<int64_t>({1, std::min<int64_t>(512 / groups, (keys + 255) / 256),
+            p.nsplit = (int)std::max<int64_t>({1, std::min<int64_t>(512 / groups, (keys + least - 1) / least),
                                                std::min<int64_t>({keys / (kv4 ? 2048 : 1024), 16384 / groups, CA_PARTS})});
             p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
         }
@@ -911,7 +914,7 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     default: ca_type<256>(a, p, nseq, part, s); break;
     }
     if (part) {
-        if (p.nsplit > 8)
+        if (p.nsplit > 8 || rows * n_heads <= 4096)   /* 8 parts of 32 heads: 4.0 us against 8.5 */
             k_cattn_merge_wide<<<(unsigned)(rows * n_heads), 256, 0, s>>>(a, p.nsplit, part);
         else
             k_cattn_merge<<<(unsigned)((rows * n_heads * (hd / 4) + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
