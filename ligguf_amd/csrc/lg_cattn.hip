@@ -57,6 +57,44 @@ __device__ __forceinline__ v4s ca_tr16(const _Float16* p)
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p);
 }
 
+/* the scale of scores whose queries are held times 2^(14 - ex): not 0, so that
+ * it times -infinity is no NaN (queries of 1e-40: the scores differ by nothing) */
+__device__ __forceinline__ float ca_scale(float scale2, int ex) { return fmaxf(ldexpf(scale2, ex - 14), FLT_MIN); }
+
+/* A column's running maximum.  Its weights are 2^(s sc + cc), cc = 14 - m sc as
+ * rounded: the rounding is the same for all of them, and goes along when the
+ * sums are rescaled (by the difference of two cc) or joined (-cc).  Where that
+ * is so far from 0 that its rounding would matter (scores of 10^6, or no key
+ * seen yet), the maximum is taken off the scores first and cc is 14; a wave
+ * with such a column raises at every tile. */
+struct CaMax {
+    float sc, m = -0x1p40f, cc = 14.0f;   /* (-2^40: below any score) */
+    bool any_far = true;                  /* of the wave */
+
+    __device__ __forceinline__ bool far(float c) const { return fabsf(c) > 0x1p22f; }
+    __device__ __forceinline__ bool due(float mn) const { return __builtin_amdgcn_ballot_w64(mn > m) || any_far; }
+    /* maximum mn of a tile's scores; returns what the sums so far are to be
+     * multiplied by, and in *off what to take off the tile's scores */
+    __device__ __forceinline__ float raise(float mn, float* off)
+    {
+        mn = fmaxf(mn, m);
+        const float c = __builtin_fmaf(-mn, sc, 14.0f), cn = far(c) ? 14.0f : c;
+        const bool was = far(__builtin_fmaf(-m, sc, 14.0f));
+        const float al = __builtin_amdgcn_exp2f(far(c) || was ? (m - mn) * sc : cn - cc);
+        m = mn;
+        cc = cn;
+        any_far = __builtin_amdgcn_ballot_w64(far(c)) != 0;
+        *off = far(c) ? mn : 0.0f;
+        return al;
+    }
+    /* the power of two that weights are multiples of, for sums to be joined; l: the sum of weights */
+    __device__ __forceinline__ float unit(float l) const
+    {
+        const float c = __builtin_fmaf(-m, sc, 14.0f);
+        return l == 0.0f ? -INFINITY : -c;
+    }
+};
+
 /* halves that are infinite or NaN to 0; whether there were any */
 __device__ __forceinline__ bool ca_drop_bad(v4u& w)
 {
@@ -137,8 +175,12 @@ __device__ __forceinline__ float2& ca_part_ml(const CAttn& a, int nsplit, float*
  *
  * q is held times a power of two that brings the row's largest value to
  * 2^13 .. 2^14 and p times 2^14, each in two fp16 parts, so 22 bits of both
- * survive whatever their size.  Bound by the cache's bytes: the loads of one
- * tile run while the last one computes. */
+ * survive whatever their size.  The loads of one tile run while the last one
+ * computes.  fp16 is bound by the cache's bytes (32 heads of 128, 8 key heads:
+ * 64 sequences of 2000 rows 100 us, 5.2 TB/s; 24 ragged ones of up to 12000
+ * 134 us, 4.6 TB/s); 4 bits by bytes and by VALU work, 59 % of the cycles (64 of
+ * 2000 rows 36 us, 4.5 TB/s; 40 ragged ones 101 us, 3.6 TB/s), most of it the 13
+ * operations for eight values: of 16 columns four are used. */
 template <int HD, bool KV4>
 struct CaDec {
     static constexpr int KT = KV4 && HD <= 128 ? 64 : 32, NU = KT / 16, NB = KT / 32;
@@ -159,8 +201,10 @@ struct CaRows {
     v4u h[KV4 ? 1 : C::NU][KV4 ? 1 : C::NS];
     uint32_t w[KV4 ? C::NU : 1][KV4 ? C::NS : 1], dm[KV4 ? C::NU : 1][C::ND];
 
-    /* the tile's address is the wave's, a lane's part of it fits 32 bits (rows of at most 2^25 bytes); at: the lane's rows in the tile */
-    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb, const uint32_t at[C::NU], int c)
+    /* at: the lane's rows of the tile at kb.  The tile's address is the wave's, a lane's part of it fits 32 bits (rows of
+     * at most 2^25 bytes). */
+    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb, const uint32_t at[C::NU],
+                                         int c)
     {
         const uint8_t* const p0 = base + (KV4 ? lg_kv4_codes(a.c, g, kb) : lg_kv16_at(a.c, g, kb));
         const uint8_t* const q0 = base + (KV4 ? lg_kv4_dm(a.c, g, kb) : 0);
@@ -170,7 +214,8 @@ struct CaRows {
                 const uint8_t* const p = p0 + at[u] * (uint32_t)(HD / 2) + (C::RUN ? c * (HD / 8) : 4 * c);
 #pragma unroll
                 for (int s = 0; s < C::NS; s++) w[u][s] = *(const uint32_t*)(p + s * (C::RUN ? 4 : 16));
-                const uint8_t* const q = q0 + at[u] * (uint32_t)(HD / 8) + (HD == 96 ? 0 : HD == 64 ? c / 2 * 4 : c * C::ND * 4);
+                const uint8_t* const q = q0 + at[u] * (uint32_t)(HD / 8) +
+                                         (HD == 96 ? 0 : HD == 64 ? c / 2 * 4 : c * C::ND * 4);
 #pragma unroll
                 for (int i = 0; i < C::ND; i++) dm[u][i] = *(const uint32_t*)(q + 4 * i);
             } else {
@@ -202,7 +247,8 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
     __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * C::WAVE];
     __shared__ float s_ml[NW][16][2];
     const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, sp = blockIdx.x / n_kv % nsplit, seq = blockIdx.x / n_kv / nsplit;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, c = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, c = lane >> 4;
     const int tok = col / a.nrep, ncol = a.ntok * a.nrep;
     const int64_t row = (int64_t)seq * a.ntok + min(tok, a.ntok - 1);
     const int head = g * a.nrep + col % a.nrep;
@@ -234,14 +280,15 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
     tiles.chunk(sp, nsplit, chunk, &t0, &t1);
     if (part && t0 >= t1) {   /* (workgroup-uniform) */
         if ((int)threadIdx.x < ncol)
-            ca_part_ml(a, nsplit, part, HD, ((int64_t)sp * a.rows + (int64_t)seq * a.ntok + threadIdx.x / a.nrep) * a.n_heads +
-                                               g * a.nrep + threadIdx.x % a.nrep) = make_float2(-INFINITY, 0.0f);
+            ca_part_ml(a, nsplit, part, HD,
+                       ((int64_t)sp * a.rows + (int64_t)seq * a.ntok + threadIdx.x / a.nrep) * a.n_heads + g * a.nrep +
+                           threadIdx.x % a.nrep) = make_float2(-INFINITY, 0.0f);
         return;
     }
     v4f o[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) o[t] = (v4f){};
-    float l = 0.0f, mx = -INFINITY;   /* the column's maximum in units of a power of two; l over this lane's keys */
+    float l = 0.0f, unit = -INFINITY;   /* sum of weights (this lane's keys) */
     if (t0 + wave < t1) {
         const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
         const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
@@ -249,7 +296,9 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
         CaRows<HD, KV4> K, V;
         uint32_t at[NU];
         /* keys that some column does not see (wave-uniform) */
-        auto partly = [&](int kb) { return kb + KT - 1 > pmin || (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks); };
+        auto partly = [&](int kb) {
+            return kb + KT - 1 > pmin || (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks);
+        };
         /* the lane's rows of the tile at kb.  Those that none of the columns at
          * one position sees give way to one that they do, so that whatever
          * they hold takes no part; where positions differ, see `bad` below. */
@@ -276,13 +325,13 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
         big = fmaxf(big, lg_partner<4>(big));
         big = fmaxf(big, lg_partner<5>(big));
         const int ex = __builtin_amdgcn_frexp_expf(big);   /* big < 2^ex */
-        const float sc = ldexpf(a.scale2, ex - 14);
+        CaMax mx = {ca_scale(a.scale2, ex)};
 #pragma unroll
         for (int j = 0; j < NS; j++)
 #pragma unroll
             for (int e = 0; e < 8; e += 2)
-                ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j], ql[j], e);
-        float m = -0x1p40f, cc = __builtin_fmaf(-m, sc, 14.0f);   /* below any score; cc: 14 less the maximum */
+                ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j],
+                          ql[j], e);
         for (; it < t1; it += NW) {
             v4f s[NU];
 #pragma unroll
@@ -313,16 +362,16 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
             for (int u = 0; u < NU; u++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) mn = fmaxf(mn, s[u][i]);
-            if (__builtin_amdgcn_ballot_w64(mn > m)) {
+            if (mx.due(mn)) {
                 mn = fmaxf(mn, lg_partner<4>(mn));
                 mn = fmaxf(mn, lg_partner<5>(mn));
-                mn = fmaxf(mn, m);
-                const float cn = __builtin_fmaf(-mn, sc, 14.0f), al = __builtin_amdgcn_exp2f(cn - cc);
-                m = mn;
-                cc = cn;
+                float off;
+                const float al = mx.raise(mn, &off);
                 l *= al;
 #pragma unroll
                 for (int t = 0; t < NT; t++) o[t] *= al;
+#pragma unroll
+                for (int u = 0; u < NU; u++) s[u] -= off;
             }
             uint64_t bad = 0;   /* keys of the tile */
 #pragma unroll
@@ -342,7 +391,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
                 for (int u = 0; u < 2; u++) {
                     float w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * b + u][i], sc, cc));
+                    for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * b + u][i], mx.sc, mx.cc));
                     l += (w[0] + w[1]) + (w[2] + w[3]);
                     ca_split2(w[0], w[1], ph, pl, 4 * u);
                     ca_split2(w[2], w[3], ph, pl, 4 * u + 2);
@@ -374,14 +423,14 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
         }
         l += lg_partner<4>(l);
         l += lg_partner<5>(l);
-        mx = l == 0.0f ? -INFINITY : m * sc;
+        unit = mx.unit(l);
     }
     /* the waves' parts of each column together, by way of LDS */
     float* const sO = (float*)(s_raw + wave * C::WAVE);
 #pragma unroll
     for (int t = 0; t < NT; t++) *(v4f*)(sO + col * C::OST + 16 * t + 4 * c) = o[t];
     if (c == 0) {
-        s_ml[wave][col][0] = mx;
+        s_ml[wave][col][0] = unit;
         s_ml[wave][col][1] = l;
     }
     __syncthreads();
@@ -422,7 +471,12 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
  * + 4 (l / 32) + i % 4 of column l % 32, so registers 8s .. 8s+7 of the scores
  * are the lane's k of step s of the second product: keys 16s + 4h .. and
  * 16s + 8 + 4h .. of lane half h.  The next tile is on its way while one
- * computes (two LDS stages, one barrier a tile). */
+ * computes (two LDS stages, one barrier a tile).  Bound by the MFMA and VALU
+ * work of a SIMD's two waves, which overlap little (52 % and 42 % of the cycles;
+ * keeping the waves half a tile apart, or products and softmax interleaved by
+ * hand, was slower): 2000 tokens over windows of 4096 rows 254 us, 530 TFLOP/s of
+ * the products asked for, 1060 issued with the parts, 0.9 of what torch's fp16
+ * product reaches on this card. */
 template <int HD, bool KV4>
 struct CaTile {
     static constexpr int NW = HD <= 128 ? 8 : 4, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;
@@ -499,7 +553,8 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
     const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv;
     const int seq = blockIdx.x / n_kv % (a.rows / a.ntok), rest = blockIdx.x / n_kv / (a.rows / a.ntok);
     const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, h = lane >> 5;
     const int ncol = a.ntok * a.nrep, idx = cb * 32 * C::NW + 32 * wave + col;
     const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
     const int64_t row = (int64_t)seq * a.ntok + tok;
@@ -532,7 +587,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
     v16f o[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) o[t] = (v16f){};
-    float l = 0.0f, mx = -INFINITY;
+    float l = 0.0f, unit = -INFINITY;
     if (pmax >= 0) {
         const CaTiles tiles(a, pmin, pmax, KT);
         int t0, t1;
@@ -545,13 +600,14 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
         };
         CaPieces<HD, KV4> P, V;
         v8h qh[NJ], ql[NJ];
-        float sc;
+        CaMax mx;
         {
             /* queries, first keys and first values on their way together */
             v4f x[2 * NJ];
             const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * h;
 #pragma unroll
-            for (int j = 0; j < 2 * NJ; j++) x[j] = idx < ncol ? *(const v4f*)(q + 16 * (j / 2) + 4 * (j % 2)) : (v4f){};
+            for (int j = 0; j < 2 * NJ; j++)
+                x[j] = idx < ncol ? *(const v4f*)(q + 16 * (j / 2) + 4 * (j % 2)) : (v4f){};
             const int k0 = tiles.at(t0) * KT;
             if (t0 < t1) {
                 P.load(a, kc, g, k0);
@@ -563,19 +619,19 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                 big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
             big = fmaxf(big, lg_partner<5>(big));
             const int ex = __builtin_amdgcn_frexp_expf(big);
-            sc = ldexpf(a.scale2, ex - 14);
+            mx.sc = ca_scale(a.scale2, ex);
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2)
-                    ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j], ql[j], e);
+                    ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j],
+                          ql[j], e);
             if (t0 < t1) {
                 P.template store<C::KST>(s_kv, nullptr);
                 V.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax) ? s_bad[0] : nullptr);
             }
         }
         __syncthreads();
-        float m = -0x1p40f, cc = __builtin_fmaf(-m, sc, 14.0f);
         for (int it = t0; it < t1; it++) {
             const bool more = it + 1 < t1;
             const int kb = tiles.at(it) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
@@ -590,7 +646,8 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             }
             v16f s[NK];
             if (on) {
-                __builtin_amdgcn_s_setprio(1);   /* its products ahead of the other wave's softmax: 700 x 9000 251 -> 243 us */
+                /* its products ahead of the other wave's softmax: 700 x 9000 251 -> 243 us */
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int n = 0; n < NK; n++) s[n] = (v16f){};
 #pragma unroll
@@ -603,9 +660,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                     }
             }
             __builtin_amdgcn_s_setprio(0);
-            if (more) {
-                P.template store<C::KST>(nK, nullptr);
-            }
+            if (more) P.template store<C::KST>(nK, nullptr);
             if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
             if (on) {
                 if (partly(kb, wmin, wmax)) {
@@ -620,15 +675,15 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                 for (int n = 0; n < NK; n++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) mn = fmaxf(mn, s[n][i]);
-                if (__builtin_amdgcn_ballot_w64(mn > m)) {
+                if (mx.due(mn)) {
                     mn = fmaxf(mn, lg_partner<5>(mn));
-                    mn = fmaxf(mn, m);
-                    const float cn = __builtin_fmaf(-mn, sc, 14.0f), al = __builtin_amdgcn_exp2f(cn - cc);
-                    m = mn;
-                    cc = cn;
+                    float off;
+                    const float al = mx.raise(mn, &off);
                     l *= al;
 #pragma unroll
                     for (int t = 0; t < NT; t++) o[t] *= al;
+#pragma unroll
+                    for (int n = 0; n < NK; n++) s[n] -= off;
                 }
 #pragma unroll
                 for (int st = 0; st < 2 * NK; st++) {
@@ -636,13 +691,14 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
                     v8h ph, pl;
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st / 2][8 * (st & 1) + i], sc, cc));
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st / 2][8 * (st & 1) + i], mx.sc, mx.cc));
                     l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) ca_split2(w[i], w[i + 1], ph, pl, i);
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        const _Float16* const v = sV + (16 * st + 4 * h + (lane & 15) / 4) * C::VST + 32 * t + (lane & 16) + 4 * (lane & 3);
+                        const _Float16* const v =
+                            sV + (16 * st + 4 * h + (lane & 15) / 4) * C::VST + 32 * t + (lane & 16) + 4 * (lane & 3);
                         const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 8 * C::VST);
                         const v8h x = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
                         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph, o[t], 0, 0, 0);
@@ -672,7 +728,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             __syncthreads();
         }
         l += lg_partner<5>(l);
-        mx = l == 0.0f ? -INFINITY : m * sc;
+        unit = mx.unit(l);
     }
     if (idx >= ncol) return;
     const int64_t at = ((int64_t)sp * a.rows + row) * a.n_heads + head;
@@ -686,11 +742,11 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
             const v4f y = {o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
             if (HD % 32 == 0 || d < HD) *(v4f*)(dst + d) = p < 0 ? (v4f){} : y * f;
         }
-    if (part && h == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(mx, l);
+    if (part && h == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(unit, l);
 }
 
-/* the splits' parts of a row's head: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M) */
-/* few parts: a thread per four dims */
+/* The parts of a row's head together: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M).
+ * Of many rows: a thread per four dims. */
 __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const float* __restrict__ part)
 {
     const int hd = a.c.hd, dq = hd / 4;
@@ -717,7 +773,7 @@ __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const 
     *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = y * (L == 0.0f ? 0.0f : 1.0f / L);
 }
 
-/* many parts of few rows: a workgroup per row's head, the weights by one wave,
+/* Many parts or few rows: a workgroup per row's head, the weights by one wave,
  * the sums by groups of hd / 4 threads -- a thread that walks over the parts
  * waits for one load after the other (64 parts of 32 heads: 34 us) */
 __global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, const float* __restrict__ part)
@@ -753,7 +809,8 @@ __global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, c
 #pragma unroll 4
         for (int s = grp; s < nsplit; s += ng) {
             const float f = s_f[s];
-            const v4f v = f != 0.0f ? *(const v4f*)(part + (s * n + at) * hd + d) : (v4f){};   /* (no keys, no sums written) */
+            /* (no keys, no sums written) */
+            const v4f v = f != 0.0f ? *(const v4f*)(part + (s * n + at) * hd + d) : (v4f){};
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
         }
@@ -829,13 +886,14 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
     return p;
 }
 
-extern "C" size_t lg_attn_cache_workspace_size(const lg_kv_cache* cache, int nseq, int ntok, int n_heads, int window, int sinks,
-                                               int max_pos)
+extern "C" size_t lg_attn_cache_workspace_size(const lg_kv_cache* cache, int nseq, int ntok, int n_heads, int window,
+                                               int sinks, int max_pos)
 {
     if (!cache || cache->n_kv_heads <= 0 || cache->head_dim <= 0 || nseq <= 0 || ntok <= 0 || n_heads <= 0 || window < 0 ||
         sinks < 0 || max_pos < 0)
         return 0;
-    return ca_plan(nseq, ntok, n_heads, cache->n_kv_heads, cache->head_dim, window, sinks, max_pos, cache->type == LG_KV4).ws;
+    return ca_plan(nseq, ntok, n_heads, cache->n_kv_heads, cache->head_dim, window, sinks, max_pos,
+                   cache->type == LG_KV4).ws;
 }
 
 template <int HD, bool KV4>
@@ -888,7 +946,8 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     }
     const int64_t rows = (int64_t)nseq * ntok, width = (int64_t)n_heads * hd;
     if (!rows) return LG_OK;
-    if (!pos || !q || !out || !lg_al16(q) || !lg_al16(out) || q_stride % 4 || out_stride % 4 || q_stride < width || out_stride < width) {
+    if (!pos || !q || !out || !lg_al16(q) || !lg_al16(out) || q_stride % 4 || out_stride % 4 || q_stride < width ||
+        out_stride < width) {
         lg_set_error("%s: rows must be given, 16-byte aligned and as wide as their heads", who);
         return LG_ERR_ARG;
     }

@@ -185,6 +185,25 @@ def test_query_sizes(gpu, ctype, scale):
     check(gpu, ctype, 4, 2, 128, 1, 40, 300, 0, 0, np.arange(260, 300), scale=scale)
 
 
+@pytest.mark.parametrize("ctype", TYPES)
+@pytest.mark.parametrize("scale", [1e-42, 1e-38, 1e32])
+def test_queries_at_the_ends_of_fp32(gpu, ctype, scale):
+    """Denormal queries (equal weights: the mean of what is seen) and ones whose scores near fp32's
+    end (one key takes all), in tiles of which a row sees nothing."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(7)
+    n_ctx, window = 500, 40
+    cache, (K, V) = make(gpu, ctype, 1, n_ctx, 2, 64, g)
+    for ntok in (1, 4, 60):
+        q = (g.standard_normal((1, ntok, 4, 64)) * scale).astype(np.float32)
+        pos = np.linspace(5, n_ctx - 1, ntok).astype(np.int32).reshape(1, -1)
+        got = ops.attention_cache(torch.from_numpy(q.reshape(1, ntok, -1)).to(gpu), cache, torch.from_numpy(pos).to(gpu),
+                                  window=window, sinks=1).cpu().numpy().reshape(q.shape)
+        want, _ = reference(q, K, V, pos, window, 1, n_ctx - 1)
+        assert np.max(np.abs(got - want)) <= 1e-5 * np.abs(V).max()
+
+
 def test_visible_key_nan_makes_its_rows_nan(gpu):
     for ntok in (1, 5, 50):
         def edit(which, x):
