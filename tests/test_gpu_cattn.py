@@ -204,6 +204,36 @@ def test_queries_at_the_ends_of_fp32(gpu, ctype, scale):
         assert np.max(np.abs(got - want)) <= 1e-5 * np.abs(V).max()
 
 
+@pytest.mark.parametrize("ctype", TYPES)
+@pytest.mark.parametrize("order", ["up", "down", "any"])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_scores_that_come_from_afar(gpu, ctype, order, hd):
+    """Maxima that move from -10^7 .. -10^4 past 0 to 10^4 .. 10^7, near and far columns in one
+    wave.  A key's score is one product of an integer by a power of two, exact, and differs by over
+    600 powers of two from the next, so the six keys of the highest share the row: their weights
+    are equal, in parts 4 U off, their sums and the joins 40 U, the quotient 2 U."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(3)
+    n_ctx, heads, kv = 3100, 8, 2
+    k0 = (np.arange(n_ctx) // 6 * 4 - 1000.0)[{"up": slice(None), "down": slice(None, None, -1), "any": g.permutation(n_ctx)}[order]]
+
+    def edit(which, x):
+        if which == 0:
+            x[:] = 0
+            x[0, :, :, 0] = k0[:, None]
+    cache, (K, V) = make(gpu, ctype, 1, n_ctx, kv, hd, g, edit)
+    for ntok, window, sinks in ((1, 0, 0), (1, 300, 5), (4, 0, 0), (60, 0, 0), (60, 300, 5)):
+        q = np.zeros((1, ntok, heads, hd), np.float32)
+        q[..., 0] = np.array([2 ** 10, 2 ** 15, -2 ** 18, 2 ** 19, -2 ** 15, 2 ** 18, 2 ** 10, -2 ** 11]) * np.sqrt(hd / 64)
+        pos = (np.array([n_ctx - 1]) if ntok == 1 else np.linspace(3, n_ctx - 1, ntok)).astype(np.int32).reshape(1, -1)
+        got = ops.attention_cache(torch.from_numpy(q.reshape(1, ntok, -1)).to(gpu), cache, torch.from_numpy(pos).to(gpu),
+                                  window=window, sinks=sinks).cpu().numpy().reshape(q.shape)
+        want, _ = reference(q, K, V, pos, window, sinks, n_ctx - 1)
+        size, _ = reference(q, K, np.abs(V), pos, window, sinks, n_ctx - 1)
+        assert np.all(np.abs(got - want) <= 64 * U * size + 1e-37), (ntok, window, float(np.abs(got - want).max()))
+
+
 def test_visible_key_nan_makes_its_rows_nan(gpu):
     for ntok in (1, 5, 50):
         def edit(which, x):
