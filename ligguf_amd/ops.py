@@ -110,7 +110,7 @@ def swiglu_quant(hb: torch.Tensor, hb2: torch.Tensor, qtype: int = Q8_K):
 # --------------------------------------------------------------------------
 # A serving loop makes these calls once per layer and token: each costs the host a few
 # microseconds beside the launches themselves, so the checks below read a tensor's fields once.
-_FP32, _INT32 = torch.float32, torch.int32
+_FP32, _INT32, _DENSE = torch.float32, torch.int32, torch.contiguous_format
 _raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream(i).cuda_stream without the Stream object
 
 
@@ -141,6 +141,12 @@ def _rows(t, i, nseq, ntok, width, name):
     if (s2 != 1 and width > 1) or (nseq > 1 and s0 != row * ntok):
         _refuse(f"{name}: rows of strides {t.stride()} are not one run")
     return t.data_ptr(), row
+
+
+def _fresh(like, rows, width):
+    """A dense tensor like `like` (whose last axis is `width`) and its (pointer, floats from row to row)."""
+    t = torch.empty_like(like, memory_format=_DENSE)
+    return t, (t.data_ptr(), width if rows > 1 else (width + 3) // 4 * 4)
 
 
 def _pos(pos):
@@ -220,13 +226,14 @@ def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None,
         q_out, rq, rqo = None, (None, 0), (None, 0)
     else:
         rq = _rows(q, *at, qd, "q")
-        if q_out is None:
-            q_out = q.new_empty((nseq, ntok, qd))
-        rqo = _rows(q_out, *at, qd, "q_out")
+        q_out, rqo = _fresh(q, nseq * ntok, qd) if q_out is None else (q_out, _rows(q_out, *at, qd, "q_out"))
     rk = _rows(k, *at, kd, "k")
-    if k_out is None and want_k:
-        k_out = k.new_empty((nseq, ntok, kd))
-    rko = (None, 0) if k_out is None else _rows(k_out, *at, kd, "k_out")
+    if k_out is not None:
+        rko = _rows(k_out, *at, kd, "k_out")
+    elif want_k:
+        k_out, rko = _fresh(k, nseq * ntok, kd)
+    else:
+        rko = (None, 0)
     if cache is None:
         rv, desc = (None, 0), None
     else:
@@ -278,12 +285,10 @@ def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max
     if heads * hd != width:
         _refuse(f"rows of {width} values are no heads of {hd}")
     rows = _rows(q, i, nseq, ntok, width, "q")
-    if out is None:
-        out = q.new_empty((nseq, ntok, width))
+    out, ro = _fresh(q, nseq * ntok, width) if out is None else (out, _rows(out, i, nseq, ntok, width, "out"))
     lib, desc = load(), C.byref(cache.desc)
     workspace, ws = _work(lib.lg_attn_cache_workspace_size(desc, nseq, ntok, heads, window, sinks, max_pos), workspace, q)
-    _on(i, lib.lg_attn_cache, *rows, desc, p, nseq, ntok, heads, window, sinks, max_pos,
-        *_rows(out, i, nseq, ntok, width, "out"), *ws)
+    _on(i, lib.lg_attn_cache, *rows, desc, p, nseq, ntok, heads, window, sinks, max_pos, *ro, *ws)
     return out
 
 
