@@ -796,7 +796,8 @@ __global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, c
         M = lg_group_max<64>(M);
 #pragma unroll
         for (int k = 0; k < CA_PARTS / 64; k++) {
-            const float f = x[k].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[k].x - M);
+            /* -1: no keys, no sums written (0 counts: it may meet an infinity) */
+            const float f = x[k].y == 0.0f ? -1.0f : __builtin_amdgcn_exp2f(x[k].x - M);
             s_f[threadIdx.x + 64 * k] = f;
             L = __builtin_fmaf(x[k].y, f, L);
         }
@@ -809,8 +810,7 @@ __global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, c
 #pragma unroll 4
         for (int s = grp; s < nsplit; s += ng) {
             const float f = s_f[s];
-            /* (no keys, no sums written) */
-            const v4f v = f != 0.0f ? *(const v4f*)(part + (s * n + at) * hd + d) : (v4f){};
+            const v4f v = f == -1.0f ? (v4f){} : *(const v4f*)(part + (s * n + at) * hd + d);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
         }

@@ -281,6 +281,28 @@ def test_visible_infinity_in_a_value(gpu):
         assert not torch.isfinite(got[..., bad]).any() and torch.equal(got[..., ~bad], want[..., ~bad])
 
 
+@pytest.mark.parametrize("ntok", [1, 4, 60])
+@pytest.mark.parametrize("n_ctx", [200, 3100])
+def test_visible_infinity_in_a_value_of_no_weight(gpu, ntok, n_ctx):
+    """Also where the key's weight, or that of all the keys of its part, is 0 in fp32."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(6)
+
+    def edit(which, x):
+        x[0, :, :, 0] = [np.linspace(-50, 50, n_ctx)[:, None], x[0, :, :, 0]][which]
+        if which == 1:
+            x[0, 7, 1, 5] = np.inf
+    cache, _ = make(gpu, L.F16, 1, n_ctx, 2, 64, g, edit)
+    q = torch.randn(1, ntok, 4, 64, generator=torch.Generator().manual_seed(2)).to(gpu)
+    q[..., 0] = 100.0
+    pos = torch.arange(n_ctx - ntok, n_ctx, dtype=torch.int32, device=gpu)[None]
+    got = ops.attention_cache(q.flatten(2), cache, pos).view(ntok, 4, 64).isfinite()
+    assert got[:, :2].all() and not got[:, 2:, 5].any()
+    got[:, 2:, 5] = True
+    assert got.all()
+
+
 def test_prompts_over_many_column_blocks_and_parts(gpu):
     """Several blocks of columns, the last one cut, whole and with the keys in parts."""
     check(gpu, L.F16, 4, 2, 64, 1, 333, 340, 0, 0, np.arange(7, 340))
