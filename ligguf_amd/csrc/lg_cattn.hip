@@ -477,9 +477,9 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
  * hand, was slower): 2000 tokens over windows of 4096 rows 254 us, 530 TFLOP/s of
  * the products asked for, 1060 issued with the parts, 0.9 of what torch's fp16
  * product reaches on this card. */
-template <int HD, bool KV4>
+template <int HD, bool KV4, int NW_>
 struct CaTile {
-    static constexpr int NW = HD <= 128 ? 8 : 4, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;
+    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;
     static constexpr int NJ = HD / 16, NT = (HD + 31) / 32;
     static constexpr int KST = HD + 8;                       /* halves per K row in LDS */
     static constexpr int VST = NT * 32 + 32;                 /* and per V row: rows 64 bytes on */
@@ -488,9 +488,9 @@ struct CaTile {
     static constexpr int STAGE = KT * (KST + VST);           /* halves */
 };
 
-template <int HD, bool KV4>
+template <int HD, bool KV4, int NW>
 struct CaPieces {
-    using C = CaTile<HD, KV4>;
+    using C = CaTile<HD, KV4, NW>;
     v4u h[KV4 ? 1 : C::NP];
     uint2 w[KV4 ? C::NP : 1];
     uint32_t dm[KV4 ? C::NP : 1];
@@ -540,11 +540,12 @@ struct CaPieces {
     }
 };
 
-template <int HD, bool KV4>
-__global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void k_cattn_tile(CAttn a, int ncb, int nsplit,
-                                                                                        float* __restrict__ part)
+/* (256 registers a lane, or 512 where those would not do) */
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4) ? 2 : 1)) void k_cattn_tile(
+    CAttn a, int ncb, int nsplit, float* __restrict__ part)
 {
-    using C = CaTile<HD, KV4>;
+    using C = CaTile<HD, KV4, NW>;
     constexpr int KT = C::KT, NK = C::NK, NJ = C::NJ, NT = C::NT;
     __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
     __shared__ int s_pos[2 * C::NW];
@@ -598,7 +599,7 @@ __global__ __launch_bounds__((HD <= 128 ? 512 : 256), (HD <= 128 ? 2 : 1)) void 
         auto partly = [&](int kb, int lo, int hi) {
             return kb + KT - 1 > lo || (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
         };
-        CaPieces<HD, KV4> P, V;
+        CaPieces<HD, KV4, NW> P, V;
         v8h qh[NJ], ql[NJ];
         CaMax mx;
         {
@@ -827,7 +828,7 @@ __global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, c
 struct CaPlan {
     bool dec;     /* up to 16 columns a key head */
     int ncb;      /* else: blocks of columns of a sequence's key head */
-    bool wide;    /* dec: eight waves a workgroup */
+    bool wide;    /* eight waves a workgroup, else four */
     int nsplit, chunk;   /* parts of the keys, tiles in a part */
     size_t ws;
 };
@@ -842,22 +843,39 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
     int64_t keys = (int64_t)max_pos + 1;
     if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
     if (!p.dec) {
-        const int64_t width = hd <= 128 ? 256 : 128;
-        p.ncb = (int)((cols + width - 1) / width);
-        /* Parts of the keys: whole rounds of 256 workgroups (one a CU), each as
-         * long as its tiles and, measured, some four more for its start and end;
-         * joined parts are written and read once, about 14 MB in a tile's
-         * time.  700 rows over 9000 keys (88 workgroups, us): 1 part 428, 2
-         * 234, 3 321, 4 259, 5 220, 6 280, 8 232. */
-        const int64_t wgs = nseq * n_kv * p.ncb, kt = hd <= 128 ? 64 : 32;
-        const double tiles = (double)((window > 0 ? keys : std::max<int64_t>(1, keys - ntok / 2)) + kt - 1) / kt;
+        /* Blocks of columns by workgroups of eight waves or, at 128 dims and less,
+         * of four where those fit the 256 CUs at once, and parts of the keys.
+         * The unit of time is a tile of an eight-wave workgroup (2.9 us at 128
+         * dims); a tile of four waves alone on their CU takes 0.95 of it, a
+         * start and end 4.5 and 2.6; joined parts are a second launch and are
+         * written and read once, about 19 MB in a unit.  Without a window the
+         * last columns see all keys, the mean half a prompt less.  32 heads of
+         * 128 over 8 key heads, us in (waves, parts) as chosen and others: 100
+         * tokens of 100 keys (4, 1) 14.3, (8, 1) 15.7; 1000 keys (4, 8) 27.9,
+         * (4, 1) 51, (8, 4) 33; 6000 keys (8, 16) 40, (8, 8) 56, (4, 8) 49; 700
+         * of 700 (4, 1) 38, (8, 1) 45; of 9000 (8, 5) 198, (8, 2) 226, (8, 3)
+         * 284, (8, 1) 419; 2000 of 2000 (8, 2) 92, (8, 1) 105. */
+        const int kt = hd <= 128 ? 64 : 32;
         double best = 0.0;
-        for (int ns = 1; ns <= 64 && (ns == 1 || tiles / ns >= 4.0); ns++) {
-            double cost = (double)((wgs * ns + 255) / 256) * (tiles / ns + 4.0);
-            if (ns > 1) cost += 1.5 + 8e-6 / 14.0 * ns * (double)(nseq * ntok) * n_heads * hd;
-            if (ns == 1 || cost < best) {
-                best = cost;
-                p.nsplit = ns;
+        for (int nw = hd <= 128 ? 8 : 4; nw >= 4; nw /= 2) {
+            const bool small = hd <= 128 && nw == 4;
+            const int64_t width = 32 * nw, ncb = (cols + width - 1) / width, wgs = nseq * n_kv * ncb;
+            if (small && cols <= 128) break;   /* (no more workgroups than of eight) */
+            int64_t seen = (int64_t)max_pos + 1, mean = std::max<int64_t>(1, seen - ntok / 2);
+            if (window > 0) seen = mean = std::min(seen, (int64_t)window + sinks + width * n_kv / n_heads);
+            const double last = (double)((seen + kt - 1) / kt), tiles = (double)(mean + kt - 1) / kt;
+            const double each = small ? 0.95 : 1.0, ends = small ? 2.6 : 4.5;
+            for (int ns = 1; ns <= 64 && (ns == 1 || last / ns >= 1.5); ns++) {
+                if (small && wgs * ns > 256) break;
+                double cost = std::max(last / ns * each + ends,
+                                       (double)((wgs * ns + 255) / 256) * (tiles / ns * each + ends));
+                if (ns > 1) cost += 2.0 + 6e-6 / 14.0 * ns * (double)(nseq * ntok) * n_heads * hd;
+                if (!p.ncb || cost < best) {
+                    best = cost;
+                    p.ncb = (int)ncb;
+                    p.nsplit = ns;
+                    p.wide = nw == 8;
+                }
             }
         }
     } else {
@@ -901,14 +919,15 @@ static void ca_launch(const CAttn& a, const CaPlan& p, int nseq, float* part, hi
 {
     const int64_t n = (int64_t)nseq * a.c.n_kv * p.nsplit;
     if constexpr (HD <= 128)
-        if (p.dec && p.wide) {
-            k_cattn_dec<HD, KV4, 8><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
+        if (p.wide) {
+            if (p.dec) k_cattn_dec<HD, KV4, 8><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
+            else k_cattn_tile<HD, KV4, 8><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.nsplit, part);
             return;
         }
     if (p.dec)
         k_cattn_dec<HD, KV4, 4><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
     else
-        k_cattn_tile<HD, KV4><<<(unsigned)(n * p.ncb), CaTile<HD, KV4>::NTH, 0, s>>>(a, p.ncb, p.nsplit, part);
+        k_cattn_tile<HD, KV4, 4><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.nsplit, part);
 }
 
 template <int HD>
