@@ -265,6 +265,21 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
             x[2 * s + 1] = in ? *(const v4f*)(q + d + 4) : (v4f){};
         }
     }
+    /* Without a window a lone workgroup's waves know their first tiles before
+     * the positions, and read them along (512 fp16 keys 10.7 -> 10.4 us, of 32
+     * sequences 15.0 -> 14.3); not where a wave has but one (256 keys 7.3 -> 8.4,
+     * the last being read twice) or in 4 bits (8.5 -> 9.1). */
+    const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
+    const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
+    CaRows<HD, KV4> K, V;
+    uint32_t at[NU];
+    const int early = NW == 8 && !KV4 && a.window <= 0 && a.max_pos >= NW * KT ? wave * KT : -1;
+    if (early >= 0) {
+#pragma unroll
+        for (int u = 0; u < NU; u++) at[u] = min(16 * u + col, a.max_pos - early);
+        K.load(a, kc, g, early, at, c);
+        V.load(a, vc, g, early, at, c);
+    }
     if (col >= ncol || p > a.max_pos) p = -1;
     int pmin = p < 0 ? INT32_MAX : p, pmax = p;
 #pragma unroll
@@ -290,11 +305,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
     for (int t = 0; t < NT; t++) o[t] = (v4f){};
     float l = 0.0f, unit = -INFINITY;   /* sum of weights (this lane's keys) */
     if (t0 + wave < t1) {
-        const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
-        const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
         _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
-        CaRows<HD, KV4> K, V;
-        uint32_t at[NU];
         /* keys that some column does not see (wave-uniform) */
         auto partly = [&](int kb) {
             return kb + KT - 1 > pmin || (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks);
@@ -313,9 +324,13 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
             }
         };
         int it = t0 + wave, kb = tiles.at(it) * KT;
-        rows_of(kb);
-        K.load(a, kc, g, kb, at, c);
-        V.load(a, vc, g, kb, at, c);
+        if (kb != early || (pmin == pmax && partly(kb))) {
+            rows_of(kb);
+            K.load(a, kc, g, kb, at, c);
+            V.load(a, vc, g, kb, at, c);
+        }
+        /* (all of these loads ahead of what waits for the query: 0.3 to 0.8 us) */
+        __builtin_amdgcn_sched_barrier(0);
         /* the query in two parts, while the first keys come */
         v8h qh[NS], ql[NS];
         float big = 0.0f;
@@ -884,7 +899,7 @@ static CaPlan ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
          * cost an eager caller 4 more): fp16 256 keys 8.0 / 8.5, 512 11.3 / 8.6,
          * 768 14.7 / 8.9, but of 32 sequences 512 15 / 19, 1024 25 / 29; 4 bits
          * 512 8.4 / 9.4, 768 9.5 / 9.7, 1024 11.7 / 9.6, of 32 sequences 13.5
-         * / 17.
+         * / 17 (both 0.3 to 0.9 less since the first loads go ahead).
          * Else two workgroups a CU, of 64 keys at least in fp16 (512 keys
          * 8.6 us, with 128 9.5, with 256 11.0) and 256 in 4 bits (6000 keys
          * 11.0 us, with 64 12.2); and chunks short enough to even out ragged

@@ -244,6 +244,21 @@ def test_visible_key_nan_makes_its_rows_nan(gpu):
 
 
 @pytest.mark.parametrize("ctype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_ctx", [257, 400, 512])
+def test_short_contexts_whose_rows_end_early(gpu, ctype, hd, n_ctx):
+    """Single tokens at the borders of tiles and idle slots, NaN behind every position, whatever is
+    read before the positions are known."""
+    pos = [n_ctx - 1, 0, -1, 31, 32, 255, 256, n_ctx - 2, n_ctx]
+
+    def edit(which, x):
+        for s, p in enumerate(pos):
+            x[s, p + 1 if p < n_ctx else 0:] = np.nan
+    got, _, _ = check(gpu, ctype, 8, 2, hd, len(pos), 1, n_ctx, 0, 0, pos, edit=edit)
+    assert not got[2].any() and not got[-1].any()
+
+
+@pytest.mark.parametrize("ctype", TYPES)
 @pytest.mark.parametrize("ntok", [1, 4, 40])
 def test_queries_of_rows_without_a_token(gpu, ctype, ntok):
     """NaN and infinities in the queries of idle rows stay there, and their outputs are zeros."""
