@@ -6,7 +6,8 @@ in-tree build (``build.py``) and a thin host-side mirror for Python callers:
 
 * ``lib``    -- ctypes binding of every C-ABI symbol;
 * ``ops``    -- per-op calls on torch device tensors, named after the
-               reference's math layer (fast/lil_math.h);
+               reference's math layer (fast/lil_math.h), and the calls for
+               many tokens, many sequences and long contexts;
 * ``model``  -- host model description (synthetic or GGUF) and ``Engine``;
 * ``gguf``   -- GGUF v3 reader/writer;
 * ``encode`` -- weight encoders (fp32 -> GGUF blocks).

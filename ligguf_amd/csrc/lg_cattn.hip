@@ -487,11 +487,13 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
  * are the lane's k of step s of the second product: keys 16s + 4h .. and
  * 16s + 8 + 4h .. of lane half h.  The next tile is on its way while one
  * computes (two LDS stages, one barrier a tile).  Bound by the MFMA and VALU
- * work of a SIMD's two waves, which overlap little (52 % and 42 % of the cycles;
- * keeping the waves half a tile apart, or products and softmax interleaved by
- * hand, was slower): 2000 tokens over windows of 4096 rows 254 us, 530 TFLOP/s of
- * the products asked for, 1060 issued with the parts, 0.9 of what torch's fp16
- * product reaches on this card. */
+ * work of a SIMD's two waves, 52 % and 42 % of the cycles, at 2.04 of 2.4 GHz
+ * (keeping the waves half a tile apart, products and softmax interleaved by
+ * hand, or V's fragments read a step ahead was no faster): 2000 tokens over
+ * windows of 4096 rows 260 us, 520 TFLOP/s of the products asked for, 1040 issued
+ * with the parts, 0.88 of what torch's fp16 product reaches on this card.  One
+ * wave a SIMD does a tile in 0.9 of the time of two: two to a SIMD wherever
+ * there are columns enough. */
 template <int HD, bool KV4, int NW_>
 struct CaTile {
     static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;

