@@ -66,11 +66,18 @@ __device__ __forceinline__ float ca_scale(float scale2, int ex) { return fmaxf(l
  * sums are rescaled (by the difference of two cc) or joined (-cc).  Where that
  * is so far from 0 that its rounding would matter (scores of 10^6, or no key
  * seen yet), the maximum is taken off the scores first and cc is 14; a wave
- * with such a column raises at every tile. */
+ * with such a column raises at every tile.  cc belongs to m from the start: of
+ * small queries -2^40 sc is near, and a first tile without a key of the column
+ * would else raise from 14 by a factor that is infinite. */
 struct CaMax {
-    float sc, m = -0x1p40f, cc = 14.0f;   /* (-2^40: below any score) */
-    bool any_far = true;                  /* of the wave */
+    float sc, m, cc;
+    bool any_far;                         /* of the wave */
 
+    __device__ __forceinline__ explicit CaMax(float scale) : sc(scale), m(-0x1p40f), any_far(true)   /* (-2^40: below any score) */
+    {
+        const float c = __builtin_fmaf(-m, sc, 14.0f);
+        cc = far(c) ? 14.0f : c;
+    }
     __device__ __forceinline__ bool far(float c) const { return fabsf(c) > 0x1p22f; }
     __device__ __forceinline__ bool due(float mn) const { return __builtin_amdgcn_ballot_w64(mn > m) || any_far; }
     /* maximum mn of a tile's scores; returns what the sums so far are to be
@@ -340,7 +347,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
         big = fmaxf(big, lg_partner<4>(big));
         big = fmaxf(big, lg_partner<5>(big));
         const int ex = __builtin_amdgcn_frexp_expf(big);   /* big < 2^ex */
-        CaMax mx = {ca_scale(a.scale2, ex)};
+        CaMax mx(ca_scale(a.scale2, ex));
 #pragma unroll
         for (int j = 0; j < NS; j++)
 #pragma unroll
@@ -618,7 +625,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4)
         };
         CaPieces<HD, KV4, NW> P, V;
         v8h qh[NJ], ql[NJ];
-        CaMax mx;
+        CaMax mx(0.0f);
         {
             /* queries, first keys and first values on their way together */
             v4f x[2 * NJ];
@@ -637,7 +644,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4)
                 big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
             big = fmaxf(big, lg_partner<5>(big));
             const int ex = __builtin_amdgcn_frexp_expf(big);
-            mx.sc = ca_scale(a.scale2, ex);
+            mx = CaMax(ca_scale(a.scale2, ex));
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
