@@ -473,9 +473,12 @@ int lg_kv4_read(const lg_kv_cache* cache, int nseq, int pos0, int npos, uint16_t
  * reads head h / (n_heads / n_kv_heads).  head_dim 48 (LG_F16 only), 64, 96,
  * 128 or 256.  max_pos < n_ctx bounds the positions: a row beyond it counts as
  * one without a token, and its output is zeros.  A row's result does not
- * depend on what invisible rows hold, infinities and NaN included; one in the
- * query or in a visible key makes the row's head NaN, one in a visible value
- * makes its dim infinite or NaN.  out does not overlap q.
+ * depend on what invisible rows hold, infinities and NaN included.  One in the
+ * query or a NaN in a visible key makes the row's head NaN; an infinity in a
+ * visible key makes its score infinite (NaN where the query's value is 0): at
+ * -infinity the key has no weight, at +infinity or where no visible key has a
+ * weight the row's head is NaN.  One in a visible value makes its dim infinite
+ * or NaN.  out does not overlap q.
  * fp32 queries and the softmax's weights enter the products as two fp16
  * parts, about 22 bits.  workspace: lg_attn_cache_workspace_size bytes of
  * device memory, 16-byte aligned (NULL when that is 0), which nothing else may

@@ -41,6 +41,27 @@ __device__ __forceinline__ void ca_split2(float x0, float x1, v8h& hi, v8h& lo, 
     lo[i + 1] = y[1];
 }
 
+/* A query's values x0, x1, times 2^(14 - ex), in two parts that have x's sign
+ * and are 0 only if x is: both products with an infinity are then the one that
+ * x's is (NaN where x is 0), and so is their sum.  hi is rounded towards 0, so
+ * that lo has its sign, 22 bits in all; a part that would be 0 takes the least
+ * fp16, at most 2^-37 of the row's largest value. */
+__device__ __forceinline__ void ca_query2(float x0, float x1, int ex, v8h& hi, v8h& lo, int i)
+{
+    typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+    const float y0 = ldexpf(x0, 14 - ex), y1 = ldexpf(x1, 14 - ex);
+    const u2 least = {(uint16_t)(x0 != 0.0f), (uint16_t)(x1 != 0.0f)}, sign = {0x8000, 0x8000};
+    const lg_h2 h = __builtin_bit_cast(lg_h2, __builtin_amdgcn_cvt_pkrtz(y0, y1));
+    const lg_h2 l = __builtin_convertvector(((lg_f2){y0 - (float)h[0], y1 - (float)h[1]}), lg_h2);
+    const u2 hb = __builtin_bit_cast(u2, h), lb = __builtin_bit_cast(u2, l);
+    const lg_h2 a = __builtin_bit_cast(lg_h2, __builtin_elementwise_max(hb & ~sign, least) | (hb & sign));
+    const lg_h2 b = __builtin_bit_cast(lg_h2, __builtin_elementwise_max(lb & ~sign, least) | (hb & sign));
+    hi[i] = a[0];
+    hi[i + 1] = a[1];
+    lo[i] = b[0];
+    lo[i + 1] = b[1];
+}
+
 /* the wave's LDS writes before its other lanes' reads */
 __device__ __forceinline__ void ca_wave_sync()
 {
@@ -352,8 +373,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
         for (int j = 0; j < NS; j++)
 #pragma unroll
             for (int e = 0; e < 8; e += 2)
-                ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j],
-                          ql[j], e);
+                ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
         for (; it < t1; it += NW) {
             v4f s[NU];
 #pragma unroll
@@ -479,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
             *(v4f*)(part + at * HD + d) = y;
             if (d == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(M, L);
         } else {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            const float inv = 1.0f / L;   /* (0 times infinity where every visible key is -infinity) */
             const int pk = a.pos[r];
             *(v4f*)(a.out + r * a.os + (size_t)hh * HD + d) = pk < 0 || pk > a.max_pos ? (v4f){} : y * inv;
         }
@@ -649,8 +669,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4)
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2)
-                    ca_split2(ldexpf(x[2 * j + e / 4][e % 4], 14 - ex), ldexpf(x[2 * j + e / 4][e % 4 + 1], 14 - ex), qh[j],
-                          ql[j], e);
+                    ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
             if (t0 < t1) {
                 P.template store<C::KST>(s_kv, nullptr);
                 V.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax) ? s_bad[0] : nullptr);
@@ -758,7 +777,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4)
     if (idx >= ncol) return;
     const int64_t at = ((int64_t)sp * a.rows + row) * a.n_heads + head;
     float* const dst = part ? part + at * HD : a.out + row * a.os + (size_t)head * HD;
-    const float f = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    const float f = part ? 1.0f : 1.0f / l;   /* (0: every visible key is -infinity) */
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -795,7 +814,7 @@ __global__ __launch_bounds__(256) void k_cattn_merge(CAttn a, int nsplit, const 
             for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
         }
     }
-    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = y * (L == 0.0f ? 0.0f : 1.0f / L);
+    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = p < 0 || p > a.max_pos ? (v4f){} : y * (1.0f / L);
 }
 
 /* Many parts or few rows: a workgroup per row's head, the weights by one wave,
@@ -845,7 +864,7 @@ __global__ __launch_bounds__(256) void k_cattn_merge_wide(CAttn a, int nsplit, c
     if (grp) return;
     for (int k = 1; k < ng; k++) y += s_y[threadIdx.x + k * dq];
     const float L = s_l;
-    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = p < 0 || p > a.max_pos || L == 0.0f ? (v4f){} : y * (1.0f / L);
+    *(v4f*)(a.out + row * a.os + (size_t)head * hd + d) = p < 0 || p > a.max_pos ? (v4f){} : y * (1.0f / L);
 }
 
 /* How a call is cut, from its sizes alone. */
