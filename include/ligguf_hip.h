@@ -386,7 +386,8 @@ int lg_swiglu_quant(float* hb, const float* hb2, int n, int qtype, void* out_q, 
  * replay.  Strides are in floats, from one row to the next; pointers and
  * strides of fp32 rows are multiples of 16 bytes.  The calling thread's
  * current device must be the one that owns the pointers and the stream.
- * Nothing is allocated, and no call keeps state for the next. */
+ * Nothing is allocated, and no call keeps state for the next.  A call that
+ * would need a grid of 2^32 threads or more (10^7 rows and up) is refused. */
 
 /* A layer's cache of nseq sequences in the caller's device memory, for keys
  * and values alike, n_ctx <= 2^30 rows:

@@ -1021,6 +1021,14 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     a.nrep = n_heads / a.c.n_kv;
     a.scale2 = 1.44269504088896341f / sqrtf((float)hd);
     const CaPlan p = ca_plan(nseq, ntok, n_heads, a.c.n_kv, hd, window, sinks, max_pos, a.c.type == LG_KV4);
+    /* workgroups of the kernel and, of a split call, of its join */
+    const int64_t blocks = (int64_t)nseq * a.c.n_kv * p.nsplit * (p.dec ? 1 : p.ncb);
+    const bool by_group = p.nsplit > 8 || rows * n_heads <= 4096;   /* 8 parts of 32 heads: 4.0 us against 8.5 */
+    const int64_t joins = p.ws ? by_group ? rows * n_heads : (rows * n_heads * (hd / 4) + 255) / 256 : 0;
+    if (!lg_grid_fits(blocks, p.wide ? 512 : 256) || !lg_grid_fits(joins, 256)) {
+        lg_set_error("%s: %lld rows of %d heads are too many for one call", who, (long long)rows, n_heads);
+        return LG_ERR_ARG;
+    }
     if (p.ws && (!workspace || !lg_al16(workspace) || workspace_bytes < p.ws)) {
         lg_set_error("%s: workspace of %zu bytes, 16-byte aligned, %zu needed", who, workspace_bytes, p.ws);
         return LG_ERR_ARG;
@@ -1035,10 +1043,8 @@ extern "C" int lg_attn_cache(const float* q, int64_t q_stride, const lg_kv_cache
     default: ca_type<256>(a, p, nseq, part, s); break;
     }
     if (part) {
-        if (p.nsplit > 8 || rows * n_heads <= 4096)   /* 8 parts of 32 heads: 4.0 us against 8.5 */
-            k_cattn_merge_wide<<<(unsigned)(rows * n_heads), 256, 0, s>>>(a, p.nsplit, part);
-        else
-            k_cattn_merge<<<(unsigned)((rows * n_heads * (hd / 4) + 255) / 256), 256, 0, s>>>(a, p.nsplit, part);
+        if (by_group) k_cattn_merge_wide<<<(unsigned)joins, 256, 0, s>>>(a, p.nsplit, part);
+        else k_cattn_merge<<<(unsigned)joins, 256, 0, s>>>(a, p.nsplit, part);
     }
     return lg_check_launch(who);
 }

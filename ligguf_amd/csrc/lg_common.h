@@ -273,6 +273,9 @@ struct lg_rand_guard {
     ~lg_rand_guard() { setstate(caller); }
 };
 
+/* a grid of fewer than 2^32 threads, all that HIP takes in a dimension */
+static inline bool lg_grid_fits(int64_t blocks, int threads) { return blocks <= (int64_t)(UINT32_MAX / threads); }
+
 /* host helper: turn a failed kernel launch into LG_ERR_HIP */
 int lg_check_launch(const char* what);
 int lg_launch_read_probe(const void* buf, size_t bytes, hipStream_t s);

@@ -292,7 +292,7 @@ static void rope_launch(const RopeArgs& a, int64_t rows, int all, hipStream_t s)
      * token's, so that its angles (in double) are worked out once; few: one
      * round each, for more of them at a time */
     const int rounds = (all + 4 * (64 / G) - 1) / (4 * (64 / G));
-    const int nblk = rows >= 512 ? 1 : rounds;
+    const int nblk = rows >= 512 || !lg_grid_fits(rows * rounds, 256) ? 1 : rounds;
     k_rope_tokens<HALF, N, G><<<(unsigned)(rows * nblk), 256, 0, s>>>(a, nblk, nblk == 1 ? rounds : 1);
 }
 
@@ -352,7 +352,7 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
         }
     }
     const int waves = n_heads + n_kv_heads * (cache ? 2 : 1);
-    if (rows > INT32_MAX / waves) {
+    if (rows > INT32_MAX / waves || !lg_grid_fits(rows, 256)) {
         lg_set_error("%s: %lld rows of %d heads are too many for one call", who, (long long)rows, waves);
         return LG_ERR_ARG;
     }
@@ -361,16 +361,15 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
     return lg_check_launch(who);
 }
 
-/* One thread per word of eight codes; keys, then values.  I: 32 bits where the
- * words of a sequence are fewer (64-bit divisions cost more than the reads). */
-template <typename I>
+/* One thread per word of eight codes; keys, then values.  Fewer than 2^32 words of
+ * a sequence (64-bit divisions cost more than the reads). */
 __global__ __launch_bounds__(256) void k_kv4_read(LgKv c, int pos0, int npos, uint16_t* __restrict__ ko,
                                                   uint16_t* __restrict__ vo)
 {
-    const I hw = c.hd / 8, i = (I)blockIdx.x * 256 + threadIdx.x;   /* words of a head's row */
-    if (i >= (I)npos * c.n_kv * hw) return;
-    const I r = i / hw;
-    const int wd = (int)(i - r * hw), p = (int)(r / (I)c.n_kv), g = (int)(r - p * (I)c.n_kv), seq = blockIdx.y;
+    const uint32_t hw = c.hd / 8, i = blockIdx.x * 256 + threadIdx.x;   /* words of a head's row */
+    if (i >= (uint32_t)npos * c.n_kv * hw) return;
+    const uint32_t r = i / hw, n_kv = c.n_kv;
+    const int wd = (int)(i - r * hw), p = (int)(r / n_kv), g = (int)(r - p * n_kv), seq = blockIdx.y;
     const uint8_t* const b = (blockIdx.z ? c.v : c.k) + (size_t)seq * c.seq;
     const uint32_t w = ((const uint32_t*)(b + lg_kv4_codes(c, g, pos0 + p)))[wd];
     const uint32_t dm = ((const uint32_t*)(b + lg_kv4_dm(c, g, pos0 + p)))[wd / 4];
@@ -400,13 +399,12 @@ extern "C" int lg_kv4_read(const lg_kv_cache* cache, int nseq, int pos0, int npo
         return LG_ERR_ARG;
     }
     const int64_t n = ((int64_t)npos * c.n_kv * (c.hd / 8) + 255) / 256;
-    if (n > INT32_MAX) {
+    if (!lg_grid_fits(n, 256)) {
         lg_set_error("%s: %d rows are too many for one call", who, npos);
         return LG_ERR_ARG;
     }
     if (!n || !nseq) return LG_OK;
     const dim3 grid((unsigned)n, nseq, 2);
-    if (n <= INT32_MAX / 256) k_kv4_read<uint32_t><<<grid, 256, 0, (hipStream_t)stream>>>(c, pos0, npos, k_out, v_out);
-    else k_kv4_read<uint64_t><<<grid, 256, 0, (hipStream_t)stream>>>(c, pos0, npos, k_out, v_out);
+    k_kv4_read<<<grid, 256, 0, (hipStream_t)stream>>>(c, pos0, npos, k_out, v_out);
     return lg_check_launch(who);
 }

@@ -344,7 +344,12 @@ extern "C" int lg_logprobs(const float* logits, int64_t stride, int rows, int vo
      * 256 of 16000 11 against 8.  Rows in parts of 4096 logits and a second
      * launch to join them were faster for one row of 151936 only (11 us against
      * 16, without the host's time for that launch; 32000 logits 9 against 8). */
-    if (rows > 512 && vocab <= 32768) k_logp<256><<<rows, 256, 0, (hipStream_t)stream>>>(a);
+    const bool narrow = rows > 512 && vocab <= 32768;
+    if (!lg_grid_fits(rows, narrow ? 256 : 1024)) {
+        lg_set_error("%s: %d rows are too many for one call", who, rows);
+        return LG_ERR_ARG;
+    }
+    if (narrow) k_logp<256><<<rows, 256, 0, (hipStream_t)stream>>>(a);
     else k_logp<1024><<<rows, 1024, 0, (hipStream_t)stream>>>(a);
     return lg_check_launch(who);
 }

@@ -308,3 +308,49 @@ def test_python_refusals(gpu):
     for a in ((-1, 1), (0, 5), (3, 2), (5, None)):
         with pytest.raises(L.LgError):
             ops.kv_values(four, *a)
+
+
+def test_few_rows_of_more_heads_than_a_grid_takes(gpu):
+    """511 rows of 65536 query, key and value heads of two values: a workgroup per round of heads would be 25
+    million of them."""
+    import torch
+    from ligguf_amd import ops
+    n, heads = 511, 65536
+    g = torch.Generator(device=gpu).manual_seed(5)
+    q, k, v = (torch.randn(1, n, 2 * heads, generator=g, device=gpu) for _ in range(3))
+    pos = torch.arange(n, dtype=torch.int32, device=gpu)[None]
+    cache = ops.KvCache.empty(ops.F16, n, heads, 2, 1, gpu)
+    freq = torch.full((1,), 0.1, device=gpu)
+    qo, ko = ops.qk_norm_rope_tokens(q, k, v, pos, freq, 2, cache=cache, want_k=True)
+    for x, y in ((q, qo), (k, ko)):
+        for t in (0, 300, n - 1):
+            want, tol = expected(x[0, t].cpu().numpy().reshape(1, heads, 2), None, np.array([t]), freq.cpu().numpy(), 2, False, 1.0, 1e-6)
+            assert np.all(np.abs(y[0, t].cpu().numpy().reshape(want.shape) - want) <= tol + 1e-30)
+    assert torch.equal(cache.k, ko.half()) and torch.equal(cache.v, v.half())
+    del q, k, v, qo, ko, x, y, cache
+    torch.cuda.empty_cache()
+
+
+def test_reading_back_past_31_bits_of_words(gpu):
+    """More than 2^31 words of codes in one call, rows on both sides of the border (34 GB each of keys
+    and values; the cache's keys and values are the same memory)."""
+    import torch
+    from ligguf_amd import ops
+    kv, hd, n = 8, 256, (1 << 23) + 40
+    if torch.cuda.mem_get_info(gpu)[0] < 100 << 30:
+        pytest.skip("needs 80 GB of device memory")
+    x = torch.randn(1, 6, kv * hd, generator=torch.Generator(device=gpu).manual_seed(6), device=gpu)
+    mem = torch.zeros(1, L.load().lg_kv_bytes(L.KV4, n, kv, hd), dtype=torch.uint8, device=gpu)
+    cache = ops.KvCache(mem, mem, kv, hd, ops.KV4, n)
+    at = [0, 1, (1 << 22) + 3, (1 << 23) - 1, 1 << 23, n - 1]
+    pos = torch.tensor([at], dtype=torch.int32, device=gpu)
+    ops.qk_norm_rope_tokens(None, x, x, pos, None, hd, rope_dim=0, cache=cache)
+    out = ops.kv_values(cache)
+    want = pack(x.cpu().numpy())[3].reshape(6, -1)
+    for t in out:
+        for i, p in enumerate(at):
+            assert np.array_equal(t[0, p].cpu().numpy(), want[i])
+        for p in (2, (1 << 22) + 2, (1 << 23) - 2, (1 << 23) + 1, n - 2):
+            assert not t[0, p].any()
+    del out, t, mem, cache
+    torch.cuda.empty_cache()

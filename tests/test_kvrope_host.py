@@ -116,3 +116,13 @@ def test_read_refuses_an_fp16_cache():
     assert L.load().lg_kv4_read(C.byref(c), 1, 0, 1, P, P, None) == -2
     c = cache(type=L.KV4)
     assert L.load().lg_kv4_read(C.byref(c), 1, 32, 0, P, P, None) == 0
+
+
+def test_grids_past_32_bits_are_refused():
+    """2^24 workgroups of 256 threads: more than a launch takes."""
+    err = L.load().lg_last_error
+    assert rope(ntok=1 << 24) == -1 and b"too many" in err(None)
+    assert rope(nseq=1 << 14, ntok=1 << 10, nh=0, kv=1, c=cache(n_ctx=1 << 20, kv=1)) == -1 and b"too many" in err(None)
+    c = cache(type=L.KV4, n_ctx=1 << 28)
+    for npos in (1 << 28, (1 << 28) - 15):       # 2 heads of eight words: 2^32 words, 2^24 workgroups
+        assert L.load().lg_kv4_read(C.byref(c), 1, 0, npos, P, P, None) == -1 and b"too many" in err(None)

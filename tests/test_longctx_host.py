@@ -55,3 +55,12 @@ def logp(x=P, stride=100, rows=2, vocab=100, toks=P, top=3, lp=P, ent=P, ids=P, 
 ])
 def test_logprobs_refusals(kw):
     assert logp(**kw) == -1 and L.load().lg_last_error(None)
+
+
+def test_grids_past_32_bits_are_refused():
+    """2^24 workgroups of 256 threads, 2^22 of 1024: more than a launch takes."""
+    err = L.load().lg_last_error
+    assert attn(nseq=1 << 23, heads=2) == -1 and b"too many" in err(None)
+    assert attn(nseq=1 << 20, ntok=64, heads=8, qs=512, os=512, c=cache(kv=8)) == -1 and b"too many" in err(None)
+    assert logp(rows=1 << 24) == -1 and b"too many" in err(None)
+    assert logp(rows=1 << 22, vocab=40000, stride=40000) == -1 and b"too many" in err(None)
