@@ -101,7 +101,7 @@ struct RopeArgs {
     LgKv c;   /* c.type 0: no cache */
 };
 
-/* cos, sin of pos * freq, times mscale.  Far positions need the angle in
+/* cos, sin of pos * freq, times mscale, rounded once.  Far positions need the angle in
  * double: at 10^5 radians fp32 would leave 0.004 of it.  a / 2 pi with its low
  * half in a fused multiply-add, less the nearest whole number of turns. */
 __device__ __forceinline__ float2 lg_turn(int pos, float freq, float mscale)
@@ -111,7 +111,7 @@ __device__ __forceinline__ float2 lg_turn(int pos, float freq, float mscale)
     const double r = __builtin_fma(a, inv, -n) + a * inv_lo;
     double s, c;
     sincospi(2.0 * r, &s, &c);
-    return make_float2((float)c * mscale, (float)s * mscale);
+    return make_float2((float)(c * mscale), (float)(s * mscale));
 }
 
 typedef float v2f __attribute__((ext_vector_type(2), aligned(4)));

@@ -354,3 +354,22 @@ def test_reading_back_past_31_bits_of_words(gpu):
             assert not t[0, p].any()
     del out, t, mem, cache
     torch.cuda.empty_cache()
+
+
+def test_rotation_by_a_scaled_angle_rounds_once(gpu):
+    """The pair (1, 0) becomes mscale (cos, sin) itself: the factors, rounded to fp32 once."""
+    import torch
+    from ligguf_amd import ops
+    hd, n = 128, 500
+    freq, mscale = ops.rope_table(hd, 1e4, L.ROPE_YARN, 4.0, 4096, 32.0, 1.0)
+    assert mscale != 1.0
+    pos = torch.arange(0, 37 * n, 37, dtype=torch.int32, device=gpu)[None]
+    x = torch.zeros(1, n, hd, device=gpu)
+    x[..., ::2] = 1.0
+    got = ops.qk_norm_rope_tokens(None, x, None, pos, freq.to(gpu), hd, mscale=mscale, want_k=True)[1]
+    got = got.cpu().numpy().reshape(n, hd // 2, 2).astype(np.float64)
+    ang = pos.cpu().numpy().reshape(-1, 1).astype(np.float64) * freq.numpy().astype(np.float64)
+    for e, f in enumerate((np.cos, np.sin)):
+        want = f(ang) * float(np.float32(mscale))
+        # half a step, and what the angle's rounding to a double (2 10^4 radians: 2e-12) leaves near a border
+        assert np.all(np.abs(got[..., e] - want) <= np.spacing(np.abs(want).astype(np.float32)) / 2.0 + 1e-11)
