@@ -144,9 +144,14 @@ def _rows(t, i, nseq, ntok, width, name):
 
 
 def _fresh(like, rows, width):
-    """A dense tensor like `like` (whose last axis is `width`) and its (pointer, floats from row to row)."""
-    t = torch.empty_like(like, memory_format=_DENSE)
-    return t, (t.data_ptr(), width if rows > 1 else (width + 3) // 4 * 4)
+    """A dense tensor like `like` (whose last axis is `width`; rows of a width that is no multiple of four are
+    padded to one) and its (pointer, floats from row to row)."""
+    wide = (width + 3) // 4 * 4
+    if wide != width and rows > 1:
+        t = like.new_empty((*like.shape[:-1], wide))[..., :width]
+    else:
+        t = torch.empty_like(like, memory_format=_DENSE)
+    return t, (t.data_ptr(), wide)
 
 
 def _pos(pos):

@@ -373,3 +373,21 @@ def test_rotation_by_a_scaled_angle_rounds_once(gpu):
         want = f(ang) * float(np.float32(mscale))
         # half a step, and what the angle's rounding to a double (2 10^4 radians: 2e-12) leaves near a border
         assert np.all(np.abs(got[..., e] - want) <= np.spacing(np.abs(want).astype(np.float32)) / 2.0 + 1e-11)
+
+
+def test_padded_rows_of_odd_widths(gpu):
+    """Rows of 18 and 6 values, 16-byte aligned by padding: outputs made by the call as well as given ones."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(2)
+    buf = torch.from_numpy(g.standard_normal((2, 5, 28)).astype(np.float32)).to(gpu)
+    q, k = buf[..., :18], buf[..., 20:26]
+    pos = torch.arange(10, dtype=torch.int32, device=gpu).view(2, 5)
+    freq = ops.rope_table(6, 1e4)[0].to(gpu)
+    want = [torch.zeros(2, 5, n, device=gpu) for n in (20, 8)]
+    ops.qk_norm_rope_tokens(q, k, None, pos, freq, 6, q_out=want[0][..., :18], k_out=want[1][..., :6])
+    y, tol = expected(q.cpu().numpy().reshape(10, 3, 6), None, pos.cpu().numpy().reshape(-1), freq.cpu().numpy(), 6, False, 1.0, 1e-6)
+    assert np.all(np.abs(want[0][..., :18].cpu().numpy().reshape(y.shape) - y) <= tol + 1e-30)
+    got = ops.qk_norm_rope_tokens(q, k, None, pos, freq, 6, want_k=True)
+    assert got[0].shape == q.shape and got[1].shape == k.shape
+    assert torch.equal(got[0], want[0][..., :18]) and torch.equal(got[1], want[1][..., :6])
