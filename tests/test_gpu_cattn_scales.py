@@ -1,8 +1,10 @@
 """lg_attn_cache over the sizes that queries may have: small ones in tiles that a row does not
-see or whose scores lie far below."""
+see or whose scores lie far below, large ones of which one key takes all, and the 22 bits
+that queries and weights keep."""
 import numpy as np
 import pytest
 
+from ligguf_amd import lib as L
 from test_gpu_cattn import TYPES, U, check, make
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +52,82 @@ def test_small_queries_after_keys_far_below(gpu, ctype, ntok):
             p = np.exp(a - a.max())
             p /= p.sum()
             assert np.all(np.abs(got[0, t, h] - p @ v) <= (2 * len(k) + 168) * U * (p @ np.abs(v)))
+
+
+@pytest.mark.parametrize("ctype", TYPES)
+def test_large_queries_give_the_top_keys_value(gpu, ctype):
+    """Scores of 10^6 and more, whose highest lies thousands above the next: its value, off by the
+    parts of its weight (4 U), the sum's and the quotient's roundings."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(1)
+    for hd in (64, 128, 256):
+        for ntok, n_ctx in ((1, 300), (40, 300), (2, 5000)):
+            cache, (K, V) = make(gpu, ctype, 1, n_ctx, 2, hd, g)
+            q = (g.standard_normal((1, ntok, 4, hd)) * 1e6).astype(np.float32)
+            pos = np.arange(n_ctx - ntok, n_ctx, dtype=np.int32)[None]
+            got = ops.attention_cache(torch.from_numpy(q.reshape(1, ntok, -1)).to(gpu), cache, torch.from_numpy(pos).to(gpu))
+            got = got.cpu().numpy().reshape(q.shape)
+            seen = 0
+            for t in range(ntok):
+                for h in range(4):
+                    a = K[0, :pos[0, t] + 1, h // 2] @ q[0, t, h].astype(np.float64) / np.sqrt(hd)
+                    top = np.sort(a)[-2:]
+                    if top[1] - top[0] < 3000:    # (scores of 10^7 are 1 or so off in fp32)
+                        continue
+                    v = V[0, a.argmax(), h // 2]
+                    assert np.all(np.abs(got[0, t, h] - v) <= 16 * U * np.abs(v))
+                    seen += 1
+            assert seen >= 2 * ntok
+
+
+def in_half(x):
+    """x as the first fp16 part alone would hold it, under the power of two of its largest value."""
+    e = np.frexp(np.abs(x).max(-1, keepdims=True))[1]
+    return np.ldexp(np.ldexp(x, 14 - e).astype(np.float16).astype(np.float64), e - 14)
+
+
+@pytest.mark.parametrize("ctype,hd", [(L.F16, 48), (L.F16, 64), (L.F16, 128), (L.F16, 256), (L.KV4, 64), (L.KV4, 128), (L.KV4, 256)])
+@pytest.mark.parametrize("ntok,n_ctx", [(1, 300), (1, 5000), (4, 5000), (60, 300), (60, 5000)])
+def test_queries_and_weights_keep_22_bits(gpu, ctype, hd, ntok, n_ctx):
+    """40 keys, spread over the context, of one value each, in dims of their own, with scores within
+    4; the rest lie 200 below and have no weight.  So a score is one product, off by the parts of the
+    query value (4 nats x 4 U, and 2 U of its own for 4-bit values), and an output is one weight by
+    the sum: 8 nats x 2.5 U of the scale's rounding, 6 U of the exponent's (up to 16), 2 U of exp2, 4 U
+    of the weight's parts, 3 U each for at most 40 rescalings by a new maximum, 18 U for two joins, 2 U for
+    the quotient: 190 U, as much for the sum, and 50 U of its additions.  One part alone is off by
+    up to 2^12 U."""
+    import torch
+    from ligguf_amd import ops
+    g = np.random.default_rng(hd + n_ctx)
+    n, heads, kv = 40, 8, 2
+    at = np.linspace(3, n_ctx - ntok, n).astype(int)
+    dims = np.stack([1 + g.permutation(hd - 1)[:n] for _ in range(kv)])
+
+    def edit(which, x):
+        if which == 0:
+            x[:] = 0
+            x[0, :, :, 0] = -64 * np.sqrt(hd) / 8
+        x[0, at] = 0
+        for k in range(kv):
+            x[0, at, k, dims[k]] = 1
+    cache, (K, V) = make(gpu, ctype, 1, n_ctx, kv, hd, g, edit)
+    q = g.uniform(-4, 4, (1, ntok, heads, hd)) * np.sqrt(hd)
+    q[..., 0] = 32
+    q = q.astype(np.float32)
+    pos = np.arange(n_ctx - ntok, n_ctx, dtype=np.int32)[None]
+    got = ops.attention_cache(torch.from_numpy(q.reshape(1, ntok, -1)).to(gpu), cache, torch.from_numpy(pos).to(gpu))
+    got = got.cpu().numpy().reshape(q.shape).astype(np.float64)
+
+    def weights(q, part):
+        k = np.stack([K[0, at, h * kv // heads] for h in range(heads)])
+        a = (k[None] @ q[0].astype(np.float64)[..., None])[..., 0] / np.sqrt(hd)
+        p = np.exp(a - a.max(-1, keepdims=True))
+        return (in_half(p) if part else p) / p.sum(-1, keepdims=True)
+    want, tol = weights(q, False), 450 * U
+    val = np.stack([V[0, at, h * kv // heads, dims[h * kv // heads]] for h in range(heads)])
+    out = np.stack([got[0, :, h, dims[h * kv // heads]].T for h in range(heads)], 1)
+    assert np.abs(out / val / want - 1).max() <= tol
+    # what the bound is for: it would not hold with one part
+    assert np.abs(weights(in_half(q.astype(np.float64)), False) / want - 1).max() > 4 * tol
+    assert np.abs(weights(q, True) / want - 1).max() > 4 * tol

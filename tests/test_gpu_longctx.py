@@ -170,3 +170,31 @@ def test_over_a_contexts_logits(gpu):
         assert max(abs(a[1] - ref[a[0]]) for a in alts) <= near
     assert eng.logprobs(77)[2] == []
     eng.close()
+
+
+@pytest.mark.parametrize("ctype", [L.F16, L.KV4])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+def test_tokens_one_by_one(gpu, ctype, window, sinks):
+    """Every step of a conversation of single tokens against the formulas over its own cache, and that
+    cache against a prompt's.  The rows of both come from torch products of another shape, which differ in
+    the last bits: an fp16 value is off by one rounding, a 4-bit one by one code (a step of d, a fifteenth
+    of its group's range) and the roundings of d at 15 and of m."""
+    import torch
+    toy, one = Toy(gpu, ctype, window, sinks), Toy(gpu, ctype, window, sinks)
+    toks = torch.randint(0, VOCAB, (2, 150), generator=torch.Generator().manual_seed(5)).int().to(gpu)
+    pos = torch.arange(150, dtype=torch.int32, device=gpu).repeat(2, 1)
+    pos[1, 97:] = -1
+    toy.step(toks, pos)
+    for t in range(150):
+        p = pos[:, t:t + 1].contiguous()
+        check(one, p, one.step(toks[:, t:t + 1].contiguous(), p))
+    for a, b in zip(toy.values(), one.values()):
+        assert not a[0, 150:].any() and not a[1, 97:].any() and not b[0, 150:].any() and not b[1, 97:].any()
+        x, y = (z.reshape(2, -1, KV, HD // 32, 32) for z in (a, b))
+        top = np.abs(y).max(-1, keepdims=True)
+        if ctype == L.F16:
+            near = np.abs(y) * 2.0 ** -10 + 2.0 ** -24
+        else:
+            near = (y.max(-1, keepdims=True) - y.min(-1, keepdims=True)) / 15 * (1 + 16 * 2.0 ** -10) + 3 * 2.0 ** -10 * top + 2.0 ** -20
+        # (the products' own difference, 128 terms of fp32, is far below)
+        assert np.all(np.abs(x - y) <= near + 1e-5 * top)
