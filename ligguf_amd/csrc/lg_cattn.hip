@@ -206,8 +206,8 @@ __device__ __forceinline__ float2& ca_part_ml(const CAttn& a, int nsplit, float*
  * survive whatever their size.  The loads of one tile run while the last one
  * computes.  fp16 is bound by the cache's bytes (32 heads of 128, 8 key heads:
  * 64 sequences of 2000 rows 100 us, 5.2 TB/s; 24 ragged ones of up to 12000
- * 134 us, 4.6 TB/s); 4 bits by bytes and by VALU work, 59 % of the cycles (64 of
- * 2000 rows 36 us, 4.5 TB/s; 40 ragged ones 101 us, 3.6 TB/s), most of it the 13
+ * 131 to 143 us on several cards, 4.3 to 4.6 TB/s); 4 bits by bytes and by VALU work, 62 % of the cycles (64 of
+ * 2000 rows 36 us, 4.5 TB/s; 40 ragged ones 104 us, 3.9 TB/s), most of it the 13
  * operations for eight values: of 16 columns four are used. */
 template <int HD, bool KV4>
 struct CaDec {
@@ -514,7 +514,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAtt
  * are the lane's k of step s of the second product: keys 16s + 4h .. and
  * 16s + 8 + 4h .. of lane half h.  The next tile is on its way while one
  * computes (two LDS stages, one barrier a tile).  Bound by the MFMA and VALU
- * work of a SIMD's two waves, 52 % and 42 % of the cycles, at 2.04 of 2.4 GHz
+ * work of a SIMD's two waves, 51 % and 44 % of the cycles, at 2.04 of 2.4 GHz
  * (keeping the waves half a tile apart, products and softmax interleaved by
  * hand, or V's fragments read a step ahead was no faster): 2000 tokens over
  * windows of 4096 rows 260 us, 520 TFLOP/s of the products asked for, 1040 issued

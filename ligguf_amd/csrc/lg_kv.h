@@ -33,8 +33,8 @@ __device__ __forceinline__ size_t lg_kv4_dm(const LgKv& c, int g, int pos)
     return (size_t)c.n_kv * c.n_ctx * (c.hd / 2) + ((size_t)g * c.n_ctx + pos) * (c.hd / 8);
 }
 
-/* the eight fp16 values of a word of codes: 2j, 2j + 1 in v[j].  A code under
- * the exponent of 1024 is 1024 + c (in bits 0..3) or 1024 + 16 c (4..7); taking
+/* the eight fp16 values of a word of codes: 2j, 2j + 1 in v[j], by the published
+ * method of products of fp16 by 4-bit weights.  A code under the exponent of 1024 is 1024 + c (in bits 0..3) or 1024 + 16 c (4..7); taking
  * the 1024 off, for the latter as x / 16 - 64, is exact.  c d + m is one fused
  * fp16 multiply-add, the one rounding that the format has.  The constants are
  * kept in registers: v_and_or_b32 takes no literal, and as literals they cost

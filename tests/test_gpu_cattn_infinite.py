@@ -23,7 +23,7 @@ def plain(q, K, V, pos):
             g = h * K.shape[1] // heads
             k, v = K[:pos[t] + 1, g], V[:pos[t] + 1, g]
             with np.errstate(invalid="ignore"):
-                a = np.array([(x * q[t, h].astype(np.float64)).sum() for x in k]) / np.sqrt(hd)
+                a = (k * q[t, h].astype(np.float64)).sum(1) / np.sqrt(hd)
                 p = np.exp(a - a.max())
                 p = p / p.sum()
                 out[t, h] = p @ v
