@@ -115,7 +115,8 @@ struct CaMax {
         *off = far(c) ? mn : 0.0f;
         return al;
     }
-    /* the power of two that weights are multiples of, for sums to be joined; l: the sum of weights */
+    /* the power of two that weights are multiples of, for sums to be joined; l: the sum of weights.  (Of far columns
+     * as rounded: off by up to 2^-24 of itself, less than scores of that size are by their 22 bits.) */
     __device__ __forceinline__ float unit(float l) const
     {
         const float c = __builtin_fmaf(-m, sc, 14.0f);
