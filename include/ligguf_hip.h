@@ -506,6 +506,84 @@ int lg_logprobs(const float* logits, int64_t stride, int rows, int vocab, const 
                 float* entropy, int* top_id, float* top_logprob, void* stream);
 
 /* ===================================================================== */
+/* Several continuations of one prompt (device pointers, asynchronous)    */
+/* ===================================================================== */
+/* Beams, samples of one question, questions about one document: sequences
+ * whose caches lie in pages, so that they can hold the same rows without
+ * copies of them.  Conventions as above; no counterpart in the reference.
+ *
+ * A layer's caches in pages: page i < n_pages is "sequence" i of `pool`, whose
+ * n_ctx is the rows of a page (a power of two, 16 .. 65536; seq_bytes below 2^32).  Row j of
+ * sequence s is row j % n_ctx of page table[s * table_stride + j / n_ctx]
+ * (device memory, read by the kernels); entries outside 0 .. n_pages - 1 are no
+ * pages.  A table row has max_pages entries that may be read, max_pages * n_ctx
+ * <= 2^30. */
+typedef struct {
+    lg_kv_cache pool;
+    int32_t n_pages, max_pages;
+    const int32_t* table;
+    int64_t table_stride;
+} lg_kv_pages;
+
+/* lg_qk_norm_rope_tokens with the cache write into pages: row r is written
+ * where its sequence's table has position pos[r], and is not written where it
+ * has no page there.  Positions from max_pages * n_ctx on hold no token.  No
+ * two rows of a call may be written to the same place: pages that several
+ * sequences hold are not written by more than one of them. */
+int lg_qk_norm_rope_paged(const float* q, int64_t q_stride, float* q_out, int64_t q_out_stride, const float* k,
+                          int64_t k_stride, float* k_out, int64_t k_out_stride, const float* v, int64_t v_stride,
+                          const float* qw, const float* kw, int n_heads, int n_kv_heads, int head_dim, int rope_dim,
+                          int layout, const float* freq, float mscale, float eps, const int* pos, int nseq, int ntok,
+                          const lg_kv_pages* cache, void* stream);
+
+/* lg_attn_cache over pages.  With prefix (device memory, one for each `group`
+ * sequences; nseq is a multiple of group) the sequences of a group share
+ * their first rows: rows j < prefix[g] are read from the pages of its first
+ * sequence, once for all of them, the others from each sequence's own; values
+ * outside 0 .. max_prefix count as the nearest.  NULL or max_prefix 0: nothing is
+ * shared.  Keys without a page are not seen.  A row's head is zeros where no
+ * key that it sees has a weight (none seen, or all at -infinity).  max_pos <
+ * max_pages * n_ctx. */
+size_t lg_attn_paged_workspace_size(const lg_kv_pages* cache, int nseq, int ntok, int n_heads, int window, int sinks,
+                                    int max_pos, int group, int max_prefix);
+int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages* cache, const int* pos, int nseq, int ntok,
+                  int n_heads, int window, int sinks, int max_pos, const int* prefix, int group, int max_prefix,
+                  float* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The best continuations of each of ngroups groups of `beams` rows of logits
+ * (rows as lg_logprobs takes them): candidate (b, t) has the score
+ *   scores[b] + log softmax(row b)[t]
+ * and the `top` highest, ties by the lower beam, then by the higher logit and the lower
+ * token, go to score, parent (the beam, 0 .. beams - 1) and token, [ngroups][top]
+ * each.  With done (may be NULL), a beam whose done is not 0 has the one
+ * candidate (b, end) of score scores[b]; its logits are not read.  No
+ * candidates: scores and sums that are no finite numbers (an idle beam has
+ * -infinity), logits of -infinity.  Where there are fewer than top, the rest is
+ * (-infinity, -1, -1).  Sums and scores are joined in double and rounded once.
+ * beams and top are 1 .. 64.  workspace as lg_attn_cache. */
+#define LG_BEAMS_MAX 64
+size_t lg_beam_select_workspace_size(int ngroups, int beams, int vocab, int top);
+int lg_beam_select(const float* logits, int64_t stride, const float* scores, const int* done, int end, int ngroups,
+                   int beams, int vocab, int top, float* score, int* parent, int* token, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* The tables of chosen beams, in place: beam i of group g goes on from beam
+ * parent[g * beams + i] of its group (from itself where parent is outside
+ * 0 .. beams - 1), each of which holds length[g] rows in every layer.  With n
+ * = length / n_ctx full pages and r = length % n_ctx rows in the next:
+ *   - entries 0 .. n - 1 of i's row become the parent's;
+ *   - if r > 0, entry n: the first beam to go on from a parent takes its page,
+ *     the others, in order, the pages of those from which none goes on, and
+ *     rows 0 .. r - 1 of the parent's page are copied there, keys and values,
+ *     in each of the n_pools layers (their pools are alike; one table for all).
+ * Entries behind are left as they are.  The pages at entry n have to differ
+ * within a group.  A group whose length is outside 0 .. max_pages * n_ctx is
+ * left as it is.  workspace: 16 bytes a sequence, as lg_attn_cache. */
+int lg_beam_reorder(const lg_kv_cache* pools, int n_pools, int n_pages, int32_t* table, int64_t table_stride,
+                    int max_pages, const int* parent, const int* length, int ngroups, int beams, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* ===================================================================== */
 /* BERT sentence embedding and the vector memory (fast/vdb.cpp)           */
 /* ===================================================================== */
 /* The chat driver's retrieval memory embeds every logged user turn and each

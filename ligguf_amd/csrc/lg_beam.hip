@@ -1,0 +1,362 @@
+/* lg_beam.hip -- the best continuations over beams and vocabulary, and the page
+ * tables of the chosen ones. */
+#include <algorithm>
+
+#include "lg_kv.h"
+#include "lg_topk.h"
+
+struct BeamArgs {
+    const float *logits, *scores;
+    const int* done;
+    int64_t stride;
+    int end, beams, vocab, top, parts, part;   /* a row in `parts` of `part` logits (the last one fewer) */
+    float2* mz;       /* of each row's parts: maximum, sum of e^(x - m) */
+    uint64_t* keys;   /* and its highest entries (lp_key), `top` places each */
+    float* score;
+    int *parent, *token;
+};
+
+/* whether a row's logits are read: an unfinished beam that has a score */
+__device__ __forceinline__ bool bm_live(const BeamArgs& a, int64_t row)
+{
+    return fabsf(a.scores[row]) <= FLT_MAX && !(a.done && a.done[row]);
+}
+
+constexpr float BM_LOG2E = 1.44269504088896341f;
+
+/* A part of a row: its maximum, the sum of e^(x - m) and its `top` highest
+ * entries in order. */
+template <int T>
+__global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
+{
+    __shared__ LpShared s;
+    const int64_t row = blockIdx.x / a.parts;
+    const int part = blockIdx.x % a.parts, t = threadIdx.x;
+    if (!bm_live(a, row)) return;
+    const int first = part * a.part, n = min(a.part, a.vocab - first);
+    const LpRow r(a.logits + row * a.stride + first, n);
+    const int nq = r.quads();
+    float m = -FLT_MAX, z = 0.0f, mine = -INFINITY;
+    for (int q = t; q < nq; q += T) {
+        const float4 v = r.load(q);
+        mine = fmaxf(fmaxf(mine, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+        const float mn = fmaxf(m, mine);
+        z *= __builtin_amdgcn_exp2f((m - mn) * BM_LOG2E);
+        m = mn;
+        z += (__builtin_amdgcn_exp2f((v.x - m) * BM_LOG2E) + __builtin_amdgcn_exp2f((v.y - m) * BM_LOG2E)) +
+             (__builtin_amdgcn_exp2f((v.z - m) * BM_LOG2E) + __builtin_amdgcn_exp2f((v.w - m) * BM_LOG2E));
+    }
+    const uint32_t ord = lp_ord(mine);
+    {   /* of T / 256 neighbours */
+        uint32_t o = ord;
+        if constexpr (T >= 512) o = max(o, (uint32_t)lg_partner<0>((int)o));
+        if constexpr (T >= 1024) o = max(o, (uint32_t)lg_partner<1>((int)o));
+        if (t % (T / 256) == 0) s.top[t / (T / 256)] = o;
+    }
+    auto join = [&]() {   /* m, z over the wave */
+        const float M = lg_group_max<64>(m);
+        z = lg_group_sum<64>(z * __builtin_amdgcn_exp2f(fmaxf(m - M, -1e30f) * BM_LOG2E));
+        m = M;
+    };
+    join();
+    if (t % 64 == 0) s.sums[t / 64] = make_float4(m, z, 0.0f, 0.0f);
+    __syncthreads();
+    {
+        const float4 v = t % 64 < T / 64 ? s.sums[t % 64] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
+        m = v.x;
+        z = v.y;
+        join();
+    }
+    const int64_t at = row * a.parts + part;
+    if (t == 0) a.mz[at] = make_float2(m, z);
+    const int top = min(a.top, n);
+    const int c = lp_top<T>(s, r, nq, 0, top, ord, z != z);
+    lp_emit<T>(s, c, top, [&](int rank, uint64_t k) { a.keys[at * a.top + rank] = k - (uint32_t)first; });   /* (~id - first = ~(id + first)) */
+}
+
+/* A group: log sums of its beams' parts, then every part's entries as scores in
+ * double.  The entries of a part are in order, so those ahead of one are counted
+ * list by list, by halving. */
+__global__ __launch_bounds__(256) void k_beam_group(BeamArgs a)
+{
+    extern __shared__ double s_score[];   /* [beams][parts][top] */
+    __shared__ double s_off[LG_BEAMS_MAX];
+    __shared__ int s_kind[LG_BEAMS_MAX], s_n;   /* 0: no candidates, 1: logits, 2: finished */
+    const int64_t row0 = (int64_t)blockIdx.x * a.beams;
+    const int t = threadIdx.x, lists = a.beams * a.parts;
+    if (t < a.beams) {
+        const float sc = a.scores[row0 + t];
+        int kind = 0;
+        double off = 0.0;
+        if (fabsf(sc) <= FLT_MAX) {
+            if (a.done && a.done[row0 + t]) kind = 2;
+            else {
+                const float2* const mz = a.mz + (row0 + t) * a.parts;
+                float M = -FLT_MAX;
+                for (int p = 0; p < a.parts; p++) M = fmaxf(M, mz[p].x);
+                double z = 0.0;
+                for (int p = 0; p < a.parts; p++) z += mz[p].y * exp((double)mz[p].x - (double)M);
+                off = (double)M + log(z);
+                kind = fabs(off) <= (double)FLT_MAX ? 1 : 0;   /* (no NaN, no infinity) */
+            }
+        }
+        s_kind[t] = kind;
+        s_off[t] = kind == 2 ? -(double)sc : off;
+    }
+    if (t == 0) s_n = 0;
+    __syncthreads();
+    const int64_t key0 = row0 * a.parts * a.top;
+    auto held = [&](int l) { return min(a.top, min(a.part, a.vocab - l % a.parts * a.part)); };   /* entries of list l */
+    for (int i = t; i < lists * a.top; i += 256) {
+        const int l = i / a.top, b = l / a.parts;
+        double v = -INFINITY;
+        if (s_kind[b] == 1 && i % a.top < held(l))
+            v = (double)a.scores[row0 + b] + ((double)lp_value(a.keys[key0 + i]) - s_off[b]);
+        if (s_kind[b] == 2 && i % (a.top * a.parts) == 0) v = -s_off[b];
+        s_score[i] = v;
+    }
+    __syncthreads();
+    for (int i = t; i < lists * a.top; i += 256) {
+        const double v = s_score[i];
+        if (!(v > -INFINITY)) continue;
+        const int l = i / a.top, b = l / a.parts;
+        int rank = i % a.top;
+        for (int o = 0; o < lists && rank < a.top; o++) {
+            if (o == l) continue;
+            /* entries of list o ahead of this one: the higher ones, and equal ones of a lower beam or, of the
+             * same beam, of a higher logit or a lower token */
+            int lo = 0, hi = a.top;
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                const double w = s_score[o * a.top + mid];
+                bool ahead = w > v;
+                if (w == v) ahead = o / a.parts != b ? o < l : a.keys[key0 + o * a.top + mid] > a.keys[key0 + i];
+                if (ahead) lo = mid + 1;
+                else hi = mid;
+            }
+            rank += lo;
+        }
+        if (rank < a.top) {
+            const int64_t at = (int64_t)blockIdx.x * a.top + rank;
+            a.score[at] = (float)v;
+            a.parent[at] = b;
+            a.token[at] = s_kind[b] == 2 ? a.end : (int)~(uint32_t)a.keys[key0 + i];
+            atomicAdd(&s_n, 1);
+        }
+    }
+    __syncthreads();
+    if (t >= s_n && t < a.top) {
+        const int64_t at = (int64_t)blockIdx.x * a.top + t;
+        a.score[at] = -INFINITY;
+        a.parent[at] = -1;
+        a.token[at] = -1;
+    }
+}
+
+/* Parts of a row: enough of them for the 256 CUs, of 4096 logits at least; and the
+ * entries of a group's parts, which a workgroup holds as doubles, at most 4096
+ * (more where one part a beam has them). */
+static int bm_parts(int64_t rows, int beams, int vocab, int top)
+{
+    const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(rows, 1));
+    return (int)std::max<int64_t>(1, std::min({want, (int64_t)vocab / 4096, (int64_t)4096 / ((int64_t)beams * top)}));
+}
+
+static bool bm_sizes(int ngroups, int beams, int vocab, int top)
+{
+    return ngroups >= 0 && beams > 0 && beams <= LG_BEAMS_MAX && top > 0 && top <= LG_BEAMS_MAX && vocab > 0 &&
+           vocab <= INT32_MAX - 16;
+}
+
+extern "C" size_t lg_beam_select_workspace_size(int ngroups, int beams, int vocab, int top)
+{
+    if (!bm_sizes(ngroups, beams, vocab, top)) return 0;
+    const int64_t rows = (int64_t)ngroups * beams;
+    return (size_t)rows * bm_parts(rows, beams, vocab, top) * (sizeof(float2) + 8 * (size_t)top);
+}
+
+extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* scores, const int* done, int end, int ngroups,
+                              int beams, int vocab, int top, float* score, int* parent, int* token, void* workspace,
+                              size_t workspace_bytes, void* stream)
+{
+    const char* who = "lg_beam_select";
+    if (!bm_sizes(ngroups, beams, vocab, top) || stride < vocab) {
+        lg_set_error("%s: bad sizes (%d groups of %d beams, rows of %d, %lld apart, top %d)", who, ngroups, beams, vocab,
+                     (long long)stride, top);
+        return LG_ERR_ARG;
+    }
+    if (!ngroups) return LG_OK;
+    if (!logits || ((uintptr_t)logits & 3) || !scores || !score || !parent || !token) {
+        lg_set_error("%s: logits, scores and outputs must be given", who);
+        return LG_ERR_ARG;
+    }
+    const int64_t rows = (int64_t)ngroups * beams;
+    BeamArgs a = {logits, scores, done, stride, end, beams, vocab, top, bm_parts(rows, beams, vocab, top), 0, nullptr, nullptr,
+                  score, parent, token};
+    /* (parts begin 16 bytes apart, so that all are as aligned as the row) */
+    a.part = (vocab / a.parts + 4) & ~3;
+    if ((int64_t)a.part * (a.parts - 1) >= vocab) a.part = (vocab + a.parts - 1) / a.parts;
+    if (!lg_grid_fits(rows * a.parts, 1024)) {
+        lg_set_error("%s: %lld rows are too many for one call", who, (long long)rows);
+        return LG_ERR_ARG;
+    }
+    const size_t need = lg_beam_select_workspace_size(ngroups, beams, vocab, top);
+    if (!workspace || !lg_al16(workspace) || workspace_bytes < need) {
+        lg_set_error("%s: workspace of %zu bytes, 16-byte aligned, %zu needed", who, workspace_bytes, need);
+        return LG_ERR_ARG;
+    }
+    a.mz = (float2*)workspace;
+    a.keys = (uint64_t*)(a.mz + rows * a.parts);
+    hipStream_t s = (hipStream_t)stream;
+    const int lists = beams * a.parts * top;
+    k_beam_rows<1024><<<(unsigned)(rows * a.parts), 1024, 0, s>>>(a);
+    k_beam_group<<<ngroups, 256, lists * sizeof(double), s>>>(a);
+    return lg_check_launch(who);
+}
+
+/* ---- the tables of chosen beams ---- */
+
+struct ReorderArgs {
+    int* table;
+    int64_t tstride;
+    const int *parent, *length;
+    int beams, max_pages, n_pages, shift;
+    int4* jobs;   /* of each sequence: copy rows 0 .. z - 1 of page x to page y */
+};
+
+constexpr int BM_ENTRIES = 64;   /* table entries of a group's beams that LDS holds at a time */
+
+/* A group: who takes which part-filled page, then the full pages' entries. */
+__global__ __launch_bounds__(256) void k_beam_tables(ReorderArgs a)
+{
+    __shared__ int s_par[LG_BEAMS_MAX], s_page[LG_BEAMS_MAX], s_spare[LG_BEAMS_MAX], s_tab[LG_BEAMS_MAX][BM_ENTRIES];
+    const int g = blockIdx.x, t = threadIdx.x, len = a.length[g];
+    int* const table = a.table + (int64_t)g * a.beams * a.tstride;
+    const bool on = len >= 0 && len <= a.max_pages << a.shift;
+    const int n = on ? len >> a.shift : 0, rows = on ? len & ((1 << a.shift) - 1) : 0;
+    if (t < a.beams) {
+        const int p = a.parent[g * a.beams + t];
+        s_par[t] = (uint32_t)p < (uint32_t)a.beams ? p : t;
+        s_page[t] = rows ? table[t * a.tstride + n] : 0;
+    }
+    __syncthreads();
+    if (t < 64) {   /* a lane a beam */
+        const int par = t < a.beams ? s_par[t] : -1;
+        bool first = true, none = true;
+        for (int i = 0; i < a.beams; i++) {
+            if (i < t && s_par[i] == par) first = false;
+            if (s_par[i] == t) none = false;
+        }
+        const uint64_t below = ((uint64_t)1 << t) - 1;
+        const uint64_t others = __builtin_amdgcn_ballot_w64(t < a.beams && !first);
+        const uint64_t spare = __builtin_amdgcn_ballot_w64(t < a.beams && none);
+        if (t < a.beams && none) s_spare[__builtin_popcountll(spare & below)] = s_page[t];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (t < a.beams) {
+            const int src = s_page[par], dst = first ? src : s_spare[__builtin_popcountll(others & below)];
+            if (rows) table[t * a.tstride + n] = dst;
+            const bool copy = rows && !first && (uint32_t)src < (uint32_t)a.n_pages && (uint32_t)dst < (uint32_t)a.n_pages && src != dst;
+            a.jobs[g * a.beams + t] = make_int4(src, dst, copy ? rows : 0, 0);
+        }
+    }
+    for (int e0 = 0; e0 < n; e0 += BM_ENTRIES) {
+        const int w = min(BM_ENTRIES, n - e0);
+        for (int i = t; i < a.beams * BM_ENTRIES; i += 256) {
+            const int b = i / BM_ENTRIES, e = i % BM_ENTRIES;
+            if (e < w) s_tab[b][e] = table[b * a.tstride + e0 + e];
+        }
+        __syncthreads();
+        for (int i = t; i < a.beams * BM_ENTRIES; i += 256) {
+            const int b = i / BM_ENTRIES, e = i % BM_ENTRIES, p = s_par[b];
+            if (e < w && p != b) table[b * a.tstride + e0 + e] = s_tab[p][e];
+        }
+        __syncthreads();
+    }
+}
+
+constexpr int BM_POOLS = 64;   /* layers a launch */
+
+struct CopyArgs {
+    uint8_t* pool[BM_POOLS][2];
+    const int4* jobs;
+    LgKv c;
+};
+
+/* rows of a page: [rows][n_kv][hd] fp16 are one run, 4-bit ones a run of codes and
+ * one of pairs for each head */
+__global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a)
+{
+    const int4 j = a.jobs[blockIdx.x];
+    if (!j.z) return;
+    uint8_t* const p = a.pool[blockIdx.y][blockIdx.z];
+    const uint8_t* const src = p + (size_t)j.x * a.c.seq;
+    uint8_t* const dst = p + (size_t)j.y * a.c.seq;
+    auto run = [&](size_t at, int bytes) {   /* multiples of 4: an fp16 row of an odd number of heads may be 4 bytes */
+        for (int i = threadIdx.x * 4; i < bytes; i += 1024) *(uint32_t*)(dst + at + i) = *(const uint32_t*)(src + at + i);
+    };
+    if (a.c.type == LG_F16) run(0, j.z * a.c.n_kv * a.c.hd * 2);
+    else
+        for (int g = 0; g < a.c.n_kv; g++) {
+            run(lg_kv4_codes(a.c, g, 0), j.z * (a.c.hd / 2));
+            run(lg_kv4_dm(a.c, g, 0), j.z * (a.c.hd / 8));
+        }
+}
+
+extern "C" int lg_beam_reorder(const lg_kv_cache* pools, int n_pools, int n_pages, int32_t* table, int64_t table_stride,
+                               int max_pages, const int* parent, const int* length, int ngroups, int beams, void* workspace,
+                               size_t workspace_bytes, void* stream)
+{
+    const char* who = "lg_beam_reorder";
+    if (!pools || n_pools < 1 || ngroups < 0 || beams < 1 || beams > LG_BEAMS_MAX) {
+        lg_set_error("%s: bad argument (%d layers, %d groups of %d beams)", who, n_pools, ngroups, beams);
+        return LG_ERR_ARG;
+    }
+    ReorderArgs r = {table, table_stride, parent, length, beams, max_pages, n_pages, 0, (int4*)workspace};
+    CopyArgs c = {};
+    for (int i = 0; i < n_pools; i++) {
+        const lg_kv_pages p = {pools[i], n_pages, max_pages, table, table_stride};
+        const int rc = lg_kv_pages_arg(&p, who, &c.c, &r.shift);
+        if (rc) return rc;
+        if (pools[i].type != pools[0].type || pools[i].n_ctx != pools[0].n_ctx || pools[i].n_kv_heads != pools[0].n_kv_heads ||
+            pools[i].head_dim != pools[0].head_dim || pools[i].seq_bytes != pools[0].seq_bytes) {
+            lg_set_error("%s: layer %d has other pages than the first", who, i);
+            return LG_ERR_ARG;
+        }
+    }
+    if (c.c.type == LG_F16 && c.c.hd % 2) {
+        lg_set_error("%s: heads of %d values", who, c.c.hd);
+        return LG_ERR_ARG;
+    }
+    if ((int64_t)c.c.n_ctx * c.c.n_kv * c.c.hd * 2 > INT32_MAX - 1024) {
+        lg_set_error("%s: pages of %d rows of %d heads are too large", who, c.c.n_ctx, c.c.n_kv);
+        return LG_ERR_ARG;
+    }
+    if (!ngroups) return LG_OK;
+    if (!parent || !length) {
+        lg_set_error("%s: parents and lengths must be given", who);
+        return LG_ERR_ARG;
+    }
+    const int64_t nseq = (int64_t)ngroups * beams;
+    if (!lg_grid_fits(nseq, 256)) {
+        lg_set_error("%s: %lld sequences are too many for one call", who, (long long)nseq);
+        return LG_ERR_ARG;
+    }
+    if (!workspace || !lg_al16(workspace) || workspace_bytes < (size_t)nseq * sizeof(int4)) {
+        lg_set_error("%s: workspace of %zu bytes, 16-byte aligned, %zu needed", who, workspace_bytes, (size_t)nseq * sizeof(int4));
+        return LG_ERR_ARG;
+    }
+    hipStream_t s = (hipStream_t)stream;
+    k_beam_tables<<<ngroups, 256, 0, s>>>(r);
+    c.jobs = r.jobs;
+    for (int l = 0; l < n_pools; l += BM_POOLS) {
+        const int n = std::min(BM_POOLS, n_pools - l);
+        for (int i = 0; i < n; i++) {
+            c.pool[i][0] = (uint8_t*)pools[l + i].k;
+            c.pool[i][1] = (uint8_t*)pools[l + i].v;
+        }
+        k_beam_copy<<<dim3((unsigned)nseq, n, 2), 256, 0, s>>>(c);
+    }
+    return lg_check_launch(who);
+}

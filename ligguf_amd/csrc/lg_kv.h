@@ -16,6 +16,9 @@ struct LgKv {
 /* LG_OK, or the refusal of a cache that a call names (nseq sequences) */
 int lg_kv_arg(const lg_kv_cache* c, int nseq, const char* who, LgKv* out);
 
+/* LG_OK, or the refusal of caches in pages; *out their pool, a page per sequence */
+int lg_kv_pages_arg(const lg_kv_pages* c, const char* who, LgKv* out, int* shift);
+
 static inline bool lg_al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 /* byte offsets within one sequence: a head's fp16 row; its codes and its

@@ -40,6 +40,27 @@ int lg_kv_arg(const lg_kv_cache* c, int nseq, const char* who, LgKv* out)
     return LG_OK;
 }
 
+int lg_kv_pages_arg(const lg_kv_pages* c, const char* who, LgKv* out, int* shift)
+{
+    const int rc = lg_kv_arg(&c->pool, c->n_pages, who, out);
+    if (rc) return rc;
+    const int n = c->pool.n_ctx;
+    if (n < 16 || n > 65536 || (n & (n - 1)) || c->pool.seq_bytes > UINT32_MAX) {
+        lg_set_error("%s: pages of %d rows, %zu bytes (a power of two from 16 to 65536, bytes below 2^32)", who, n, c->pool.seq_bytes);
+        return LG_ERR_ARG;
+    }
+    if (c->n_pages <= 0 || c->max_pages <= 0 || c->max_pages > (1 << 30) / n) {
+        lg_set_error("%s: %d pages of %d rows, up to %d a sequence", who, c->n_pages, n, c->max_pages);
+        return LG_ERR_ARG;
+    }
+    if (!c->table || ((uintptr_t)c->table & 3) || c->table_stride < c->max_pages || c->table_stride > INT32_MAX) {
+        lg_set_error("%s: table rows %lld apart, %d entries needed", who, (long long)c->table_stride, c->max_pages);
+        return LG_ERR_ARG;
+    }
+    *shift = __builtin_ctz(n);
+    return LG_OK;
+}
+
 extern "C" int lg_rope_table(int scaling, int rope_dim, double base, double factor, int orig_ctx, double p0, double p1,
                              float* freq, float* mscale)
 {
@@ -99,6 +120,10 @@ struct RopeArgs {
     int n_heads, n_kv, hd, rope, ntok;
     float mscale, eps;
     LgKv c;   /* c.type 0: no cache */
+    int n_ctx;           /* positions below it have a place in the cache */
+    const int* table;    /* of pages (NULL: a sequence of c for each of the call's), */
+    int64_t tstride;
+    int n_pages, shift;  /* which have 2^shift rows */
 };
 
 /* cos, sin of pos * freq, times mscale, rounded once.  Far positions need the angle in
@@ -139,7 +164,10 @@ __global__ __launch_bounds__(256) void k_rope_tokens(RopeArgs a, int nblk, int p
     const int pos = a.pos[row];
     const int np = a.rope / 2, hd = a.hd, seq = row / a.ntok;
     const int n_all = a.n_heads + a.n_kv * (a.c.type ? 2 : 1);
-    const bool on = pos >= 0 && (!a.c.type || pos < a.c.n_ctx);   /* (workgroup-uniform) */
+    const bool on = pos >= 0 && (!a.c.type || pos < a.n_ctx);   /* (workgroup-uniform) */
+    size_t at_seq = (size_t)seq * a.c.seq;   /* the token's place: sequence or page, row of it */
+    int at_row = pos;
+    bool put = a.c.type && on;
 
     struct Head {
         int kind, g;   /* 0 query, 1 key, 2 value, 3 none */
@@ -197,6 +225,12 @@ __global__ __launch_bounds__(256) void k_rope_tokens(RopeArgs a, int nblk, int p
             }
         }
         if (i == 0) {   /* (the first loads are on their way) */
+            if (put && a.table) {
+                const int id = a.table[seq * a.tstride + (pos >> a.shift)];
+                put = (uint32_t)id < (uint32_t)a.n_pages;
+                at_seq = (size_t)(uint32_t)id * a.c.seq;
+                at_row = pos & ((1 << a.shift) - 1);
+            }
             if (on && (int)threadIdx.x < np) s_cs[threadIdx.x] = lg_turn(pos, a.freq[threadIdx.x], a.mscale);
             __syncthreads();
         }
@@ -234,10 +268,10 @@ __global__ __launch_bounds__(256) void k_rope_tokens(RopeArgs a, int nblk, int p
             }
             if (kind < 2 && y && in(j)) st(y + (size_t)g * hd, j, value, e);
         }
-        if (!a.c.type || !on) continue;
+        if (!put) continue;   /* (workgroup-uniform) */
         if (a.c.type == LG_F16) {
             if (kind == 1 || kind == 2) {
-                uint16_t* const r = (uint16_t*)((value ? a.c.v : a.c.k) + (size_t)seq * a.c.seq + lg_kv16_at(a.c, g, pos));
+                uint16_t* const r = (uint16_t*)((value ? a.c.v : a.c.k) + at_seq + lg_kv16_at(a.c, g, at_row));
 #pragma unroll
                 for (int j = 0; j < J; j++)
                     if (in(j)) {
@@ -275,10 +309,10 @@ __global__ __launch_bounds__(256) void k_rope_tokens(RopeArgs a, int nblk, int p
             uint32_t dm;
             const uint32_t code = lg_kv4_encode(v, &dm);
             if (k < HPW && (z.kind == 1 || z.kind == 2)) {
-                uint8_t* const c = (z.kind == 2 ? a.c.v : a.c.k) + (size_t)seq * a.c.seq;
+                uint8_t* const c = (z.kind == 2 ? a.c.v : a.c.k) + at_seq;
                 const int wd = lane % hw;
-                ((uint32_t*)(c + lg_kv4_codes(a.c, z.g, pos)))[wd] = code;
-                if (wd % 4 == 0) ((uint32_t*)(c + lg_kv4_dm(a.c, z.g, pos)))[wd / 4] = dm;
+                ((uint32_t*)(c + lg_kv4_codes(a.c, z.g, at_row)))[wd] = code;
+                if (wd % 4 == 0) ((uint32_t*)(c + lg_kv4_dm(a.c, z.g, at_row)))[wd / 4] = dm;
             }
             __builtin_amdgcn_wave_barrier();   /* the row's reads before the next round's writes */
         }
@@ -311,14 +345,13 @@ static bool rows_bad(const void* p, int64_t stride, int64_t least)
     return !p || !lg_al16(p) || stride % 4 || stride < least;
 }
 
-extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q_out, int64_t q_out_stride,
-                                      const float* k, int64_t k_stride, float* k_out, int64_t k_out_stride,
-                                      const float* v, int64_t v_stride, const float* qw, const float* kw, int n_heads,
-                                      int n_kv_heads, int head_dim, int rope_dim, int layout, const float* freq,
-                                      float mscale, float eps, const int* pos, int nseq, int ntok,
-                                      const lg_kv_cache* cache, void* stream)
+/* cache: the call's sequences, or pages' pool; NULL: none */
+static int rope_call(const char* who, const float* q, int64_t q_stride, float* q_out, int64_t q_out_stride, const float* k,
+                     int64_t k_stride, float* k_out, int64_t k_out_stride, const float* v, int64_t v_stride, const float* qw,
+                     const float* kw, int n_heads, int n_kv_heads, int head_dim, int rope_dim, int layout,
+                     const float* freq, float mscale, float eps, const int* pos, int nseq, int ntok,
+                     const lg_kv_cache* cache, const lg_kv_pages* pages, void* stream)
 {
-    const char* who = "lg_qk_norm_rope_tokens";
     if (nseq < 0 || ntok < 0 || n_heads < 0 || n_kv_heads <= 0 || n_heads > 65536 || n_kv_heads > 65536) {
         lg_set_error("%s: bad sizes (%d sequences of %d tokens, %d / %d heads)", who, nseq, ntok, n_heads, n_kv_heads);
         return LG_ERR_ARG;
@@ -341,10 +374,17 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
         return LG_ERR_ARG;
     }
     RopeArgs a = {q, k, v, qw, kw, freq, q_out, k_out, pos, q_stride, q_out_stride, k_stride, k_out_stride, v_stride,
-                  n_heads, n_kv_heads, head_dim, rope_dim, ntok, mscale, eps, {}};
+                  n_heads, n_kv_heads, head_dim, rope_dim, ntok, mscale, eps, {}, 0, nullptr, 0, 0, 0};
     if (cache) {
-        const int rc = lg_kv_arg(cache, nseq, who, &a.c);
+        const int rc = pages ? lg_kv_pages_arg(pages, who, &a.c, &a.shift) : lg_kv_arg(cache, nseq, who, &a.c);
         if (rc) return rc;
+        a.n_ctx = a.c.n_ctx;
+        if (pages) {
+            a.n_ctx = pages->max_pages * a.c.n_ctx;
+            a.table = pages->table;
+            a.tstride = pages->table_stride;
+            a.n_pages = pages->n_pages;
+        }
         if (cache->n_kv_heads != n_kv_heads || cache->head_dim != head_dim) {
             lg_set_error("%s: the cache has %d heads of %d, the keys %d of %d", who, cache->n_kv_heads,
                          cache->head_dim, n_kv_heads, head_dim);
@@ -359,6 +399,33 @@ extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q
     if (layout == LG_ROPE_HALF) rope_shape<true>(a, rows, waves, (hipStream_t)stream);
     else rope_shape<false>(a, rows, waves, (hipStream_t)stream);
     return lg_check_launch(who);
+}
+
+extern "C" int lg_qk_norm_rope_tokens(const float* q, int64_t q_stride, float* q_out, int64_t q_out_stride,
+                                      const float* k, int64_t k_stride, float* k_out, int64_t k_out_stride,
+                                      const float* v, int64_t v_stride, const float* qw, const float* kw, int n_heads,
+                                      int n_kv_heads, int head_dim, int rope_dim, int layout, const float* freq,
+                                      float mscale, float eps, const int* pos, int nseq, int ntok,
+                                      const lg_kv_cache* cache, void* stream)
+{
+    return rope_call("lg_qk_norm_rope_tokens", q, q_stride, q_out, q_out_stride, k, k_stride, k_out, k_out_stride, v, v_stride,
+                     qw, kw, n_heads, n_kv_heads, head_dim, rope_dim, layout, freq, mscale, eps, pos, nseq, ntok, cache,
+                     nullptr, stream);
+}
+
+extern "C" int lg_qk_norm_rope_paged(const float* q, int64_t q_stride, float* q_out, int64_t q_out_stride, const float* k,
+                                     int64_t k_stride, float* k_out, int64_t k_out_stride, const float* v,
+                                     int64_t v_stride, const float* qw, const float* kw, int n_heads, int n_kv_heads,
+                                     int head_dim, int rope_dim, int layout, const float* freq, float mscale, float eps,
+                                     const int* pos, int nseq, int ntok, const lg_kv_pages* cache, void* stream)
+{
+    const char* who = "lg_qk_norm_rope_paged";
+    if (!cache) {
+        lg_set_error("%s: no cache", who);
+        return LG_ERR_ARG;
+    }
+    return rope_call(who, q, q_stride, q_out, q_out_stride, k, k_stride, k_out, k_out_stride, v, v_stride, qw, kw, n_heads,
+                     n_kv_heads, head_dim, rope_dim, layout, freq, mscale, eps, pos, nseq, ntok, &cache->pool, cache, stream);
 }
 
 /* One thread per word of eight codes; keys, then values.  Fewer than 2^32 words of

@@ -72,6 +72,10 @@ class LgKvCache(C.Structure):
                 ("head_dim", C.c_int32), ("seq_bytes", C.c_size_t)]
 
 
+class LgKvPages(C.Structure):
+    _fields_ = [("pool", LgKvCache), ("n_pages", C.c_int32), ("max_pages", C.c_int32), ("table", _vp), ("table_stride", C.c_int64)]
+
+
 # Every exported symbol of include/ligguf_hip.h with its ctypes signature.
 SIGNATURES = {
     "lg_row_size": (C.c_int64, [C.c_int, C.c_int64]),
@@ -129,6 +133,17 @@ SIGNATURES = {
     "lg_attn_cache": (C.c_int, [_vp, C.c_int64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
                                 C.c_int64, _vp, C.c_size_t, _vp]),
     "lg_logprobs": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp]),
+    "lg_qk_norm_rope_paged": (C.c_int, [_vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64,
+                                        _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_float,
+                                        C.c_float, _vp, C.c_int, C.c_int, _vp, _vp]),
+    "lg_attn_paged_workspace_size": (C.c_size_t, [_vp] + [C.c_int] * 8),
+    "lg_attn_paged": (C.c_int, [_vp, C.c_int64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int,
+                                C.c_int, _vp, C.c_int64, _vp, C.c_size_t, _vp]),
+    "lg_beam_select_workspace_size": (C.c_size_t, [C.c_int] * 4),
+    "lg_beam_select": (C.c_int, [_vp, C.c_int64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp,
+                                 C.c_size_t, _vp]),
+    "lg_beam_reorder": (C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int64, C.c_int, _vp, _vp, C.c_int, C.c_int, _vp, C.c_size_t,
+                                  _vp]),
     "lg_bert_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "lg_bert_destroy": (C.c_int, [_vp]),
     "lg_bert_last_error": (C.c_char_p, [_vp]),

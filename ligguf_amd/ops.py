@@ -204,6 +204,45 @@ class KvCache:
         return cls(*(torch.zeros(shape, dtype=dt, device=device) for _ in range(2)), n_kv_heads, head_dim, type, n_ctx)
 
 
+class PagedKvCache:
+    """One layer's keys and values of many sequences in pages of `page` rows
+    (lg_kv_pages): F16 pools [n_pages, page, n_kv_heads * head_dim] or KV4 bytes
+    [n_pages, lg_kv_bytes of a page or more, a multiple of 16], and an int32
+    table [nseq, max_pages] of page numbers (-1: no page), whose rows may be
+    part of longer ones.  `pool` is the pages as a KvCache, a page per sequence."""
+
+    def __init__(self, k, v, table, n_kv_heads: int, head_dim: int, type: int = F16, page: int = None):
+        self.pool = p = KvCache(k, v, n_kv_heads, head_dim, type, page)
+        if (table.dtype is not _INT32 or table.get_device() != p.index or table.dim() != 2 or not table.numel()
+                or (table.shape[1] > 1 and table.stride(1) != 1)):
+            _refuse(f"table: int32 [nseq, max_pages] with dense rows on GPU {p.index} wanted")
+        self.k, self.v, self.table, self.type, self.page, self.n_pages = k, v, table, type, p.n_ctx, p.nseq
+        self.nseq, self.max_pages = table.shape
+        self.n_kv_heads, self.head_dim, self.index, self.n_ctx = n_kv_heads, head_dim, p.index, self.max_pages * p.n_ctx
+        stride = table.stride(0) if self.nseq > 1 else self.max_pages
+        self.desc = L.LgKvPages(p.desc, p.nseq, self.max_pages, table.data_ptr(), stride)
+
+    @classmethod
+    def empty(cls, type: int, n_pages: int, page: int, n_kv_heads: int, head_dim: int, table) -> "PagedKvCache":
+        """Pages of zeros on the table's device."""
+        c = KvCache.empty(type, page, n_kv_heads, head_dim, n_pages, table.device)
+        return cls(c.k, c.v, table, n_kv_heads, head_dim, type, page)
+
+
+class PagedLayers:
+    """The caches of a model's layers that have one table: what beam_reorder moves."""
+
+    def __init__(self, caches):
+        c = caches[0] if caches else _refuse("no layers")
+        for x in caches:
+            if (x.table.data_ptr() != c.table.data_ptr() or x.table.shape != c.table.shape or x.table.stride() != c.table.stride()
+                    or (x.type, x.page, x.n_pages, x.n_kv_heads, x.head_dim) != (c.type, c.page, c.n_pages, c.n_kv_heads, c.head_dim)):
+                _refuse("layers of one table and pages of one form wanted")
+        self.caches, self.table, self.index, self.nseq = list(caches), c.table, c.index, c.nseq
+        self.desc = (L.LgKvCache * len(caches))(*(x.pool.desc for x in caches))
+        self.args = (self.desc, len(caches), c.n_pages, c.table.data_ptr(), c.desc.table_stride, c.max_pages)
+
+
 def rope_table(rope_dim: int, base: float, scaling: int = L.ROPE_PLAIN, factor: float = 1.0, orig_ctx: int = 0, p0: float = 0.0,
                p1: float = 0.0):
     """lg_rope_table: (rope_dim / 2 frequencies as a CPU tensor, mscale)."""
@@ -214,11 +253,11 @@ def rope_table(rope_dim: int, base: float, scaling: int = L.ROPE_PLAIN, factor: 
 
 
 def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None, half: bool = False, qw=None, kw=None,
-                        eps: float = 1e-6, mscale: float = 1.0, cache: KvCache = None, want_k: bool = False, q_out=None,
-                        k_out=None):
+                        eps: float = 1e-6, mscale: float = 1.0, cache=None, want_k: bool = False, q_out=None, k_out=None):
     """lg_qk_norm_rope_tokens on q, k, v [nseq, ntok, heads * head_dim] (views of
     a fused q | k | v row are fine; q or, without a cache, v may be None) and pos
-    [nseq, ntok]: the rotated queries and keys; keys only with want_k or k_out."""
+    [nseq, ntok]: the rotated queries and keys; keys only with want_k or k_out.
+    cache: a KvCache, or a PagedKvCache (lg_qk_norm_rope_paged)."""
     rope_dim = head_dim if rope_dim is None else rope_dim
     p, i = _pos(pos), pos.get_device()
     nseq, ntok = pos.shape
@@ -245,7 +284,9 @@ def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None,
         if cache.index != i or cache.nseq != nseq or v is None:
             _refuse(f"cache: values and {nseq} sequences on GPU {i} wanted")
         rv, desc = _rows(v, *at, kd, "v"), C.byref(cache.desc)
-    _on(i, load().lg_qk_norm_rope_tokens, *rq, *rqo, *rk, *rko, *rv, _vec(qw, head_dim, i, "qw"), _vec(kw, head_dim, i, "kw"),
+    lib = load()
+    fn = lib.lg_qk_norm_rope_paged if cache.__class__ is PagedKvCache else lib.lg_qk_norm_rope_tokens
+    _on(i, fn, *rq, *rqo, *rk, *rko, *rv, _vec(qw, head_dim, i, "qw"), _vec(kw, head_dim, i, "kw"),
         qd // head_dim, kd // head_dim, head_dim, rope_dim, 1 if half else 0, _vec(freq, rope_dim // 2, i, "freq"), mscale, eps, p,
         nseq, ntok, desc)
     return q_out, k_out
@@ -297,6 +338,86 @@ def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max
     return out
 
 
+def attention_paged(q, cache: PagedKvCache, pos, window: int = 0, sinks: int = 0, max_pos: int = None, prefix=None,
+                    max_prefix: int = None, out=None, workspace=None):
+    """lg_attn_paged: attention_cache over pages.  prefix, int32 [groups] on the GPU
+    (nseq is a multiple of groups): the sequences of a group share so many first
+    rows, which lie in the pages of its first one and are read once for all;
+    max_prefix, a bound of them (max_pos + 1 by default), sizes the launch."""
+    p, i = _pos(pos), pos.get_device()
+    nseq, ntok = pos.shape
+    if cache.index != i or cache.nseq != nseq:
+        _refuse(f"cache: {nseq} sequences on GPU {i} wanted")
+    max_pos = cache.n_ctx - 1 if max_pos is None else max_pos
+    group, pp = 1, None
+    if prefix is None:
+        max_prefix = 0
+    else:
+        groups = prefix.numel()
+        if prefix.dtype is not _INT32 or prefix.get_device() != i or not prefix.is_contiguous() or not groups or nseq % groups:
+            _refuse(f"prefix: contiguous int32 on GPU {i} wanted, one for each group of {nseq} sequences")
+        group, pp = nseq // groups or 1, prefix.data_ptr()
+        max_prefix = max_pos + 1 if max_prefix is None else max_prefix
+    width, hd = q.shape[-1], cache.head_dim
+    heads = width // hd
+    if heads * hd != width:
+        _refuse(f"rows of {width} values are no heads of {hd}")
+    rows = _rows(q, i, nseq, ntok, width, "q")
+    out, ro = _fresh(q, nseq * ntok, width) if out is None else (out, _rows(out, i, nseq, ntok, width, "out"))
+    lib, desc = load(), C.byref(cache.desc)
+    need = lib.lg_attn_paged_workspace_size(desc, nseq, ntok, heads, window, sinks, max_pos, group, max_prefix)
+    workspace, ws = _work(need, workspace, q)
+    _on(i, lib.lg_attn_paged, *rows, desc, p, nseq, ntok, heads, window, sinks, max_pos, pp, group, max_prefix, *ro, *ws)
+    return out
+
+
+class BeamChoice(NamedTuple):
+    score: torch.Tensor          # fp32 [groups, top], the highest first
+    parent: torch.Tensor         # int32: the beam that each goes on from, -1: none
+    token: torch.Tensor          # int32
+
+
+def beam_select(logits, scores, top: int, done=None, end: int = -1, workspace=None) -> BeamChoice:
+    """lg_beam_select of logits [groups, beams, vocab] (dense rows, one run of
+    them) and scores [groups, beams]: the `top` best continuations of each group.
+    done, int32 [groups, beams]: beams that have ended (with the token `end`)."""
+    if logits.dtype is not _FP32 or not logits.is_cuda or logits.dim() != 3:
+        _refuse("logits: fp32 [groups, beams, vocab] on the GPU wanted")
+    i, (groups, beams, vocab) = logits.get_device(), logits.shape
+    s0, s1, s2 = logits.stride()
+    row = s1 if beams > 1 else s0 if groups > 1 else vocab
+    if (s2 != 1 and vocab > 1) or (groups > 1 and s0 != row * beams):
+        _refuse(f"logits: rows of strides {logits.stride()} are not one run")
+    for t, dt, name in ((scores, _FP32, "scores"), (done, _INT32, "done")):
+        if t is None and name == "done":
+            continue
+        if t.dtype is not dt or t.get_device() != i or t.shape != (groups, beams) or not t.is_contiguous():
+            _refuse(f"{name}: contiguous {dt} [{groups}, {beams}] on {logits.device} wanted")
+    if top < 1:
+        _refuse(f"top {top}")
+    lib, new = load(), logits.new_empty
+    score = new((groups, top))
+    both = torch.empty((2, groups, top), dtype=_INT32, device=logits.device)
+    parent, token = both.unbind()
+    workspace, ws = _work(lib.lg_beam_select_workspace_size(groups, beams, vocab, top), workspace, logits)
+    _on(i, lib.lg_beam_select, logits.data_ptr(), row, scores.data_ptr(), None if done is None else done.data_ptr(), end, groups, beams,
+        vocab, top, score.data_ptr(), parent.data_ptr(), token.data_ptr(), *ws)
+    return BeamChoice(score, parent, token)
+
+
+def beam_reorder(layers: PagedLayers, parent, length, workspace=None) -> None:
+    """lg_beam_reorder, in place: the sequences go on from `parent` (int32 [groups,
+    beams], beams of their group) with length rows each (int32 [groups])."""
+    i = layers.index
+    for t, name in ((parent, "parent"), (length, "length")):
+        if t.dtype is not _INT32 or t.get_device() != i or not t.is_contiguous():
+            _refuse(f"{name}: contiguous int32 on GPU {i} wanted")
+    if parent.dim() != 2 or length.shape != parent.shape[:1] or parent.numel() != layers.nseq:
+        _refuse(f"parent {tuple(parent.shape)}, length {tuple(length.shape)}: {layers.nseq} sequences in groups wanted")
+    workspace, ws = _work(16 * layers.nseq, workspace, parent)
+    _on(i, load().lg_beam_reorder, *layers.args, parent.data_ptr(), length.data_ptr(), *parent.shape, *ws)
+
+
 class Logprobs(NamedTuple):
     logprob: torch.Tensor        # [rows], None without tokens
     entropy: torch.Tensor        # [rows]
@@ -327,4 +448,4 @@ def logprobs(logits, toks=None, top: int = 0) -> Logprobs:
 
 __all__ = ["dequantize_row", "quantize_q8_0", "quantize_q8_K", "matvec", "rmsnorm_quant", "qk_norm_rope_kv",
            "attention", "swiglu_quant", "KvCache", "rope_table", "qk_norm_rope_tokens", "kv_values",
-           "attention_cache", "Logprobs", "logprobs", "Q8_0", "Q8_K", "F32", "F16", "KV4"]
+           "attention_cache", "PagedKvCache", "PagedLayers", "attention_paged", "BeamChoice", "beam_select", "beam_reorder", "Logprobs", "logprobs", "Q8_0", "Q8_K", "F32", "F16", "KV4"]
