@@ -553,9 +553,8 @@ int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages* cache, co
 /* The best continuations of each of ngroups groups of `beams` rows of logits
  * (rows as lg_logprobs takes them): candidate (b, t) has the score
  *   scores[b] + log softmax(row b)[t]
- * and the `top` highest, ties by the lower beam, then by the higher logit and the lower
- * token, go to score, parent (the beam, 0 .. beams - 1) and token, [ngroups][top]
- * each.  With done (may be NULL), a beam whose done is not 0 has the one
+ * and the `top` highest, ties by the lower beam and then the lower token, go to
+ * score, parent (the beam, 0 .. beams - 1) and token, [ngroups][top] each.  With done (may be NULL), a beam whose done is not 0 has the one
  * candidate (b, end) of score scores[b]; its logits are not read.  No
  * candidates: scores and sums that are no finite numbers (an idle beam has
  * -infinity), logits of -infinity.  Where there are fewer than top, the rest is

@@ -22,10 +22,9 @@ __device__ __forceinline__ bool bm_live(const BeamArgs& a, int64_t row)
     return fabsf(a.scores[row]) <= FLT_MAX && !(a.done && a.done[row]);
 }
 
-constexpr float BM_LOG2E = 1.44269504088896341f;
-
 /* A part of a row: its maximum, the sum of e^(x - m) and its `top` highest
- * entries in order. */
+ * entries in order.  16 values of a thread at a time, the next ones on their way
+ * (as k_logp). */
 template <int T>
 __global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
 {
@@ -37,16 +36,57 @@ __global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
     const LpRow r(a.logits + row * a.stride + first, n);
     const int nq = r.quads();
     float m = -FLT_MAX, z = 0.0f, mine = -INFINITY;
-    for (int q = t; q < nq; q += T) {
-        const float4 v = r.load(q);
-        mine = fmaxf(fmaxf(mine, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+    auto take = [&](const float4 (&v)[4]) __attribute__((always_inline)) {
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[4 * j] = v[j].x;
+            x[4 * j + 1] = v[j].y;
+            x[4 * j + 2] = v[j].z;
+            x[4 * j + 3] = v[j].w;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) mine = fmaxf(mine, x[i]);
         const float mn = fmaxf(m, mine);
-        z *= __builtin_amdgcn_exp2f((m - mn) * BM_LOG2E);
+        z *= __builtin_amdgcn_exp2f((m - mn) * LP_LOG2E);
         m = mn;
-        z += (__builtin_amdgcn_exp2f((v.x - m) * BM_LOG2E) + __builtin_amdgcn_exp2f((v.y - m) * BM_LOG2E)) +
-             (__builtin_amdgcn_exp2f((v.z - m) * BM_LOG2E) + __builtin_amdgcn_exp2f((v.w - m) * BM_LOG2E));
+        float zs[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; i++) zs[i % 4] += __builtin_amdgcn_exp2f((x[i] - m) * LP_LOG2E);
+        z += (zs[0] + zs[1]) + (zs[2] + zs[3]);
+    };
+    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const int off = r.sh ? 1 : 0, full = (n + r.sh) / 4;
+    int q = off;
+    float4 v[4];
+    if (q + 4 * T <= full) {
+        const float4* const p = (const float4*)(r.x - r.sh) + t;
+        float4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = p[q + j * T];
+        for (; q + 4 * T <= full; q += 4 * T) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = w[j];
+            if (q + 8 * T <= full)
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = p[q + (4 + j) * T];
+            take(v);
+        }
+    }
+    for (; q < nq; q += 4 * T) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int at = q + t + j * T;
+            v[j] = at < nq ? r.load(at) : none;
+        }
+        take(v);
     }
     const uint32_t ord = lp_ord(mine);
+    if (off) {   /* the cut quad of a row that is not aligned, which no thread counts among its own */
+        v[0] = t == 0 ? r.load(0) : none;
+        v[1] = v[2] = v[3] = none;
+        take(v);
+    }
     {   /* of T / 256 neighbours */
         uint32_t o = ord;
         if constexpr (T >= 512) o = max(o, (uint32_t)lg_partner<0>((int)o));
@@ -55,97 +95,162 @@ __global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
     }
     auto join = [&]() {   /* m, z over the wave */
         const float M = lg_group_max<64>(m);
-        z = lg_group_sum<64>(z * __builtin_amdgcn_exp2f(fmaxf(m - M, -1e30f) * BM_LOG2E));
+        z = lg_group_sum<64>(z * __builtin_amdgcn_exp2f(fmaxf(m - M, -1e30f) * LP_LOG2E));
         m = M;
     };
     join();
     if (t % 64 == 0) s.sums[t / 64] = make_float4(m, z, 0.0f, 0.0f);
     __syncthreads();
     {
-        const float4 v = t % 64 < T / 64 ? s.sums[t % 64] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
-        m = v.x;
-        z = v.y;
+        const float4 y = t % 64 < T / 64 ? s.sums[t % 64] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
+        m = y.x;
+        z = y.y;
         join();
     }
     const int64_t at = row * a.parts + part;
     if (t == 0) a.mz[at] = make_float2(m, z);
     const int top = min(a.top, n);
-    const int c = lp_top<T>(s, r, nq, 0, top, ord, z != z);
+    const int c = lp_top<T>(s, r, nq, off, top, ord, z != z);
     lp_emit<T>(s, c, top, [&](int rank, uint64_t k) { a.keys[at * a.top + rank] = k - (uint32_t)first; });   /* (~id - first = ~(id + first)) */
 }
 
+constexpr int BM_HELD = 4096;    /* entries of a group's parts that its workgroup holds as doubles */
+constexpr int BM_LISTS = 1024;   /* and parts */
+constexpr int BM_VALS = 256;     /* candidates whose values lie side by side */
+
 /* A group: log sums of its beams' parts, then every part's entries as scores in
- * double.  The entries of a part are in order, so those ahead of one are counted
- * list by list, by halving. */
-__global__ __launch_bounds__(256) void k_beam_group(BeamArgs a)
+ * double.  The first few entries of each part, `top` together at least, have a
+ * top-th highest of their own, and only entries that are no lower than it are
+ * compared with each other: places by counting, first a hundred or so, then
+ * hardly more than `top`.  Bound by its chain: loads, an exponential and a
+ * logarithm in double, six barriers. */
+template <int T>
+__global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
 {
     extern __shared__ double s_score[];   /* [beams][parts][top] */
-    __shared__ double s_off[LG_BEAMS_MAX];
+    __shared__ double s_off[LG_BEAMS_MAX], s_lse[LG_BEAMS_MAX], s_val[BM_VALS], s_least;
+    __shared__ uint32_t s_id[BM_HELD];    /* the complements of the entries' tokens */
+    union Lists {
+        float2 mz[BM_LISTS];
+        double z[BM_LISTS];
+        uint16_t list[BM_HELD];
+    };
+    __shared__ Lists s;
     __shared__ int s_kind[LG_BEAMS_MAX], s_n;   /* 0: no candidates, 1: logits, 2: finished */
-    const int64_t row0 = (int64_t)blockIdx.x * a.beams;
-    const int t = threadIdx.x, lists = a.beams * a.parts;
+    const int64_t row0 = (int64_t)blockIdx.x * a.beams, key0 = row0 * a.parts * a.top;
+    const int t = threadIdx.x, lists = a.beams * a.parts, n = lists * a.top, run = a.parts * a.top;
     if (t < a.beams) {
         const float sc = a.scores[row0 + t];
-        int kind = 0;
-        double off = 0.0;
-        if (fabsf(sc) <= FLT_MAX) {
-            if (a.done && a.done[row0 + t]) kind = 2;
-            else {
-                const float2* const mz = a.mz + (row0 + t) * a.parts;
-                float M = -FLT_MAX;
-                for (int p = 0; p < a.parts; p++) M = fmaxf(M, mz[p].x);
-                double z = 0.0;
-                for (int p = 0; p < a.parts; p++) z += mz[p].y * exp((double)mz[p].x - (double)M);
-                off = (double)M + log(z);
-                kind = fabs(off) <= (double)FLT_MAX ? 1 : 0;   /* (no NaN, no infinity) */
-            }
-        }
-        s_kind[t] = kind;
-        s_off[t] = kind == 2 ? -(double)sc : off;
+        s_kind[t] = !(fabsf(sc) <= FLT_MAX) ? 0 : a.done && a.done[row0 + t] ? 2 : 1;
+        s_off[t] = (double)sc;
     }
-    if (t == 0) s_n = 0;
+    /* (what beams without logits left there is not used) */
+    for (int l = t; l < lists; l += T) s.mz[l] = a.mz[row0 * a.parts + l];
+    for (int i = t; i < n; i += T) {
+        const uint64_t k = a.keys[key0 + i];
+        s_score[i] = (double)lp_value(k);
+        s_id[i] = (uint32_t)k;
+    }
+    if (t == 0) {
+        s_n = 0;
+        s_least = -INFINITY;
+    }
     __syncthreads();
-    const int64_t key0 = row0 * a.parts * a.top;
-    auto held = [&](int l) { return min(a.top, min(a.part, a.vocab - l % a.parts * a.part)); };   /* entries of list l */
-    for (int i = t; i < lists * a.top; i += 256) {
-        const int l = i / a.top, b = l / a.parts;
+    /* the parts' sums over their beam's maximum, an exponential a thread */
+    auto top_of = [&](int b) {
+        float M = -FLT_MAX;
+        for (int p = 0; p < a.parts; p++) M = fmaxf(M, s.mz[b * a.parts + p].x);
+        return M;
+    };
+    double z[BM_LISTS / T];
+#pragma unroll
+    for (int k = 0; k < BM_LISTS / T; k++) {
+        const int l = t + k * T;
+        z[k] = l < lists ? s.mz[l].y * (a.parts > 1 ? exp((double)s.mz[l].x - (double)top_of(l / a.parts)) : 1.0) : 0.0;
+    }
+    const float M = t < a.beams ? top_of(t) : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < BM_LISTS / T; k++)
+        if (t + k * T < lists) s.z[t + k * T] = z[k];
+    __syncthreads();
+    if (t < a.beams) {
+        double sum = 0.0;
+        for (int p = 0; p < a.parts; p++) sum += s.z[t * a.parts + p];
+        const double lse = (double)M + log(sum);
+        s_lse[t] = lse;
+        if (s_kind[t] == 1 && !(fabs(lse) <= (double)FLT_MAX)) s_kind[t] = 0;   /* (NaN, infinities) */
+    }
+    __syncthreads();
+    for (int i = t; i < n; i += T) {
+        const int b = i / run, in = i - b * run, part = in / a.top, at = in - part * a.top;
+        const int held = min(a.top, min(a.part, a.vocab - part * a.part));
         double v = -INFINITY;
-        if (s_kind[b] == 1 && i % a.top < held(l))
-            v = (double)a.scores[row0 + b] + ((double)lp_value(a.keys[key0 + i]) - s_off[b]);
-        if (s_kind[b] == 2 && i % (a.top * a.parts) == 0) v = -s_off[b];
+        if (s_kind[b] == 1 && at < held) v = s_off[b] + (s_score[i] - s_lse[b]);
+        if (s_kind[b] == 2 && in == 0) {
+            v = s_off[b];
+            s_id[i] = ~(uint32_t)a.end;
+        }
         s_score[i] = v;
     }
-    __syncthreads();
-    for (int i = t; i < lists * a.top; i += 256) {
-        const double v = s_score[i];
-        if (!(v > -INFINITY)) continue;
-        const int l = i / a.top, b = l / a.parts;
-        int rank = i % a.top;
-        for (int o = 0; o < lists && rank < a.top; o++) {
-            if (o == l) continue;
-            /* entries of list o ahead of this one: the higher ones, and equal ones of a lower beam or, of the
-             * same beam, of a higher logit or a lower token */
-            int lo = 0, hi = a.top;
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                const double w = s_score[o * a.top + mid];
-                bool ahead = w > v;
-                if (w == v) ahead = o / a.parts != b ? o < l : a.keys[key0 + o * a.top + mid] > a.keys[key0 + i];
-                if (ahead) lo = mid + 1;
-                else hi = mid;
+    /* place of entry i, value v, among the c entries of s.list: those that are higher, or equal and ahead in the order of
+     * beams, parts and entries.  Eight values at a time, no branches (16 entries of 8 beams: 12 us with them), whatever
+     * lies behind the c-th being -infinity; equal values are rare and looked at again. */
+    auto place = [&](int c, int i, double v) __attribute__((always_inline)) {
+        int rank = 0, same = 0;
+        const int fast = min(c, BM_VALS);
+        for (int o = 0; o < fast; o += 8)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const double w = s_val[o + e];
+                rank += w > v ? 1 : 0;
+                same += w == v ? 1 : 0;
             }
-            rank += lo;
+        for (int o = fast; o < c; o++) {
+            const double w = s_score[s.list[o]];
+            rank += w > v ? 1 : 0;
+            same += w == v ? 1 : 0;
         }
+        if (same > 1)
+            for (int o = 0; o < c; o++) rank += s.list[o] < i && s_score[s.list[o]] == v ? 1 : 0;
+        return rank;
+    };
+    auto gather = [&](int c) {
+        for (int k = t; k < BM_VALS; k += T) s_val[k] = k < c ? s_score[s.list[k]] : -INFINITY;
+    };
+    const int each = (a.top + lists - 1) / lists, heads = each * lists;   /* (fewer than top + lists) */
+    __syncthreads();
+    for (int k = t; k < heads; k += T) s.list[k] = (uint16_t)(k / each * a.top + k % each);
+    __syncthreads();
+    gather(heads);
+    __syncthreads();
+    for (int k = t; k < heads; k += T) {
+        const int i = s.list[k];
+        const double v = s_score[i];
+        if (v > -INFINITY && place(heads, i, v) == a.top - 1) s_least = v;
+    }
+    __syncthreads();
+    const double least = s_least;   /* (-infinity: fewer than `top` of them are any) */
+    for (int i = t; i < n; i += T) {
+        const double v = s_score[i];
+        if (v > -INFINITY && v >= least) s.list[atomicAdd(&s_n, 1)] = (uint16_t)i;   /* (in whatever order: ranked below) */
+    }
+    __syncthreads();
+    const int cand = s_n;
+    gather(cand);
+    __syncthreads();
+    for (int k = t; k < cand; k += T) {
+        const int i = s.list[k];
+        const double v = s_score[i];
+        const int rank = place(cand, i, v);
         if (rank < a.top) {
             const int64_t at = (int64_t)blockIdx.x * a.top + rank;
             a.score[at] = (float)v;
-            a.parent[at] = b;
-            a.token[at] = s_kind[b] == 2 ? a.end : (int)~(uint32_t)a.keys[key0 + i];
-            atomicAdd(&s_n, 1);
+            a.parent[at] = i / run;
+            a.token[at] = (int)~s_id[i];
         }
     }
-    __syncthreads();
-    if (t >= s_n && t < a.top) {
+    if (t >= cand && t < a.top) {
         const int64_t at = (int64_t)blockIdx.x * a.top + t;
         a.score[at] = -INFINITY;
         a.parent[at] = -1;
@@ -159,7 +264,8 @@ __global__ __launch_bounds__(256) void k_beam_group(BeamArgs a)
 static int bm_parts(int64_t rows, int beams, int vocab, int top)
 {
     const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(rows, 1));
-    return (int)std::max<int64_t>(1, std::min({want, (int64_t)vocab / 4096, (int64_t)4096 / ((int64_t)beams * top)}));
+    return (int)std::max<int64_t>(1, std::min({want, (int64_t)vocab / 4096, (int64_t)BM_HELD / ((int64_t)beams * top),
+                                                  (int64_t)BM_LISTS / beams}));
 }
 
 static bool bm_sizes(int ngroups, int beams, int vocab, int top)
@@ -210,7 +316,7 @@ extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* 
     hipStream_t s = (hipStream_t)stream;
     const int lists = beams * a.parts * top;
     k_beam_rows<1024><<<(unsigned)(rows * a.parts), 1024, 0, s>>>(a);
-    k_beam_group<<<ngroups, 256, lists * sizeof(double), s>>>(a);
+    k_beam_group<256><<<ngroups, 256, lists * sizeof(double), s>>>(a);
     return lg_check_launch(who);
 }
 
@@ -293,8 +399,21 @@ __global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a)
     uint8_t* const p = a.pool[blockIdx.y][blockIdx.z];
     const uint8_t* const src = p + (size_t)j.x * a.c.seq;
     uint8_t* const dst = p + (size_t)j.y * a.c.seq;
-    auto run = [&](size_t at, int bytes) {   /* multiples of 4: an fp16 row of an odd number of heads may be 4 bytes */
-        for (int i = threadIdx.x * 4; i < bytes; i += 1024) *(uint32_t*)(dst + at + i) = *(const uint32_t*)(src + at + i);
+    auto run = [&](size_t at, int bytes) {   /* multiples of 4 from 16-byte addresses on */
+        const int n = bytes / 16;
+        const uint4* const x = (const uint4*)(src + at);
+        uint4* const y = (uint4*)(dst + at);
+        int i = threadIdx.x;
+        for (; i + 3 * 256 < n; i += 4 * 256) {
+            const uint4 v0 = x[i], v1 = x[i + 256], v2 = x[i + 512], v3 = x[i + 768];
+            y[i] = v0;
+            y[i + 256] = v1;
+            y[i + 512] = v2;
+            y[i + 768] = v3;
+        }
+        for (; i < n; i += 256) y[i] = x[i];
+        i = 4 * n + threadIdx.x;
+        if (i < bytes / 4) ((uint32_t*)y)[i] = ((const uint32_t*)x)[i];
     };
     if (a.c.type == LG_F16) run(0, j.z * a.c.n_kv * a.c.hd * 2);
     else
