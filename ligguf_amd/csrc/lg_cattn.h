@@ -1,6 +1,6 @@
-/* lg_cattn.h -- the kernels of attention of many rows over the caches that callers
- * keep: contiguous ones (lg_cattn.hip) and pages (lg_pattn.hip), fp16 or 4
- * bits, causal, with a sliding window and first positions that stay visible. */
+/* lg_cattn.h -- attention of many rows over the caches that callers keep, causal,
+ * with a sliding window and first positions that stay visible: what contiguous
+ * caches (lg_cattn.hip) and pages (lg_pattn.hip) have in common, fp16 or 4 bits. */
 #pragma once
 
 #include <float.h>
@@ -40,12 +40,46 @@ struct CAttnPaged : CAttn {
         *lo = share ? 0 : n;
         *hi = share ? n : INT32_MAX;
     }
-    /* the page of row `key` (wave-uniform) of table row t, -1: none.  The
-     * table is read through the constant address space: scalar loads. */
-    __device__ __forceinline__ int page_at(const int* t, int key) const
+    __device__ __forceinline__ bool is_page(int id) const { return (uint32_t)id < (uint32_t)n_pages; }
+    /* the table's entry for row `key` of table row t (rows past max_pos, which
+     * nothing sees, take its) */
+    __device__ __forceinline__ int entry(const int* t, int key) const { return t[min(key, max_pos) >> shift]; }
+};
+
+/* What a column at position p sees of the keys [lo, hi): none, bit by bit, are the
+ * present tile's groups of 16 rows without a page.  Without branches: as a
+ * chain of conditions around the write of -infinity (clang 22, gfx950) the
+ * compiler dropped the write of the first score. */
+struct CaSeen {
+    int lo, hi, wlo, sinks;
+    __device__ __forceinline__ CaSeen(const CAttnPaged& a, int p, int klo, int khi)
+        : lo(klo), hi(min(p, khi - 1)), wlo(a.window > 0 ? p - a.window + 1 : INT32_MIN), sinks(a.sinks)
     {
-        const int id = ((const __attribute__((address_space(4))) int*)t)[key >> shift];
-        return (uint32_t)id < (uint32_t)n_pages ? id : -1;
+    }
+    __device__ __forceinline__ bool operator()(int key, int kb, int none) const
+    {
+        return (key >= lo) & (key <= hi) & ((key >= wlo) | (key < sinks)) & !(none >> ((key - kb) >> 4) & 1);
+    }
+};
+
+/* A tile's table entries, that of its rows 16 j .. in lane j (mod 8): loaded ahead
+ * like any other vector load, in the order of the keys and values, so that
+ * nothing waits for them alone. */
+struct CaEntries {
+    int e;
+    __device__ __forceinline__ void load(const CAttnPaged& a, const int* trow, int kb)
+    {
+        e = a.entry(trow, kb + 16 * (threadIdx.x & 7));
+    }
+    /* those of the tile's n groups of 16 rows that are no pages, bit by bit */
+    __device__ __forceinline__ int none(const CAttnPaged& a, int n) const
+    {
+        return (int)__builtin_amdgcn_ballot_w64(!a.is_page(e)) & ((1 << n) - 1);
+    }
+    /* where group j's (the wave's j) page lies in a pool, page 0 in place of none */
+    __device__ __forceinline__ size_t at(const CAttnPaged& a, int j) const
+    {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(a.is_page(e) ? e : 0, j) * (uint32_t)a.c.seq;
     }
 };
 
@@ -120,25 +154,33 @@ __device__ __forceinline__ float ca_scale(float scale2, int ex) { return fmaxf(l
  * seen yet), the maximum is taken off the scores first and cc is 14; a wave
  * with such a column raises at every tile.  cc belongs to m from the start: of
  * small queries -2^40 sc is near, and a first tile without a key of the column
- * would else raise from 14 by a factor that is infinite. */
-struct CaMax {
+ * would else raise from 14 by a factor that is infinite.  With LAG the maximum
+ * follows only scores that are 2^LAG times above it: weights are up to 2^(BASE +
+ * LAG), which fp16 has to hold, and the sums are rescaled but once or twice. */
+template <int BASE_, int LAG>
+struct CaMaxOf {
+    static constexpr float BASE = (float)BASE_;
     float sc, m, cc;
     bool any_far;                         /* of the wave */
 
-    __device__ __forceinline__ explicit CaMax(float scale) : sc(scale), m(-0x1p40f), any_far(true)   /* (-2^40: below any score) */
+    __device__ __forceinline__ explicit CaMaxOf(float scale) : sc(scale), m(-0x1p40f), any_far(true)   /* (-2^40: below any score) */
     {
-        const float c = __builtin_fmaf(-m, sc, 14.0f);
-        cc = far(c) ? 14.0f : c;
+        const float c = __builtin_fmaf(-m, sc, BASE);
+        cc = far(c) ? BASE : c;
     }
     __device__ __forceinline__ bool far(float c) const { return fabsf(c) > 0x1p22f; }
-    __device__ __forceinline__ bool due(float mn) const { return __builtin_amdgcn_ballot_w64(mn > m) || any_far; }
+    __device__ __forceinline__ bool due(float mn) const
+    {
+        if constexpr (LAG > 0) return __builtin_amdgcn_ballot_w64((mn - m) * sc > (float)LAG) || any_far;
+        else return __builtin_amdgcn_ballot_w64(mn > m) || any_far;
+    }
     /* maximum mn of a tile's scores; returns what the sums so far are to be
      * multiplied by, and in *off what to take off the tile's scores */
     __device__ __forceinline__ float raise(float mn, float* off)
     {
         mn = fmaxf(mn, m);
-        const float c = __builtin_fmaf(-mn, sc, 14.0f), cn = far(c) ? 14.0f : c;
-        const bool was = far(__builtin_fmaf(-m, sc, 14.0f));
+        const float c = __builtin_fmaf(-mn, sc, BASE), cn = far(c) ? BASE : c;
+        const bool was = far(__builtin_fmaf(-m, sc, BASE));
         const float al = __builtin_amdgcn_exp2f(far(c) || was ? (m - mn) * sc : cn - cc);
         m = mn;
         cc = cn;
@@ -150,10 +192,11 @@ struct CaMax {
      * as rounded: off by up to 2^-24 of itself, less than scores of that size are by their 22 bits.) */
     __device__ __forceinline__ float unit(float l) const
     {
-        const float c = __builtin_fmaf(-m, sc, 14.0f);
+        const float c = __builtin_fmaf(-m, sc, BASE);
         return l == 0.0f ? -INFINITY : -c;
     }
 };
+using CaMax = CaMaxOf<14, 0>;
 
 /* halves that are infinite or NaN to 0; whether there were any */
 __device__ __forceinline__ bool ca_drop_bad(v4u& w)
@@ -192,7 +235,8 @@ __device__ __forceinline__ v4f ca_values(const LgKv& c, const uint8_t* v, int g,
 template <bool KV4>
 __device__ __forceinline__ v4f ca_values(const CAttnPaged& a, const uint8_t* v, const int* t, int g, int key, int d)
 {
-    return ca_values<KV4>(a.c, v + (size_t)max(a.page_at(t, key), 0) * a.c.seq, g, key & (a.page_rows() - 1), d);
+    const int id = a.entry(t, key);   /* (of a key that is seen: a page) */
+    return ca_values<KV4>(a.c, v + (size_t)(a.is_page(id) ? id : 0) * a.c.seq, g, key & (a.page_rows() - 1), d);
 }
 
 /* o plus those of x that are infinite or NaN */
@@ -317,14 +361,14 @@ struct CaRows {
             }
         }
     }
-    /* of pages: rows 16 u .. of the tile are 16 of page id[u] (-1: of whichever), row c16 the lane's */
-    __device__ __forceinline__ void load(const CAttnPaged& a, const uint8_t* base, int g, int kb, const int id[C::NU],
+    /* of pages: rows 16 u .. of the tile are 16 of one page, row c16 the lane's */
+    __device__ __forceinline__ void load(const CAttnPaged& a, const uint8_t* base, int g, int kb, const CaEntries& id,
                                          int c16, int c)
     {
 #pragma unroll
         for (int u = 0; u < C::NU; u++) {
             const int row = (kb + 16 * u) & (a.page_rows() - 1);
-            const uint8_t* const b = base + (size_t)max(id[u], 0) * a.c.seq;
+            const uint8_t* const b = base + id.at(a, u);
             if constexpr (KV4) {
                 const uint8_t* const p = b + lg_kv4_codes(a.c, g, row) + (c16 * (uint32_t)(HD / 2) + (C::RUN ? c * (HD / 8) : 4 * c));
 #pragma unroll
@@ -426,14 +470,13 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
         _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
         /* of pages: those of the present tile, the next and the one after (their
          * table entries are on their way a tile ahead) */
-        int id[NU], id1[NU], id2[NU];
+        CaEntries id, id1, id2;
         const int* trow = nullptr;
         int none = 0;   /* rows 16 u .. of the present tile have no page: bit u */
         if constexpr (A::paged) trow = a.table + (int64_t)seq * a.tstep * a.tstride;
-        auto ids_of = [&](int i, int (&to)[NU]) __attribute__((always_inline)) {
+        auto ids_of = [&](int i, CaEntries& to) __attribute__((always_inline)) {
             if constexpr (A::paged)
-#pragma unroll
-                for (int u = 0; u < NU; u++) to[u] = i < t1 ? a.page_at(trow, min(tiles.at(i) * KT + 16 * u, a.max_pos)) : -1;
+                if (i < t1) to.load(a, trow, tiles.at(i) * KT);
         };
         /* keys that some column does not see (wave-uniform) */
         auto partly = [&](int kb) {
@@ -441,10 +484,9 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
                 if (kb + KT > khi || kb < klo || none) return true;
             return kb + KT - 1 > pmin || (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks);
         };
-        auto sees = [&](int kb, int key) {
-            if constexpr (A::paged)
-                if (key < klo || key >= khi || (none >> ((key - kb) / 16) & 1)) return false;
-            return ca_sees(a, p, key);
+        auto sees = [&](int kb, int key) __attribute__((always_inline)) {
+            if constexpr (A::paged) return CaSeen(a, p, klo, khi)(key, kb, none);
+            else return ca_sees(a, p, key);
         };
         /* the lane's rows of the tile at kb.  Those that none of the columns at
          * one position sees give way to one that they do, so that whatever
@@ -503,9 +545,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
             if constexpr (A::paged) {
                 ids_of(it + 2 * NW, id2);
                 if (kn >= 0) K.load(a, kc, g, kn, id1, col, c);
-                none = 0;
-#pragma unroll
-                for (int u = 0; u < NU; u++) none |= id[u] < 0 ? 1 << u : 0;
+                none = id.none(a, NU);
             } else if (kn >= 0) {
                 rows_of(kn);
                 K.load(a, kc, g, kn, at, c);
@@ -515,8 +555,10 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
 #pragma unroll
                 for (int u = 0; u < NU; u++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!sees(kb, kb + 16 * u + 4 * c + i)) s[u][i] = -INFINITY;
+                    for (int i = 0; i < 4; i++) {
+                        if constexpr (A::paged) s[u][i] = sees(kb, kb + 16 * u + 4 * c + i) ? s[u][i] : -INFINITY;
+                        else if (!sees(kb, kb + 16 * u + 4 * c + i)) s[u][i] = -INFINITY;
+                    }
             }
             float mn = s[0][0];
 #pragma unroll
@@ -586,12 +628,10 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
                     }
             }
             kb = kn;
-            if constexpr (A::paged)
-#pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    id[u] = id1[u];
-                    id1[u] = id2[u];
-                }
+            if constexpr (A::paged) {
+                id = id1;
+                id1 = id2;
+            }
         }
         l += lg_partner<4>(l);
         l += lg_partner<5>(l);
@@ -634,355 +674,6 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
             *(v4f*)(a.out + r * a.os + (size_t)hh * HD + d) = pk < 0 || pk > a.max_pos || (A::paged && L == 0.0f) ? (v4f){} : y * inv;
         }
     }
-}
-
-/* Prompts: 32 columns (query heads of a key head, tokens in order) a wave, NW
- * waves a workgroup, which share tiles of KT keys in LDS; both products on
- * 32 x 32 x 16 fp16 MFMA with the operands of k_cattn_dec: lane l feeds row /
- * column l % 32, k = 8 (l / 32) .. +7, register i of a result is row 8 (i / 4)
- * + 4 (l / 32) + i % 4 of column l % 32, so registers 8s .. 8s+7 of the scores
- * are the lane's k of step s of the second product: keys 16s + 4h .. and
- * 16s + 8 + 4h .. of lane half h.  The next tile is on its way while one
- * computes (two LDS stages, one barrier a tile).  Bound by the MFMA and VALU
- * work of a SIMD's two waves, 51 % and 44 % of the cycles, at 2.04 of 2.4 GHz
- * (keeping the waves half a tile apart, products and softmax interleaved by
- * hand, or V's fragments read a step ahead was no faster): 2000 tokens over
- * windows of 4096 rows 260 us, 520 TFLOP/s of the products asked for, 1040 issued
- * with the parts, 0.88 of what torch's fp16 product reaches on this card.  One
- * wave a SIMD does a tile in 0.9 of the time of two: two to a SIMD wherever
- * there are columns enough. */
-template <int HD, bool KV4, int NW_>
-struct CaTile {
-    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;
-    static constexpr int NJ = HD / 16, NT = (HD + 31) / 32;
-    static constexpr int KST = HD + 8;                       /* halves per K row in LDS */
-    static constexpr int VST = NT * 32 + 32;                 /* and per V row: rows 64 bytes on */
-    static constexpr int PW = KV4 ? 16 : 8;                  /* values of a piece that a thread moves */
-    static constexpr int PR = HD / PW, NP = (KT * PR + NTH - 1) / NTH;   /* pieces of a row; of a tile per thread */
-    static constexpr int STAGE = KT * (KST + VST);           /* halves */
-};
-
-template <int HD, bool KV4, int NW>
-struct CaPieces {
-    using C = CaTile<HD, KV4, NW>;
-    v4u h[KV4 ? 1 : C::NP];
-    uint2 w[KV4 ? C::NP : 1];
-    uint32_t dm[KV4 ? C::NP : 1];
-
-    /* (the tile's address is the wave's, a thread's part of it fits 32 bits) */
-    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb)
-    {
-        const uint8_t* const p = base + (KV4 ? lg_kv4_codes(a.c, g, kb) : lg_kv16_at(a.c, g, kb));
-        const uint8_t* const q = base + (KV4 ? lg_kv4_dm(a.c, g, kb) : 0);
-        const int last = a.max_pos - kb;   /* (rows past it are never visible) */
-#pragma unroll
-        for (int u = 0; u < C::NP; u++) {
-            const int i = min((int)threadIdx.x + u * C::NTH, C::KT * C::PR - 1);
-            const uint32_t key = min(i / C::PR, last), x = i % C::PR;
-            if constexpr (KV4) {
-                w[u] = *(const uint2*)(p + (key * (HD / 2) + 8 * x));
-                dm[u] = *(const uint32_t*)(q + (key * (HD / 8) + x / 2 * 4));
-            } else
-                h[u] = *(const v4u*)(p + (key * (uint32_t)(a.c.n_kv * HD * 2) + 16 * x));
-        }
-    }
-    /* of pages: rows 16 j .. of the tile are 16 of page id[j] (-1: of whichever) */
-    __device__ __forceinline__ void load(const CAttnPaged& a, const uint8_t* base, int g, int kb, const int id[C::KT / 16])
-    {
-#pragma unroll
-        for (int u = 0; u < C::NP; u++) {
-            const int i = min((int)threadIdx.x + u * C::NTH, C::KT * C::PR - 1);
-            const int key = i / C::PR, x = i % C::PR, row = (kb + key) & (a.page_rows() - 1);
-            int n = id[0];
-#pragma unroll
-            for (int j = 1; j < C::KT / 16; j++) n = key >= 16 * j ? id[j] : n;
-            const uint8_t* const b = base + (size_t)(uint32_t)max(n, 0) * a.c.seq;
-            if constexpr (KV4) {
-                w[u] = *(const uint2*)(b + lg_kv4_codes(a.c, g, row) + 8 * x);
-                dm[u] = *(const uint32_t*)(b + lg_kv4_dm(a.c, g, row) + x / 2 * 4);
-            } else
-                h[u] = *(const v4u*)(b + lg_kv16_at(a.c, g, row) + 16 * x);
-        }
-    }
-    /* into rows of ST halves; with `bad`, infinities and NaN as 0 and their keys noted */
-    template <int ST>
-    __device__ __forceinline__ void store(_Float16* dst, uint32_t* bad) const
-    {
-#pragma unroll
-        for (int u = 0; u < C::NP; u++) {
-            const int i = threadIdx.x + u * C::NTH;
-            if ((C::KT * C::PR) % C::NTH == 0 || i < C::KT * C::PR) {
-                _Float16* const q = dst + i / C::PR * ST + i % C::PR * C::PW;
-                v4u x[C::PW / 8];
-                if constexpr (KV4) {
-                    lg_kv4_values(w[u].x, dm[u], (lg_h2*)&x[0]);
-                    lg_kv4_values(w[u].y, dm[u], (lg_h2*)&x[1]);
-                } else
-                    x[0] = h[u];
-                if (bad) {
-                    bool any = false;
-#pragma unroll
-                    for (int e = 0; e < C::PW / 8; e++) any |= ca_drop_bad(x[e]);
-                    if (any) atomicOr(bad + i / C::PR / 32, 1u << (i / C::PR % 32));
-                }
-#pragma unroll
-                for (int e = 0; e < C::PW / 8; e++) *(v4u*)(q + 8 * e) = x[e];
-            }
-        }
-    }
-};
-
-/* (256 registers a lane, or 512 where those would not do) */
-template <int HD, bool KV4, int NW, class A>
-__global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4) ? 2 : 1)) void k_cattn_tile(
-    A a, int ncb, int nsplit, float* __restrict__ part)
-{
-    using C = CaTile<HD, KV4, NW>;
-    constexpr int KT = C::KT, NK = C::NK, NJ = C::NJ, NT = C::NT;
-    __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
-    __shared__ int s_pos[2 * C::NW];
-    __shared__ uint32_t s_bad[3][2];
-    /* key head fastest; the last columns, which may see most, first */
-    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv;
-    const int seq = blockIdx.x / n_kv % (a.rows / a.ntok), rest = blockIdx.x / n_kv / (a.rows / a.ntok);
-    const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 31, h = lane >> 5;
-    const int ncol = a.ntok * a.nrep, idx = cb * 32 * C::NW + 32 * wave + col;
-    const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
-    const int64_t row = (int64_t)seq * a.ntok + tok;
-    int p = a.pos[row];
-    if (idx >= ncol || p > a.max_pos) p = -1;
-    int wmin = p < 0 ? INT32_MAX : p, wmax = p;   /* of the wave */
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        wmin = min(wmin, __shfl_xor(wmin, o));
-        wmax = max(wmax, __shfl_xor(wmax, o));
-    }
-    if (lane == 0) {
-        s_pos[2 * wave] = wmin;
-        s_pos[2 * wave + 1] = wmax;
-    }
-    if (threadIdx.x < 6) s_bad[threadIdx.x / 2][threadIdx.x % 2] = 0;
-    __syncthreads();
-    wmin = __builtin_amdgcn_readfirstlane(wmin);
-    wmax = __builtin_amdgcn_readfirstlane(wmax);
-    int pmin = INT32_MAX, pmax = -1;              /* of the workgroup */
-#pragma unroll
-    for (int w = 0; w < C::NW; w++) {
-        pmin = min(pmin, s_pos[2 * w]);
-        pmax = max(pmax, s_pos[2 * w + 1]);
-    }
-    pmin = __builtin_amdgcn_readfirstlane(pmin);
-    pmax = __builtin_amdgcn_readfirstlane(pmax);
-
-    typedef float v16f __attribute__((ext_vector_type(16)));
-    v16f o[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) o[t] = (v16f){};
-    float l = 0.0f, unit = -INFINITY;
-    int klo = 0, khi = INT32_MAX;
-    if constexpr (A::paged) a.range(seq, &klo, &khi);
-    if (pmax >= 0) {
-        const CaTiles tiles = ca_tiles(a, pmin, pmax, KT, klo, khi);
-        int t0, t1;
-        tiles.chunk(sp, nsplit, 0, &t0, &t1);
-        const uint8_t* const kc = a.c.k + (A::paged ? 0 : (size_t)seq * a.c.seq);
-        const uint8_t* const vc = a.c.v + (A::paged ? 0 : (size_t)seq * a.c.seq);
-        /* tiles with keys that some row of the workgroup (wave) does not see */
-        int id[KT / 16], id1[KT / 16], id2[KT / 16];   /* pages, as in k_cattn_dec */
-        const int* trow = nullptr;
-        int none = 0, none1 = 0;                       /* of the present tile and the next */
-        if constexpr (A::paged) trow = a.table + (int64_t)seq * a.tstep * a.tstride;
-        auto ids_of = [&](int i, int (&to)[KT / 16]) __attribute__((always_inline)) {
-            if constexpr (A::paged)
-#pragma unroll
-                for (int u = 0; u < KT / 16; u++)
-                    to[u] = i < t1 ? a.page_at(trow, min(tiles.at(i) * KT + 16 * u, a.max_pos)) : -1;
-        };
-        auto none_of = [&](const int (&of)[KT / 16]) {
-            int m = 0;
-            if constexpr (A::paged)
-#pragma unroll
-                for (int u = 0; u < KT / 16; u++) m |= of[u] < 0 ? 1 << u : 0;
-            return m;
-        };
-        auto partly = [&](int kb, int lo, int hi, int without) {
-            if constexpr (A::paged)
-                if (kb + KT > khi || kb < klo || without) return true;
-            return kb + KT - 1 > lo || (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
-        };
-        auto sees = [&](int kb, int key) {
-            if constexpr (A::paged)
-                if (key < klo || key >= khi || (none >> ((key - kb) / 16) & 1)) return false;
-            return ca_sees(a, p, key);
-        };
-        CaPieces<HD, KV4, NW> P, V;
-        v8h qh[NJ], ql[NJ];
-        CaMax mx(0.0f);
-        {
-            /* queries, first keys and first values on their way together */
-            v4f x[2 * NJ];
-            const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * h;
-#pragma unroll
-            for (int j = 0; j < 2 * NJ; j++)
-                x[j] = idx < ncol ? *(const v4f*)(q + 16 * (j / 2) + 4 * (j % 2)) : (v4f){};
-            const int k0 = tiles.at(t0) * KT;
-            if (t0 < t1) {
-                if constexpr (A::paged) {
-                    ids_of(t0, id);
-                    ids_of(t0 + 1, id1);
-                    none = none_of(id);
-                    P.load(a, kc, g, k0, id);
-                    V.load(a, vc, g, k0, id);
-                } else {
-                    P.load(a, kc, g, k0);
-                    V.load(a, vc, g, k0);
-                }
-            }
-            float big = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 2 * NJ; j++)
-                big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
-            big = fmaxf(big, lg_partner<5>(big));
-            const int ex = __builtin_amdgcn_frexp_expf(big);
-            mx = CaMax(ca_scale(a.scale2, ex));
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
-            if (t0 < t1) {
-                P.template store<C::KST>(s_kv, nullptr);
-                V.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax, none) ? s_bad[0] : nullptr);
-            }
-        }
-        __syncthreads();
-        for (int it = t0; it < t1; it++) {
-            const bool more = it + 1 < t1;
-            const int kb = tiles.at(it) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
-            const int cur = (it - t0) & 1, nxt = cur ^ 1, slot = (it - t0) % 3;
-            _Float16* const sK = s_kv + cur * C::STAGE;
-            _Float16* const sV = sK + KT * C::KST;
-            _Float16* const nK = s_kv + nxt * C::STAGE;
-            const bool on = kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
-            if (more) {
-                if constexpr (A::paged) {
-                    P.load(a, kc, g, kn, id1);
-                    V.load(a, vc, g, kn, id1);
-                    none1 = none_of(id1);
-                    ids_of(it + 2, id2);
-                } else {
-                    P.load(a, kc, g, kn);
-                    V.load(a, vc, g, kn);
-                }
-            }
-            v16f s[NK];
-            if (on) {
-                /* its products ahead of the other wave's softmax: 700 x 9000 251 -> 243 us */
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int n = 0; n < NK; n++) s[n] = (v16f){};
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int n = 0; n < NK; n++) {
-                        const v8h k = *(const v8h*)(sK + (32 * n + col) * C::KST + 16 * j + 8 * h);
-                        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[j], s[n], 0, 0, 0);
-                        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[j], s[n], 0, 0, 0);
-                    }
-            }
-            __builtin_amdgcn_s_setprio(0);
-            if (more) P.template store<C::KST>(nK, nullptr);
-            if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
-            if (on) {
-                if (partly(kb, wmin, wmax, none)) {
-#pragma unroll
-                    for (int n = 0; n < NK; n++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (!sees(kb, kb + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3))) s[n][i] = -INFINITY;
-                }
-                float mn = s[0][0];
-#pragma unroll
-                for (int n = 0; n < NK; n++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) mn = fmaxf(mn, s[n][i]);
-                if (mx.due(mn)) {
-                    mn = fmaxf(mn, lg_partner<5>(mn));
-                    float off;
-                    const float al = mx.raise(mn, &off);
-                    l *= al;
-#pragma unroll
-                    for (int t = 0; t < NT; t++) o[t] *= al;
-#pragma unroll
-                    for (int n = 0; n < NK; n++) s[n] -= off;
-                }
-#pragma unroll
-                for (int st = 0; st < 2 * NK; st++) {
-                    float w[8];
-                    v8h ph, pl;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st / 2][8 * (st & 1) + i], mx.sc, mx.cc));
-                    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) ca_split2(w[i], w[i + 1], ph, pl, i);
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const _Float16* const v =
-                            sV + (16 * st + 4 * h + (lane & 15) / 4) * C::VST + 32 * t + (lane & 16) + 4 * (lane & 3);
-                        const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 8 * C::VST);
-                        const v8h x = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph, o[t], 0, 0, 0);
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl, o[t], 0, 0, 0);
-                    }
-                }
-                /* infinities and NaN of keys that only some rows see: added by
-                 * itself to those that do, whatever the (positive) weight */
-#pragma unroll
-                for (int n = 0; n < NK; n++)
-                    for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][n]); keys; keys &= keys - 1) {
-                        const int key = kb + 32 * n + __builtin_ctz(keys);
-                        if (sees(kb, key))
-#pragma unroll
-                            for (int t = 0; t < NT; t++)
-#pragma unroll
-                                for (int i = 0; i < 16; i += 4) {
-                                    const int d = 32 * t + 2 * i + 4 * h;
-                                    if (HD % 32 != 0 && d >= HD) continue;
-                                    v4f x;
-                                    if constexpr (A::paged) x = ca_values<KV4>(a, vc, trow, g, key, d);
-                                    else x = ca_values<KV4>(a.c, vc, g, key, d);
-#pragma unroll
-                                    for (int e = 0; e < 4; e++) o[t][i + e] = ca_add_bad(o[t][i + e], x[e]);
-                                }
-                    }
-            }
-            if (more) V.template store<C::VST>(nK + KT * C::KST, partly(kn, pmin, pmax, none1) ? s_bad[(slot + 1) % 3] : nullptr);
-            if constexpr (A::paged) {
-                none = none1;
-#pragma unroll
-                for (int u = 0; u < KT / 16; u++) id1[u] = id2[u];
-            }
-            __syncthreads();
-        }
-        l += lg_partner<5>(l);
-        unit = mx.unit(l);
-    }
-    if (idx >= ncol) return;
-    const int64_t at = ((int64_t)ca_part(a, sp) * a.rows + row) * a.n_heads + head;
-    float* const dst = part ? part + at * HD : a.out + row * a.os + (size_t)head * HD;
-    const float f = part ? 1.0f : 1.0f / l;   /* (0: every visible key is -infinity) */
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = 32 * t + 2 * i + 4 * h;
-            const v4f y = {o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
-            if (HD % 32 == 0 || d < HD) *(v4f*)(dst + d) = p < 0 || (A::paged && !part && l == 0.0f) ? (v4f){} : y * f;
-        }
-    if (part && h == 0) ca_part_ml(a, ca_nparts(a, nsplit), part, HD, at) = make_float2(unit, l);
 }
 
 /* The parts of a row's head together: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M).

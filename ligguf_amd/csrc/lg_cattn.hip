@@ -1,6 +1,289 @@
 /* lg_cattn.hip -- attention of many rows over contiguous caches that callers keep:
- * plan, launch and entry points (the kernels: lg_cattn.h). */
+ * prompts, plan, launch and entry points (single tokens and joins: lg_cattn.h). */
 #include "lg_cattn.h"
+
+/* Prompts: 32 columns (query heads of a key head, tokens in order) a wave, NW
+ * waves a workgroup, which share tiles of KT keys in LDS; both products on
+ * 32 x 32 x 16 fp16 MFMA with the operands of k_cattn_dec: lane l feeds row /
+ * column l % 32, k = 8 (l / 32) .. +7, register i of a result is row 8 (i / 4)
+ * + 4 (l / 32) + i % 4 of column l % 32, so registers 8s .. 8s+7 of the scores
+ * are the lane's k of step s of the second product: keys 16s + 4h .. and
+ * 16s + 8 + 4h .. of lane half h.  The next tile is on its way while one
+ * computes (two LDS stages, one barrier a tile).  Bound by the MFMA and VALU
+ * work of a SIMD's two waves, 51 % and 44 % of the cycles, at 2.04 of 2.4 GHz
+ * (keeping the waves half a tile apart, products and softmax interleaved by
+ * hand, or V's fragments read a step ahead was no faster): 2000 tokens over
+ * windows of 4096 rows 260 us, 520 TFLOP/s of the products asked for, 1040 issued
+ * with the parts, 0.88 of what torch's fp16 product reaches on this card.  One
+ * wave a SIMD does a tile in 0.9 of the time of two: two to a SIMD wherever
+ * there are columns enough. */
+template <int HD, bool KV4, int NW_>
+struct CaTile {
+    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32, NK = KT / 32;
+    static constexpr int NJ = HD / 16, NT = (HD + 31) / 32;
+    static constexpr int KST = HD + 8;                       /* halves per K row in LDS */
+    static constexpr int VST = NT * 32 + 32;                 /* and per V row: rows 64 bytes on */
+    static constexpr int PW = KV4 ? 16 : 8;                  /* values of a piece that a thread moves */
+    static constexpr int PR = HD / PW, NP = (KT * PR + NTH - 1) / NTH;   /* pieces of a row; of a tile per thread */
+    static constexpr int STAGE = KT * (KST + VST);           /* halves */
+};
+
+template <int HD, bool KV4, int NW>
+struct CaPieces {
+    using C = CaTile<HD, KV4, NW>;
+    v4u h[KV4 ? 1 : C::NP];
+    uint2 w[KV4 ? C::NP : 1];
+    uint32_t dm[KV4 ? C::NP : 1];
+
+    /* (the tile's address is the wave's, a thread's part of it fits 32 bits) */
+    __device__ __forceinline__ void load(const CAttn& a, const uint8_t* base, int g, int kb)
+    {
+        const uint8_t* const p = base + (KV4 ? lg_kv4_codes(a.c, g, kb) : lg_kv16_at(a.c, g, kb));
+        const uint8_t* const q = base + (KV4 ? lg_kv4_dm(a.c, g, kb) : 0);
+        const int last = a.max_pos - kb;   /* (rows past it are never visible) */
+#pragma unroll
+        for (int u = 0; u < C::NP; u++) {
+            const int i = min((int)threadIdx.x + u * C::NTH, C::KT * C::PR - 1);
+            const uint32_t key = min(i / C::PR, last), x = i % C::PR;
+            if constexpr (KV4) {
+                w[u] = *(const uint2*)(p + (key * (HD / 2) + 8 * x));
+                dm[u] = *(const uint32_t*)(q + (key * (HD / 8) + x / 2 * 4));
+            } else
+                h[u] = *(const v4u*)(p + (key * (uint32_t)(a.c.n_kv * HD * 2) + 16 * x));
+        }
+    }
+    /* into rows of ST halves; with `bad`, infinities and NaN as 0 and their keys noted */
+    template <int ST>
+    __device__ __forceinline__ void store(_Float16* dst, uint32_t* bad) const
+    {
+#pragma unroll
+        for (int u = 0; u < C::NP; u++) {
+            const int i = threadIdx.x + u * C::NTH;
+            if ((C::KT * C::PR) % C::NTH == 0 || i < C::KT * C::PR) {
+                _Float16* const q = dst + i / C::PR * ST + i % C::PR * C::PW;
+                v4u x[C::PW / 8];
+                if constexpr (KV4) {
+                    lg_kv4_values(w[u].x, dm[u], (lg_h2*)&x[0]);
+                    lg_kv4_values(w[u].y, dm[u], (lg_h2*)&x[1]);
+                } else
+                    x[0] = h[u];
+                if (bad) {
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < C::PW / 8; e++) any |= ca_drop_bad(x[e]);
+                    if (any) atomicOr(bad + i / C::PR / 32, 1u << (i / C::PR % 32));
+                }
+#pragma unroll
+                for (int e = 0; e < C::PW / 8; e++) *(v4u*)(q + 8 * e) = x[e];
+            }
+        }
+    }
+};
+
+/* (256 registers a lane, or 512 where those would not do) */
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 8 || HD < 128 || (HD == 128 && KV4) ? 2 : 1)) void k_cattn_tile(
+    CAttn a, int ncb, int nsplit, float* __restrict__ part)
+{
+    using C = CaTile<HD, KV4, NW>;
+    constexpr int KT = C::KT, NK = C::NK, NJ = C::NJ, NT = C::NT;
+    __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
+    __shared__ int s_pos[2 * C::NW];
+    __shared__ uint32_t s_bad[3][2];
+    /* key head fastest; the last columns, which may see most, first */
+    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv;
+    const int seq = blockIdx.x / n_kv % (a.rows / a.ntok), rest = blockIdx.x / n_kv / (a.rows / a.ntok);
+    const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    const int ncol = a.ntok * a.nrep, idx = cb * 32 * C::NW + 32 * wave + col;
+    const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
+    const int64_t row = (int64_t)seq * a.ntok + tok;
+    int p = a.pos[row];
+    if (idx >= ncol || p > a.max_pos) p = -1;
+    int wmin = p < 0 ? INT32_MAX : p, wmax = p;   /* of the wave */
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        wmin = min(wmin, __shfl_xor(wmin, o));
+        wmax = max(wmax, __shfl_xor(wmax, o));
+    }
+    if (lane == 0) {
+        s_pos[2 * wave] = wmin;
+        s_pos[2 * wave + 1] = wmax;
+    }
+    if (threadIdx.x < 6) s_bad[threadIdx.x / 2][threadIdx.x % 2] = 0;
+    __syncthreads();
+    wmin = __builtin_amdgcn_readfirstlane(wmin);
+    wmax = __builtin_amdgcn_readfirstlane(wmax);
+    int pmin = INT32_MAX, pmax = -1;              /* of the workgroup */
+#pragma unroll
+    for (int w = 0; w < C::NW; w++) {
+        pmin = min(pmin, s_pos[2 * w]);
+        pmax = max(pmax, s_pos[2 * w + 1]);
+    }
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
+
+    typedef float v16f __attribute__((ext_vector_type(16)));
+    v16f o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) o[t] = (v16f){};
+    float l = 0.0f, unit = -INFINITY;
+    if (pmax >= 0) {
+        const CaTiles tiles(a, pmin, pmax, KT);
+        int t0, t1;
+        tiles.chunk(sp, nsplit, 0, &t0, &t1);
+        const uint8_t* const kc = a.c.k + (size_t)seq * a.c.seq;
+        const uint8_t* const vc = a.c.v + (size_t)seq * a.c.seq;
+        /* tiles with keys that some row of the workgroup (wave) does not see */
+        auto partly = [&](int kb, int lo, int hi) {
+            return kb + KT - 1 > lo || (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
+        };
+        CaPieces<HD, KV4, NW> P, V;
+        v8h qh[NJ], ql[NJ];
+        CaMax mx(0.0f);
+        {
+            /* queries, first keys and first values on their way together */
+            v4f x[2 * NJ];
+            const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * h;
+#pragma unroll
+            for (int j = 0; j < 2 * NJ; j++)
+                x[j] = idx < ncol ? *(const v4f*)(q + 16 * (j / 2) + 4 * (j % 2)) : (v4f){};
+            const int k0 = tiles.at(t0) * KT;
+            if (t0 < t1) {
+                P.load(a, kc, g, k0);
+                V.load(a, vc, g, k0);
+            }
+            float big = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2 * NJ; j++)
+                big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
+            big = fmaxf(big, lg_partner<5>(big));
+            const int ex = __builtin_amdgcn_frexp_expf(big);
+            mx = CaMax(ca_scale(a.scale2, ex));
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
+            if (t0 < t1) {
+                P.template store<C::KST>(s_kv, nullptr);
+                V.template store<C::VST>(s_kv + KT * C::KST, partly(k0, pmin, pmax) ? s_bad[0] : nullptr);
+            }
+        }
+        __syncthreads();
+        for (int it = t0; it < t1; it++) {
+            const bool more = it + 1 < t1;
+            const int kb = tiles.at(it) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
+            const int cur = (it - t0) & 1, nxt = cur ^ 1, slot = (it - t0) % 3;
+            _Float16* const sK = s_kv + cur * C::STAGE;
+            _Float16* const sV = sK + KT * C::KST;
+            _Float16* const nK = s_kv + nxt * C::STAGE;
+            const bool on = kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
+            if (more) {
+                P.load(a, kc, g, kn);
+                V.load(a, vc, g, kn);
+            }
+            v16f s[NK];
+            if (on) {
+                /* its products ahead of the other wave's softmax: 700 x 9000 251 -> 243 us */
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int n = 0; n < NK; n++) s[n] = (v16f){};
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int n = 0; n < NK; n++) {
+                        const v8h k = *(const v8h*)(sK + (32 * n + col) * C::KST + 16 * j + 8 * h);
+                        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[j], s[n], 0, 0, 0);
+                        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[j], s[n], 0, 0, 0);
+                    }
+            }
+            __builtin_amdgcn_s_setprio(0);
+            if (more) P.template store<C::KST>(nK, nullptr);
+            if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
+            if (on) {
+                if (partly(kb, wmin, wmax)) {
+#pragma unroll
+                    for (int n = 0; n < NK; n++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (!ca_sees(a, p, kb + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3))) s[n][i] = -INFINITY;
+                }
+                float mn = s[0][0];
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) mn = fmaxf(mn, s[n][i]);
+                if (mx.due(mn)) {
+                    mn = fmaxf(mn, lg_partner<5>(mn));
+                    float off;
+                    const float al = mx.raise(mn, &off);
+                    l *= al;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) o[t] *= al;
+#pragma unroll
+                    for (int n = 0; n < NK; n++) s[n] -= off;
+                }
+#pragma unroll
+                for (int st = 0; st < 2 * NK; st++) {
+                    float w[8];
+                    v8h ph, pl;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st / 2][8 * (st & 1) + i], mx.sc, mx.cc));
+                    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) ca_split2(w[i], w[i + 1], ph, pl, i);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const _Float16* const v =
+                            sV + (16 * st + 4 * h + (lane & 15) / 4) * C::VST + 32 * t + (lane & 16) + 4 * (lane & 3);
+                        const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 8 * C::VST);
+                        const v8h x = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph, o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl, o[t], 0, 0, 0);
+                    }
+                }
+                /* infinities and NaN of keys that only some rows see: added by
+                 * itself to those that do, whatever the (positive) weight */
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+                    for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][n]); keys; keys &= keys - 1) {
+                        const int key = kb + 32 * n + __builtin_ctz(keys);
+                        if (ca_sees(a, p, key))
+#pragma unroll
+                            for (int t = 0; t < NT; t++)
+#pragma unroll
+                                for (int i = 0; i < 16; i += 4) {
+                                    const int d = 32 * t + 2 * i + 4 * h;
+                                    if (HD % 32 != 0 && d >= HD) continue;
+                                    const v4f x = ca_values<KV4>(a.c, vc, g, key, d);
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) o[t][i + e] = ca_add_bad(o[t][i + e], x[e]);
+                                }
+                    }
+            }
+            if (more) V.template store<C::VST>(nK + KT * C::KST, partly(kn, pmin, pmax) ? s_bad[(slot + 1) % 3] : nullptr);
+            __syncthreads();
+        }
+        l += lg_partner<5>(l);
+        unit = mx.unit(l);
+    }
+    if (idx >= ncol) return;
+    const int64_t at = ((int64_t)sp * a.rows + row) * a.n_heads + head;
+    float* const dst = part ? part + at * HD : a.out + row * a.os + (size_t)head * HD;
+    const float f = part ? 1.0f : 1.0f / l;   /* (0: every visible key is -infinity) */
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * t + 2 * i + 4 * h;
+            const v4f y = {o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
+            if (HD % 32 == 0 || d < HD) *(v4f*)(dst + d) = p < 0 ? (v4f){} : y * f;
+        }
+    if (part && h == 0) ca_part_ml(a, nsplit, part, HD, at) = make_float2(unit, l);
+}
 
 CaPlan lg_ca_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos,
                   bool kv4)
@@ -90,13 +373,13 @@ static void ca_launch(const CAttn& a, const CaPlan& p, int nseq, float* part, hi
     if constexpr (HD <= 128)
         if (p.wide) {
             if (p.dec) k_cattn_dec<HD, KV4, 8, CAttn><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
-            else k_cattn_tile<HD, KV4, 8, CAttn><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.nsplit, part);
+            else k_cattn_tile<HD, KV4, 8><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.nsplit, part);
             return;
         }
     if (p.dec)
         k_cattn_dec<HD, KV4, 4, CAttn><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
     else
-        k_cattn_tile<HD, KV4, 4, CAttn><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.nsplit, part);
+        k_cattn_tile<HD, KV4, 4><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.nsplit, part);
 }
 
 template <int HD>

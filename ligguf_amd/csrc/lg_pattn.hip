@@ -2,12 +2,633 @@
  * sequences shares once for the whole group (the kernels: lg_cattn.h). */
 #include "lg_cattn.h"
 
+constexpr int PT_NW = 16, PT_SLOTS = 256;
+
+/* Many columns: 16 a wave, NW
+ * waves a workgroup, which share tiles of KT keys in LDS; the products of
+ * k_cattn_dec, 32 keys at a time:
+ *   S^T[key][col] = K Q^T      O^T[d][col] += V^T P^T
+ * 16 columns rather than 32 take half the registers, so that a SIMD has four
+ * waves to fill each other's waits with.  The next tile's rows are on their way
+ * while one computes (two LDS stages, one barrier a tile), its table entries
+ * while the one before does.  Maxima lag by up to 2^8: raised but once or twice. */
+template <int HD, bool KV4, int NW_>
+struct PaTile {
+    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32;
+    static constexpr int NS = (HD + 31) / 32, NT = HD / 16;
+    static constexpr int KST = HD + 8, VST = HD + 16;        /* halves per K and V row in LDS: 4 and 8 banks on */
+    static constexpr int PW = KV4 ? 16 : 8, PR = HD / PW;    /* values of a piece that a thread moves, pieces of a row */
+    static constexpr int NP = (2 * KT * PR + NTH - 1) / NTH; /* of a tile's keys and values per thread */
+    static constexpr int STAGE = KT * (KST + VST);           /* halves */
+    static constexpr bool WHOLE = 64 % PR == 0 && 16 % (64 / PR) == 0;   /* a wave's piece is rows of one page */
+};
+
+/* what a thread holds of a tile: pieces of its keys, then of its values */
+template <int HD, bool KV4, int NW>
+struct PaPieces {
+    using C = PaTile<HD, KV4, NW>;
+    v4u h[KV4 ? 1 : C::NP];
+    uint2 w[KV4 ? C::NP : 1];
+    uint32_t dm[KV4 ? C::NP : 1];
+
+    /* the wave's piece u: its first one, from 0 on in keys and values */
+    static __device__ __forceinline__ int first(int u)
+    {
+        return __builtin_amdgcn_readfirstlane(threadIdx.x & ~63) + u * C::NTH;
+    }
+    __device__ __forceinline__ void load(const CAttnPaged& a, int g, int kb, const CaEntries& id)
+    {
+        const int mask = a.page_rows() - 1, lane = threadIdx.x & 63;
+        const uint32_t rb = KV4 ? HD / 2 : (uint32_t)a.c.n_kv * (HD * 2);                       /* bytes from row to row */
+        const uint32_t at0 = KV4 ? (uint32_t)g * a.c.n_ctx * (HD / 2) : (uint32_t)g * (HD * 2);   /* the head's in a page */
+        const uint32_t dm0 = (uint32_t)a.c.n_ctx * ((uint32_t)a.c.n_kv * (HD / 2) + (uint32_t)g * (HD / 8));
+#pragma unroll
+        for (int u = 0; u < C::NP; u++) {
+            int i = first(u);
+            if (i >= 2 * C::KT * C::PR) break;
+            const uint8_t* const base = i < C::KT * C::PR ? a.c.k : a.c.v;
+            i = i < C::KT * C::PR ? i : i - C::KT * C::PR;
+            size_t at;
+            uint32_t row, sub, x;   /* the wave's row and the lane's beyond it */
+            if constexpr (C::WHOLE) {
+                const int k0 = i / C::PR;
+                at = id.at(a, k0 / 16);
+                row = ((kb + k0) & mask & ~15) + k0 % 16;
+                sub = lane / C::PR;
+                x = lane % C::PR;
+            } else {
+                const int key = (i + lane) / C::PR;
+                at = id.at(a, 0);
+#pragma unroll
+                for (int j = 1; j < C::KT / 16; j++) at = key >= 16 * j ? id.at(a, j) : at;
+                row = (kb + key) & mask;
+                sub = 0;
+                x = (i + lane) % C::PR;
+            }
+            /* (a page's bytes fit 32 bits) */
+            const uint8_t* const b = base + at + (at0 + row * rb);
+            if constexpr (KV4) {
+                w[u] = *(const uint2*)(b + (sub * rb + 8 * x));
+                dm[u] = *(const uint32_t*)(base + at + (dm0 + row * (HD / 8)) + (sub * (HD / 8) + x / 2 * 4));
+            } else
+                h[u] = *(const v4u*)(b + (sub * rb + 16 * x));
+        }
+    }
+    /* into a stage; with `bad`, values' infinities and NaN as 0 and their keys noted */
+    __device__ __forceinline__ void store(_Float16* stage, uint32_t* bad) const
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < C::NP; u++) {
+            const int i0 = first(u);
+            if (i0 >= 2 * C::KT * C::PR) break;
+            const bool key_row = i0 < C::KT * C::PR;
+            const int i = (key_row ? i0 : i0 - C::KT * C::PR) + lane, r = i / C::PR;
+            _Float16* const q = stage + (key_row ? r * C::KST : C::KT * C::KST + r * C::VST) + i % C::PR * C::PW;
+            v4u x[C::PW / 8];
+            if constexpr (KV4) {
+                lg_kv4_values(w[u].x, dm[u], (lg_h2*)&x[0]);
+                lg_kv4_values(w[u].y, dm[u], (lg_h2*)&x[1]);
+            } else
+                x[0] = h[u];
+            if (bad && !key_row) {
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < C::PW / 8; e++) any |= ca_drop_bad(x[e]);
+                if (any) atomicOr(bad + r / 32, 1u << (r % 32));
+            }
+#pragma unroll
+            for (int e = 0; e < C::PW / 8; e++) *(v4u*)(q + 8 * e) = x[e];
+        }
+    }
+};
+
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAttnPaged a, int ncb, int nsplit,
+                                                                           float* __restrict__ part)
+{
+    using C = PaTile<HD, KV4, NW>;
+    constexpr int KT = C::KT, NS = C::NS, NT = C::NT;
+    __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
+    __shared__ int s_pos[2 * NW];
+    __shared__ uint32_t s_bad[3][2];
+    /* key head fastest; the last columns, which may see most, first */
+    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, units = a.rows / a.ntok;
+    const int unit = blockIdx.x / n_kv % units, rest = blockIdx.x / n_kv / units;
+    const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, c = lane >> 4;
+    const int ncol = a.ntok * a.nrep, idx = (cb * NW + wave) * 16 + col;
+    const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
+    const int64_t row = (int64_t)unit * a.ntok + tok;
+    int klo, khi;
+    a.range(unit, &klo, &khi);
+    int p = a.pos[row];
+    /* the columns' queries on their way */
+    v4f x[2 * NS];
+    {
+        const float* const q = a.q + row * a.qs + (size_t)head * HD + 8 * c;
+#pragma unroll
+        for (int j = 0; j < 2 * NS; j++) {
+            const int d = 32 * (j / 2) + 4 * (j % 2);
+            x[j] = idx < ncol && (HD % 32 == 0 || d + 8 * c < HD) ? *(const v4f*)(q + d) : (v4f){};
+        }
+    }
+    if (idx >= ncol || p > a.max_pos) p = -1;
+    int wmin = p < 0 ? INT32_MAX : p, wmax = p;   /* of the wave */
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+        wmin = min(wmin, __shfl_xor(wmin, o));
+        wmax = max(wmax, __shfl_xor(wmax, o));
+    }
+    if (lane == 0) {
+        s_pos[2 * wave] = wmin;
+        s_pos[2 * wave + 1] = wmax;
+    }
+    if (threadIdx.x < 6) s_bad[threadIdx.x / 2][threadIdx.x % 2] = 0;
+    __syncthreads();
+    wmin = __builtin_amdgcn_readfirstlane(wmin);
+    wmax = __builtin_amdgcn_readfirstlane(wmax);
+    int pmin = INT32_MAX, pmax = -1;              /* of the workgroup */
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        pmin = min(pmin, s_pos[2 * w]);
+        pmax = max(pmax, s_pos[2 * w + 1]);
+    }
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
+
+    v4f o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) o[t] = (v4f){};
+    float l = 0.0f, unit2 = -INFINITY;
+    const CaTiles tiles(a, pmin, pmax, KT, klo, khi);
+    int t0, t1;
+    tiles.chunk(sp, nsplit, 0, &t0, &t1);
+    if (t0 < t1) {   /* (workgroup-uniform) */
+        const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
+        /* tiles with keys that some row of the workgroup (wave) does not see */
+        auto partly = [&](int kb, int lo, int hi, int without) {
+            return kb + KT > khi || kb < klo || without || kb + KT - 1 > lo ||
+                   (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
+        };
+        const CaSeen seen(a, p, klo, khi);
+        CaEntries id, id1;   /* of the next tile and the one after */
+        PaPieces<HD, KV4, NW> P;
+        int none;            /* rows 16 j .. of the present tile have no page: bit j */
+        id.load(a, trow, tiles.at(t0) * KT);
+        id1.load(a, trow, tiles.at(min(t0 + 1, t1 - 1)) * KT);
+        P.load(a, g, tiles.at(t0) * KT, id);
+        none = id.none(a, KT / 16);
+        v8h qh[NS], ql[NS];
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * NS; j++)
+            big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
+        big = fmaxf(big, lg_partner<4>(big));
+        big = fmaxf(big, lg_partner<5>(big));
+        const int ex = __builtin_amdgcn_frexp_expf(big);
+        CaMaxOf<7, 8> mx(ca_scale(a.scale2, ex));
+#pragma unroll
+        for (int j = 0; j < NS; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
+        P.store(s_kv, partly(tiles.at(t0) * KT, pmin, pmax, none) ? s_bad[0] : nullptr);
+        __syncthreads();
+        for (int it = t0; it < t1; it++) {
+            const bool more = it + 1 < t1;
+            const int kb = tiles.at(it) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
+            const int cur = (it - t0) & 1, slot = (it - t0) % 3;
+            const _Float16* const sK = s_kv + cur * C::STAGE;
+            const _Float16* const sV = sK + KT * C::KST;
+            const bool on = kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
+            int none1 = 0;
+            if (more) {
+                id = id1;
+                id1.load(a, trow, tiles.at(min(it + 2, t1 - 1)) * KT);
+                P.load(a, g, kn, id);
+                none1 = id.none(a, KT / 16);
+            }
+            if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
+            if (on) {
+                const bool part_seen = partly(kb, wmin, wmax, none);
+                auto sees = [&](int key) __attribute__((always_inline)) { return seen(key, kb, none); };
+#pragma unroll
+                for (int b = 0; b < KT / 32; b++) {
+                    v4f s[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        s[u] = (v4f){};
+#pragma unroll
+                        for (int j = 0; j < NS; j++) {
+                            const v8h k = HD % 32 == 0 || 32 * j + 8 * c < HD ?
+                                              *(const v8h*)(sK + (32 * b + 16 * u + col) * C::KST + 32 * j + 8 * c) : (v8h){};
+                            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], s[u], 0, 0, 0);
+                            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], s[u], 0, 0, 0);
+                        }
+                    }
+                    if (part_seen) {
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                s[u][i] = sees(kb + 32 * b + 16 * u + 4 * c + i) ? s[u][i] : -INFINITY;
+                    }
+                    float mn = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+                    for (int i = 1; i < 4; i++) mn = fmaxf(mn, fmaxf(s[0][i], s[1][i]));
+                    if (mx.due(mn)) {
+                        mn = fmaxf(mn, lg_partner<4>(mn));
+                        mn = fmaxf(mn, lg_partner<5>(mn));
+                        float off;
+                        const float al = mx.raise(mn, &off);
+                        l *= al;
+#pragma unroll
+                        for (int t = 0; t < NT; t++) o[t] *= al;
+                        s[0] -= off;
+                        s[1] -= off;
+                    }
+                    v8h ph, pl;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], mx.sc, mx.cc));
+                        l += (w[0] + w[1]) + (w[2] + w[3]);
+                        ca_split2(w[0], w[1], ph, pl, 4 * u);
+                        ca_split2(w[2], w[3], ph, pl, 4 * u + 2);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const _Float16* const v = sV + (32 * b + 4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
+                        const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
+                        const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
+                    }
+                    /* infinities and NaN of keys that only some rows see: added by
+                     * itself to those that do, whatever the (positive) weight */
+                    if (part_seen)
+                        for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][b]); keys; keys &= keys - 1) {
+                            const int key = kb + 32 * b + __builtin_ctz(keys);
+                            if (sees(key))
+#pragma unroll
+                                for (int t = 0; t < NT; t++) {
+                                    const v4f y = ca_values<KV4>(a, a.c.v, trow, g, key, 16 * t + 4 * c);
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) o[t][i] = ca_add_bad(o[t][i], y[i]);
+                                }
+                        }
+                }
+            }
+            if (more) P.store(s_kv + (cur ^ 1) * C::STAGE, partly(kn, pmin, pmax, none1) ? s_bad[(slot + 1) % 3] : nullptr);
+            none = none1;
+            __syncthreads();
+        }
+        l += lg_partner<4>(l);
+        l += lg_partner<5>(l);
+        unit2 = mx.unit(l);
+    }
+    if (idx >= ncol) return;
+    const int64_t at = ((int64_t)(a.part0 + sp) * a.rows + row) * a.n_heads + head;
+    float* const dst = (part ? part + at * HD : a.out + row * a.os + (size_t)head * HD) + 4 * c;
+    const float f = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < NT; t++) *(v4f*)(dst + 16 * t) = p < 0 || (!part && l == 0.0f) ? (v4f){} : o[t] * f;
+    if (part && c == 0) ca_part_ml(a, a.nparts, part, HD, at) = make_float2(unit2, l);
+}
+
+/* More than 16 columns (query heads of a key head, tokens in order): 16 NCB a wave,
+ * the products of k_cattn_dec,
+ *   S^T[key][col] = K Q^T      O^T[d][col] += V^T P^T
+ * with each key's and value's fragment used for all of a wave's columns.  Of a
+ * workgroup's NW waves `cw` have columns of their own and NW / cw share those,
+ * each with tiles of KT keys of its own.  Waves with the same keys read them
+ * through the first-level cache and wait for nothing but their own loads: tiles
+ * shared in LDS cost more in barriers and address work, of which all waves
+ * then do the same at the same time, than their reads took.  Maxima lag by up
+ * to 2^8: raised but once or twice. */
+template <int HD, bool KV4, int NW, int NCB>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAttnPaged a, int ncb, int cw, int nsplit,
+                                                                           float* __restrict__ part)
+{
+    using C = CaDec<HD, KV4>;
+    constexpr int KT = C::KT, NU = C::NU, NB = C::NB, NS = C::NS, NT = C::NT;
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * C::WAVE];
+    __shared__ float s_ml[NW][16][2];
+    /* key head fastest, then columns, which read the same keys; the last ones, which may see most, first */
+    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, units = a.rows / a.ntok;
+    const int cb = ncb - 1 - blockIdx.x / n_kv % ncb, rest = blockIdx.x / n_kv / ncb, unit = rest % units, sp = rest / units;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = wave / cw, nkg = NW / cw, cwave = wave - kg * cw;
+    const int col = lane & 15, c = lane >> 4;
+    const int ncol = a.ntok * a.nrep, idx0 = ((cb * cw + cwave) * NCB) * 16 + col;
+    int klo, khi;
+    a.range(unit, &klo, &khi);
+    int p[NCB];
+    v4f x[NCB][2 * NS];
+    float big[NCB];
+#pragma unroll
+    for (int n = 0; n < NCB; n++) {
+        const int idx = idx0 + 16 * n, tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
+        const int64_t row = (int64_t)unit * a.ntok + tok;
+        p[n] = a.pos[row];
+        const float* const q = a.q + row * a.qs + (size_t)head * HD;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const int d = C::dim(s, c);
+            const bool in = idx < ncol && d < HD;
+            x[n][2 * s] = in ? *(const v4f*)(q + d) : (v4f){};
+            x[n][2 * s + 1] = in ? *(const v4f*)(q + d + 4) : (v4f){};
+        }
+    }
+    int pmin = INT32_MAX, pmax = -1;   /* of the wave's columns */
+#pragma unroll
+    for (int n = 0; n < NCB; n++) {
+        if (idx0 + 16 * n >= ncol || p[n] > a.max_pos) p[n] = -1;
+        pmin = min(pmin, p[n] < 0 ? INT32_MAX : p[n]);
+        pmax = max(pmax, p[n]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+        pmin = min(pmin, __shfl_xor(pmin, o));
+        pmax = max(pmax, __shfl_xor(pmax, o));
+    }
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
+
+    v4f o[NCB][NT];
+    float l[NCB], unit2[NCB];
+#pragma unroll
+    for (int n = 0; n < NCB; n++) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[n][t] = (v4f){};
+        l[n] = 0.0f;
+        unit2[n] = -INFINITY;
+    }
+    const CaTiles tiles(a, pmin, pmax, KT, klo, khi);
+    int t0, t1;
+    tiles.chunk(sp, nsplit, 0, &t0, &t1);
+    if (kg >= nkg) t1 = t0;   /* (a wave too many) */
+    if (t0 + kg < t1) {       /* (the wave's) */
+        _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
+        const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
+        int it = t0 + kg, kb = tiles.at(it) * KT;
+        CaEntries id, id1, id2;   /* of the present tile, the next and the one after */
+        CaRows<HD, KV4> K, V;
+        auto ids_of = [&](int i, CaEntries& to) __attribute__((always_inline)) { to.load(a, trow, tiles.at(min(i, t1 - 1)) * KT); };
+        ids_of(it, id);
+        ids_of(it + nkg, id1);
+        K.load(a, a.c.k, g, kb, id, col, c);
+        V.load(a, a.c.v, g, kb, id, col, c);
+        v8h qh[NCB][NS], ql[NCB][NS];
+        int ex[NCB];
+#pragma unroll
+        for (int n = 0; n < NCB; n++) {
+            big[n] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * NS; i++)
+                big[n] = fmaxf(fmaxf(big[n], fmaxf(fabsf(x[n][i][0]), fabsf(x[n][i][1]))), fmaxf(fabsf(x[n][i][2]), fabsf(x[n][i][3])));
+            big[n] = fmaxf(big[n], lg_partner<4>(big[n]));
+            big[n] = fmaxf(big[n], lg_partner<5>(big[n]));
+            ex[n] = __builtin_amdgcn_frexp_expf(big[n]);   /* big < 2^ex */
+#pragma unroll
+            for (int j = 0; j < NS; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    ca_query2(x[n][2 * j + e / 4][e % 4], x[n][2 * j + e / 4][e % 4 + 1], ex[n], qh[n][j], ql[n][j], e);
+        }
+        CaMaxOf<7, 8> mx[NCB] = {CaMaxOf<7, 8>(ca_scale(a.scale2, ex[0])), CaMaxOf<7, 8>(ca_scale(a.scale2, ex[NCB - 1]))};
+        for (; it < t1; it += nkg) {
+            v4f s[NU][NCB];
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+#pragma unroll
+                for (int n = 0; n < NCB; n++) s[u][n] = (v4f){};
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    const v8h k = __builtin_bit_cast(v8h, K.get(u, j));
+#pragma unroll
+                    for (int n = 0; n < NCB; n++) s[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[n][j], s[u][n], 0, 0, 0);
+#pragma unroll
+                    for (int n = 0; n < NCB; n++) s[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[n][j], s[u][n], 0, 0, 0);
+                }
+            }
+            const int kn = it + nkg < t1 ? tiles.at(it + nkg) * KT : -1;
+            ids_of(it + 2 * nkg, id2);
+            if (kn >= 0) K.load(a, a.c.k, g, kn, id1, col, c);
+            const int none = id.none(a, NU);
+            /* whether some column does not see some of the keys */
+            const bool part_seen = kb + KT > khi || kb < klo || none || kb + KT - 1 > pmin ||
+                                   (a.window > 0 && kb <= pmax - a.window && kb + KT > a.sinks);
+            if (part_seen) {
+#pragma unroll
+                for (int n = 0; n < NCB; n++) {
+                    const CaSeen seen(a, p[n], klo, khi);
+#pragma unroll
+                    for (int u = 0; u < NU; u++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[u][n][i] = seen(kb + 16 * u + 4 * c + i, kb, none) ? s[u][n][i] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NCB; n++) {
+                float mn = s[0][n][0];
+#pragma unroll
+                for (int u = 0; u < NU; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mn = fmaxf(mn, s[u][n][i]);
+                if (mx[n].due(mn)) {
+                    mn = fmaxf(mn, lg_partner<4>(mn));
+                    mn = fmaxf(mn, lg_partner<5>(mn));
+                    float off;
+                    const float al = mx[n].raise(mn, &off);
+                    l[n] *= al;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) o[n][t] *= al;
+#pragma unroll
+                    for (int u = 0; u < NU; u++) s[u][n] -= off;
+                }
+            }
+            uint64_t bad = 0;   /* keys of the tile */
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < NS; j++) {
+                        v4u y = V.get(2 * b + u, j);
+                        if (part_seen) bad |= ca_row16(__builtin_amdgcn_ballot_w64(ca_drop_bad(y))) << (32 * b + 16 * u);
+                        if (HD % 32 == 0 || C::dim(j, c) < HD) *(v4u*)(sV + (16 * u + col) * C::VST + C::dim(j, c)) = y;
+                    }
+                if (b == NB - 1 && kn >= 0) V.load(a, a.c.v, g, kn, id1, col, c);
+                v8h ph[NCB], pl[NCB];
+#pragma unroll
+                for (int n = 0; n < NCB; n++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * b + u][n][i], mx[n].sc, mx[n].cc));
+                        l[n] += (w[0] + w[1]) + (w[2] + w[3]);
+                        ca_split2(w[0], w[1], ph[n], pl[n], 4 * u);
+                        ca_split2(w[2], w[3], ph[n], pl[n], 4 * u + 2);
+                    }
+                ca_wave_sync();
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const _Float16* const v = sV + (4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
+                    const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
+                    const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int n = 0; n < NCB; n++) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph[n], o[n][t], 0, 0, 0);
+#pragma unroll
+                    for (int n = 0; n < NCB; n++) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl[n], o[n][t], 0, 0, 0);
+                }
+                ca_wave_sync();   /* (the reads before the next block's writes) */
+            }
+            /* infinities and NaN of keys that only some columns see: added by
+             * itself to those that do, whatever the (positive) weight */
+            for (; bad; bad &= bad - 1) {
+                const int key = kb + __builtin_ctzll(bad);
+#pragma unroll
+                for (int n = 0; n < NCB; n++)
+                    if (CaSeen(a, p[n], klo, khi)(key, kb, none))
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            const v4f y = ca_values<KV4>(a, a.c.v, trow, g, key, 16 * t + 4 * c);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[n][t][i] = ca_add_bad(o[n][t][i], y[i]);
+                        }
+            }
+            kb = kn;
+            id = id1;
+            id1 = id2;
+        }
+#pragma unroll
+        for (int n = 0; n < NCB; n++) {
+            l[n] += lg_partner<4>(l[n]);
+            l[n] += lg_partner<5>(l[n]);
+            unit2[n] = mx[n].unit(l[n]);
+        }
+    }
+    /* a column's sums, by one lane for four dims of each t: as a part, or as they are */
+    auto put = [&](int idx, int d, v4f y, float M, float L) __attribute__((always_inline)) {
+        if (idx >= ncol) return;
+        const int tok = idx / a.nrep, head = g * a.nrep + idx % a.nrep;
+        const int64_t row = (int64_t)unit * a.ntok + tok;
+        if (part) {
+            const int64_t at = ((int64_t)(a.part0 + sp) * a.rows + row) * a.n_heads + head;
+            if (L != 0.0f) *(v4f*)(part + at * HD + d) = y;
+            if (d == 0) ca_part_ml(a, a.nparts, part, HD, at) = make_float2(M, L);
+        } else {
+            const int pk = a.pos[row];
+            *(v4f*)(a.out + row * a.os + (size_t)head * HD + d) = pk < 0 || pk > a.max_pos || L == 0.0f ? (v4f){} : y * (1.0f / L);
+        }
+    };
+    if (nkg == 1) {
+        if (kg) return;
+#pragma unroll
+        for (int n = 0; n < NCB; n++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) put(idx0 + 16 * n, 16 * t + 4 * c, o[n][t], unit2[n], l[n]);
+        return;
+    }
+    /* the waves' parts of each column together, 16 columns of each at a time, by way of LDS */
+#pragma unroll
+    for (int n = 0; n < NCB; n++) {
+        float* const sO = (float*)(s_raw + wave * C::WAVE);
+        if (n) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; t++) *(v4f*)(sO + col * C::OST + 16 * t + 4 * c) = o[n][t];
+        if (c == 0) {
+            s_ml[wave][col][0] = unit2[n];
+            s_ml[wave][col][1] = l[n];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < cw * 16 * (HD / 4); i += 64 * NW) {
+            const int w0 = i / (16 * (HD / 4)), k = i / (HD / 4) % 16, d = i % (HD / 4) * 4;
+            float M = -INFINITY, L = 0.0f;
+            for (int w = w0; w < cw * nkg; w += cw) M = fmaxf(M, s_ml[w][k][0]);
+            v4f y = {};
+            for (int w = w0; w < cw * nkg; w += cw) {
+                /* (a wave without keys has l = 0 and all zeros) */
+                const float lw = s_ml[w][k][1], f = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][k][0] - M);
+                const v4f v = *(const v4f*)((const float*)(s_raw + w * C::WAVE) + k * C::OST + d);
+                L = __builtin_fmaf(lw, f, L);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(v[e], f, y[e]);
+            }
+            put(((cb * cw + w0) * NCB + n) * 16 + k, d, y, M, L);
+        }
+    }
+}
+
+/* How a phase is cut. */
+struct PaCut {
+    bool dec;            /* up to 16 columns a key head: k_cattn_dec, as over contiguous caches */
+    bool wide;           /* eight waves a workgroup, else four */
+    bool tile;
+    int cw, ncb;         /* else: waves with columns of their own, blocks of their columns */
+    int nsplit, chunk;   /* parts of the keys, tiles in a part */
+};
+
+static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos, bool kv4)
+{
+    const int64_t cols = ntok * (n_heads / n_kv);
+    PaCut p = {};
+    if (cols <= 16) {
+        const CaPlan d = lg_ca_plan(units, ntok, n_heads, n_kv, hd, window, sinks, max_pos, kv4);
+        p.dec = true;
+        p.wide = d.wide;
+        p.nsplit = d.nsplit;
+        p.chunk = d.chunk;
+        return p;
+    }
+    p.wide = hd <= 128;
+    const int nw = p.wide ? 8 : 4, kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec::KT) */
+    const int64_t nb = (cols + 31) / 32;
+    if (hd <= 128 && cols > 64) {
+        p.tile = true;
+        const int kt = 64;
+        p.ncb = (int)((cols + 16 * PT_NW - 1) / (16 * PT_NW));
+        int64_t keys = (int64_t)max_pos + 1;
+        if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
+        const double tiles = (double)((keys + kt - 1) / kt);
+        const int64_t wgs = units * n_kv * p.ncb;
+        double best = 0.0;
+        for (int ns = 1; ns <= 64 && (ns == 1 || tiles / ns >= 1.5); ns++) {
+            const double cost = (double)((wgs * ns + PT_SLOTS - 1) / PT_SLOTS) * (2.5 + tiles / ns) + (ns > 1 ? 1.0 + 0.5e-6 * ns * (double)(units * ntok) * n_heads * hd : 0.0);
+            if (ns == 1 || cost < best) {
+                best = cost;
+                p.nsplit = ns;
+            }
+        }
+        return p;
+    }
+    for (p.cw = nw; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
+    p.ncb = (int)((nb + p.cw - 1) / p.cw);
+    int64_t keys = (int64_t)max_pos + 1;
+    if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
+    const double tiles = (double)((keys + kt - 1) / kt) / (nw / p.cw);   /* of a wave */
+    const int64_t wgs = units * n_kv * p.ncb;
+    double best = 0.0;
+    for (int ns = 1; ns <= CA_PARTS && (ns == 1 || tiles / ns >= 1.0); ns++) {
+        const double cost = (double)((wgs * ns + 255) / 256) * (6.0 + tiles / ns) + (ns > 1 ? 2.0 + 1.5e-6 * ns * (double)(units * ntok) * n_heads * hd : 0.0);
+        if (ns == 1 || cost < best) {
+            best = cost;
+            p.nsplit = ns;
+        }
+    }
+    return p;
+}
+
 /* How a call is cut: the shared rows as a sequence of all the group's rows, the
- * others sequence by sequence, each as a call over contiguous caches would be;
- * their parts one behind the other. */
+ * others sequence by sequence; their parts one behind the other. */
 struct PaPlan {
     bool shared;
-    CaPlan a, b;   /* shared rows, own rows */
+    PaCut a, b;    /* shared rows, own rows */
     int parts;     /* 1: written out as they are */
     size_t ws;
 };
@@ -17,37 +638,38 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
 {
     PaPlan p = {};
     p.shared = group > 1 && max_prefix > 0;
-    if (p.shared) p.a = lg_ca_plan(nseq / group, ntok * group, n_heads, n_kv, hd, window, sinks, std::min(max_prefix - 1, max_pos), kv4);
+    if (p.shared) p.a = pa_cut(nseq / group, ntok * group, n_heads, n_kv, hd, window, sinks, std::min(max_prefix - 1, max_pos), kv4);
     /* (the own rows' number lies in device memory: of the longest prompt's) */
-    p.b = lg_ca_plan(nseq, ntok, n_heads, n_kv, hd, window, sinks, p.shared ? std::max(max_pos - max_prefix, 0) : max_pos, kv4);
+    p.b = pa_cut(nseq, ntok, n_heads, n_kv, hd, window, sinks, p.shared ? std::max(max_pos - max_prefix, 0) : max_pos, kv4);
     p.parts = p.b.nsplit + (p.shared ? p.a.nsplit : 0);
     if (p.parts > 1) p.ws = (size_t)p.parts * nseq * ntok * n_heads * (hd + 2) * sizeof(float);
     return p;
 }
 
 template <int HD, bool KV4>
-static void pa_launch(const CAttnPaged& a, const CaPlan& p, int units, float* part, hipStream_t s)
+static void pa_launch(const CAttnPaged& a, const PaCut& p, int units, float* part, hipStream_t s)
 {
     const int64_t n = (int64_t)units * a.c.n_kv * p.nsplit;
     if constexpr (HD <= 128)
         if (p.wide) {
             if (p.dec) k_cattn_dec<HD, KV4, 8, CAttnPaged><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
-            else k_cattn_tile<HD, KV4, 8, CAttnPaged><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.nsplit, part);
+            else if (p.tile) k_pattn_tile<HD, KV4, PT_NW><<<(unsigned)(n * p.ncb), 64 * PT_NW, 0, s>>>(a, p.ncb, p.nsplit, part);
+            else k_pattn_cols<HD, KV4, 8, 2><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.cw, p.nsplit, part);
             return;
         }
     if (p.dec) k_cattn_dec<HD, KV4, 4, CAttnPaged><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
-    else k_cattn_tile<HD, KV4, 4, CAttnPaged><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.nsplit, part);
+    else k_pattn_cols<HD, KV4, 4, 2><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.cw, p.nsplit, part);
 }
 
 template <int HD>
-static void pa_type(const CAttnPaged& a, const CaPlan& p, int units, float* part, hipStream_t s)
+static void pa_type(const CAttnPaged& a, const PaCut& p, int units, float* part, hipStream_t s)
 {
     if constexpr (HD != 48)
         if (a.c.type == LG_KV4) return pa_launch<HD, true>(a, p, units, part, s);
     pa_launch<HD, false>(a, p, units, part, s);
 }
 
-static void pa_phase(const CAttnPaged& a, const CaPlan& p, int units, float* part, hipStream_t s)
+static void pa_phase(const CAttnPaged& a, const PaCut& p, int units, float* part, hipStream_t s)
 {
     switch (a.c.hd) {
     case 48: pa_type<48>(a, p, units, part, s); break;
