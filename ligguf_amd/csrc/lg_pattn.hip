@@ -4,9 +4,8 @@
 
 constexpr int PT_NW = 16, PT_SLOTS = 256;
 
-/* Many columns: 16 a wave, NW
- * waves a workgroup, which share tiles of KT keys in LDS; the products of
- * k_cattn_dec, 32 keys at a time:
+/* Many columns: 16 a wave, NW waves a workgroup, which share tiles of KT keys in
+ * LDS; the products of k_cattn_dec, SB keys at a time:
  *   S^T[key][col] = K Q^T      O^T[d][col] += V^T P^T
  * 16 columns rather than 32 take half the registers, so that a SIMD has four
  * waves to fill each other's waits with.  The next tile's rows are on their way
@@ -14,7 +13,7 @@ constexpr int PT_NW = 16, PT_SLOTS = 256;
  * while the one before does.  Maxima lag by up to 2^8: raised but once or twice. */
 template <int HD, bool KV4, int NW_>
 struct PaTile {
-    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 64 : 32;
+    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 64 ? 128 : HD <= 128 ? 64 : 32, SB = HD <= 64 ? 64 : 32;
     static constexpr int NS = (HD + 31) / 32, NT = HD / 16;
     static constexpr int KST = HD + 8, VST = HD + 16;        /* halves per K and V row in LDS: 4 and 8 banks on */
     static constexpr int PW = KV4 ? 16 : 8, PR = HD / PW;    /* values of a piece that a thread moves, pieces of a row */
@@ -103,16 +102,28 @@ struct PaPieces {
     }
 };
 
+/* Whether some column of positions lo .. hi does not see some key of the tile at kb. */
+struct PaPartly {
+    int klo, last, wlo, sinks, kt;
+    __device__ __forceinline__ PaPartly(const CAttnPaged& a, int lo, int hi, int klo_, int khi, int kt_)
+        : klo(klo_), last(min(khi - 1, lo) - kt_ + 1), wlo(a.window > 0 ? hi - a.window : INT32_MIN), sinks(a.sinks), kt(kt_)
+    {
+    }
+    __device__ __forceinline__ bool operator()(int kb, int none) const
+    {
+        return (kb < klo) | (kb > last) | (none != 0) | ((kb <= wlo) & (kb + kt > sinks));
+    }
+};
+
 template <int HD, bool KV4, int NW>
-__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAttnPaged a, int ncb, int nsplit,
-                                                                           float* __restrict__ part)
+__global__ __launch_bounds__(64 * NW, 4) void k_pattn_tile(CAttnPaged a, int ncb, int nsplit, int chunk, float* __restrict__ part)
 {
     using C = PaTile<HD, KV4, NW>;
-    constexpr int KT = C::KT, NS = C::NS, NT = C::NT;
+    constexpr int KT = C::KT, NS = C::NS, NT = C::NT, SB = C::SB, NG = SB / 16;
     __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
     __shared__ int s_pos[2 * NW];
-    __shared__ uint32_t s_bad[3][2];
-    /* key head fastest; the last columns, which may see most, first */
+    __shared__ uint32_t s_bad[3][KT / 32];
+    /* key head fastest, then the units; the last columns, which may see most, first */
     const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, units = a.rows / a.ntok;
     const int unit = blockIdx.x / n_kv % units, rest = blockIdx.x / n_kv / units;
     const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
@@ -121,6 +132,17 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
     const int ncol = a.ntok * a.nrep, idx = (cb * NW + wave) * 16 + col;
     const int tok = min(idx, ncol - 1) / a.nrep, head = g * a.nrep + idx % a.nrep;
     const int64_t row = (int64_t)unit * a.ntok + tok;
+    const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
+    /* Without a window and from row 0 on the first tile is known: its entries and
+     * rows are on their way before the positions are (there is one, unless the
+     * unit has fewer keys than the launch was cut for). */
+    const bool early = a.window <= 0 && (a.share || !a.prefix);
+    CaEntries id, id1;   /* of the next tile and the one after */
+    PaPieces<HD, KV4, NW> P;
+    if (early) {
+        id.load(a, trow, sp * chunk * KT);
+        id1.load(a, trow, (sp * chunk + 1) * KT);
+    }
     int klo, khi;
     a.range(unit, &klo, &khi);
     int p = a.pos[row];
@@ -134,6 +156,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
             x[j] = idx < ncol && (HD % 32 == 0 || d + 8 * c < HD) ? *(const v4f*)(q + d) : (v4f){};
         }
     }
+    if (early) P.load(a, g, sp * chunk * KT, id);
     if (idx >= ncol || p > a.max_pos) p = -1;
     int wmin = p < 0 ? INT32_MAX : p, wmax = p;   /* of the wave */
 #pragma unroll
@@ -145,7 +168,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
         s_pos[2 * wave] = wmin;
         s_pos[2 * wave + 1] = wmax;
     }
-    if (threadIdx.x < 6) s_bad[threadIdx.x / 2][threadIdx.x % 2] = 0;
+    if (threadIdx.x < 3 * KT / 32) s_bad[threadIdx.x / (KT / 32)][threadIdx.x % (KT / 32)] = 0;
     __syncthreads();
     wmin = __builtin_amdgcn_readfirstlane(wmin);
     wmax = __builtin_amdgcn_readfirstlane(wmax);
@@ -164,22 +187,19 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
     float l = 0.0f, unit2 = -INFINITY;
     const CaTiles tiles(a, pmin, pmax, KT, klo, khi);
     int t0, t1;
-    tiles.chunk(sp, nsplit, 0, &t0, &t1);
+    tiles.chunk(sp, nsplit, chunk, &t0, &t1);
     if (t0 < t1) {   /* (workgroup-uniform) */
-        const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
         /* tiles with keys that some row of the workgroup (wave) does not see */
-        auto partly = [&](int kb, int lo, int hi, int without) {
-            return kb + KT > khi || kb < klo || without || kb + KT - 1 > lo ||
-                   (a.window > 0 && kb <= hi - a.window && kb + KT > a.sinks);
-        };
+        const PaPartly some(a, pmin, pmax, klo, khi, KT), mine(a, wmin, wmax, klo, khi, KT);
+        const int wfirst = a.window > 0 ? wmin - a.window - KT + 1 : INT32_MIN;   /* tiles up to it are before the wave's windows */
         const CaSeen seen(a, p, klo, khi);
-        CaEntries id, id1;   /* of the next tile and the one after */
-        PaPieces<HD, KV4, NW> P;
-        int none;            /* rows 16 j .. of the present tile have no page: bit j */
-        id.load(a, trow, tiles.at(t0) * KT);
-        id1.load(a, trow, tiles.at(min(t0 + 1, t1 - 1)) * KT);
-        P.load(a, g, tiles.at(t0) * KT, id);
-        none = id.none(a, KT / 16);
+        int kb = tiles.at(t0) * KT, kn = tiles.at(min(t0 + 1, t1 - 1)) * KT;
+        if (!early) {
+            id.load(a, trow, kb);
+            id1.load(a, trow, kn);
+            P.load(a, g, kb, id);
+        }
+        int none = id.none(a, KT / 16);   /* rows 16 j .. of the present tile have no page: bit j */
         v8h qh[NS], ql[NS];
         float big = 0.0f;
 #pragma unroll
@@ -193,50 +213,56 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
         for (int j = 0; j < NS; j++)
 #pragma unroll
             for (int e = 0; e < 8; e += 2) ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
-        P.store(s_kv, partly(tiles.at(t0) * KT, pmin, pmax, none) ? s_bad[0] : nullptr);
+        P.store(s_kv, some(kb, none) ? s_bad[0] : nullptr);
         __syncthreads();
         for (int it = t0; it < t1; it++) {
             const bool more = it + 1 < t1;
-            const int kb = tiles.at(it) * KT, kn = more ? tiles.at(it + 1) * KT : 0;
             const int cur = (it - t0) & 1, slot = (it - t0) % 3;
             const _Float16* const sK = s_kv + cur * C::STAGE;
             const _Float16* const sV = sK + KT * C::KST;
-            const bool on = kb <= wmax && (a.window <= 0 || kb + KT - 1 > wmin - a.window || kb < a.sinks);
+            const bool on = (kb <= wmax) & ((kb > wfirst) | (kb < a.sinks));
+            const int k2 = tiles.at(min(it + 2, t1 - 1)) * KT;
             int none1 = 0;
-            if (more) {
-                id = id1;
-                id1.load(a, trow, tiles.at(min(it + 2, t1 - 1)) * KT);
-                P.load(a, g, kn, id);
-                none1 = id.none(a, KT / 16);
-            }
-            if (threadIdx.x < 2) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
-            if (on) {
-                const bool part_seen = partly(kb, wmin, wmax, none);
-                auto sees = [&](int key) __attribute__((always_inline)) { return seen(key, kb, none); };
+            /* the next tile's rows: not at once, when all waves would work out addresses, but where they have drifted apart */
+            auto next = [&]() __attribute__((always_inline)) {
+                if (more) {
+                    id = id1;
+                    id1.load(a, trow, k2);
+                    P.load(a, g, kn, id);
+                    none1 = id.none(a, KT / 16);
+                }
+            };
+            if (threadIdx.x < KT / 32) s_bad[(slot + 2) % 3][threadIdx.x] = 0;
+            if (!on) next();
+            else {
+                const bool part_seen = mine(kb, none);
 #pragma unroll
-                for (int b = 0; b < KT / 32; b++) {
-                    v4f s[2];
+                for (int b = 0; b < KT / SB; b++) {
+                    v4f s[NG];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
+                    for (int u = 0; u < NG; u++) {
                         s[u] = (v4f){};
 #pragma unroll
                         for (int j = 0; j < NS; j++) {
                             const v8h k = HD % 32 == 0 || 32 * j + 8 * c < HD ?
-                                              *(const v8h*)(sK + (32 * b + 16 * u + col) * C::KST + 32 * j + 8 * c) : (v8h){};
+                                              *(const v8h*)(sK + (SB * b + 16 * u + col) * C::KST + 32 * j + 8 * c) : (v8h){};
                             s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], s[u], 0, 0, 0);
                             s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], s[u], 0, 0, 0);
                         }
                     }
+                    if (b == 0) next();
                     if (part_seen) {
 #pragma unroll
-                        for (int u = 0; u < 2; u++)
+                        for (int u = 0; u < NG; u++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                s[u][i] = sees(kb + 32 * b + 16 * u + 4 * c + i) ? s[u][i] : -INFINITY;
+                                s[u][i] = seen(kb + SB * b + 16 * u + 4 * c + i, kb, none) ? s[u][i] : -INFINITY;
                     }
-                    float mn = fmaxf(s[0][0], s[1][0]);
+                    float mn = s[0][0];
 #pragma unroll
-                    for (int i = 1; i < 4; i++) mn = fmaxf(mn, fmaxf(s[0][i], s[1][i]));
+                    for (int u = 0; u < NG; u++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mn = fmaxf(mn, s[u][i]);
                     if (mx.due(mn)) {
                         mn = fmaxf(mn, lg_partner<4>(mn));
                         mn = fmaxf(mn, lg_partner<5>(mn));
@@ -245,33 +271,38 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
                         l *= al;
 #pragma unroll
                         for (int t = 0; t < NT; t++) o[t] *= al;
-                        s[0] -= off;
-                        s[1] -= off;
-                    }
-                    v8h ph, pl;
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        float w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], mx.sc, mx.cc));
-                        l += (w[0] + w[1]) + (w[2] + w[3]);
-                        ca_split2(w[0], w[1], ph, pl, 4 * u);
-                        ca_split2(w[2], w[3], ph, pl, 4 * u + 2);
+                        for (int u = 0; u < NG; u++) s[u] -= off;
                     }
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const _Float16* const v = sV + (32 * b + 4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
-                        const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
-                        const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, o[t], 0, 0, 0);
-                        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
+                    for (int d = 0; d < SB / 32; d++) {
+                        v8h ph, pl;
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            float w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * d + u][i], mx.sc, mx.cc));
+                            l += (w[0] + w[1]) + (w[2] + w[3]);
+                            ca_split2(w[0], w[1], ph, pl, 4 * u);
+                            ca_split2(w[2], w[3], ph, pl, 4 * u + 2);
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            const _Float16* const v = sV + (SB * b + 32 * d + 4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
+                            const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
+                            const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, o[t], 0, 0, 0);
+                            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
+                        }
                     }
-                    /* infinities and NaN of keys that only some rows see: added by
-                     * itself to those that do, whatever the (positive) weight */
-                    if (part_seen)
-                        for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][b]); keys; keys &= keys - 1) {
-                            const int key = kb + 32 * b + __builtin_ctz(keys);
-                            if (sees(key))
+                }
+                /* infinities and NaN of keys that only some rows see: added by
+                 * itself to those that do, whatever the (positive) weight */
+                if (part_seen)
+                    for (int w = 0; w < KT / 32; w++)
+                        for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][w]); keys; keys &= keys - 1) {
+                            const int key = kb + 32 * w + __builtin_ctz(keys);
+                            if (seen(key, kb, none))
 #pragma unroll
                                 for (int t = 0; t < NT; t++) {
                                     const v4f y = ca_values<KV4>(a, a.c.v, trow, g, key, 16 * t + 4 * c);
@@ -279,10 +310,11 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
                                     for (int i = 0; i < 4; i++) o[t][i] = ca_add_bad(o[t][i], y[i]);
                                 }
                         }
-                }
             }
-            if (more) P.store(s_kv + (cur ^ 1) * C::STAGE, partly(kn, pmin, pmax, none1) ? s_bad[(slot + 1) % 3] : nullptr);
+            if (more) P.store(s_kv + (cur ^ 1) * C::STAGE, some(kn, none1) ? s_bad[(slot + 1) % 3] : nullptr);
             none = none1;
+            kb = kn;
+            kn = k2;
             __syncthreads();
         }
         l += lg_partner<4>(l);
@@ -291,11 +323,18 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 4 : 2)) void k_pattn_tile(CAt
     }
     if (idx >= ncol) return;
     const int64_t at = ((int64_t)(a.part0 + sp) * a.rows + row) * a.n_heads + head;
-    float* const dst = (part ? part + at * HD : a.out + row * a.os + (size_t)head * HD) + 4 * c;
-    const float f = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    if (!part) {
+        const float f = p < 0 || l == 0.0f ? 0.0f : 1.0f / l;
+        float* const dst = a.out + row * a.os + (size_t)head * HD + 4 * c;
 #pragma unroll
-    for (int t = 0; t < NT; t++) *(v4f*)(dst + 16 * t) = p < 0 || (!part && l == 0.0f) ? (v4f){} : o[t] * f;
-    if (part && c == 0) ca_part_ml(a, a.nparts, part, HD, at) = make_float2(unit2, l);
+        for (int t = 0; t < NT; t++) *(v4f*)(dst + 16 * t) = f == 0.0f && (p < 0 || l == 0.0f) ? (v4f){} : o[t] * f;
+        return;
+    }
+    if (l != 0.0f) {   /* (a part without keys is not read) */
+#pragma unroll
+        for (int t = 0; t < NT; t++) *(v4f*)(part + at * HD + 4 * c + 16 * t) = o[t];
+    }
+    if (c == 0) ca_part_ml(a, a.nparts, part, HD, at) = make_float2(unit2, l);
 }
 
 /* More than 16 columns (query heads of a key head, tokens in order): 16 NCB a wave,
@@ -591,7 +630,7 @@ static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, 
     const int64_t nb = (cols + 31) / 32;
     if (hd <= 128 && cols > 64) {
         p.tile = true;
-        const int kt = 64;
+        const int kt = hd <= 64 ? 128 : 64;   /* (PaTile::KT) */
         p.ncb = (int)((cols + 16 * PT_NW - 1) / (16 * PT_NW));
         int64_t keys = (int64_t)max_pos + 1;
         if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
@@ -605,6 +644,7 @@ static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, 
                 p.nsplit = ns;
             }
         }
+        p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
         return p;
     }
     for (p.cw = nw; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
@@ -653,7 +693,7 @@ static void pa_launch(const CAttnPaged& a, const PaCut& p, int units, float* par
     if constexpr (HD <= 128)
         if (p.wide) {
             if (p.dec) k_cattn_dec<HD, KV4, 8, CAttnPaged><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
-            else if (p.tile) k_pattn_tile<HD, KV4, PT_NW><<<(unsigned)(n * p.ncb), 64 * PT_NW, 0, s>>>(a, p.ncb, p.nsplit, part);
+            else if (p.tile) k_pattn_tile<HD, KV4, PT_NW><<<(unsigned)(n * p.ncb), 64 * PT_NW, 0, s>>>(a, p.ncb, p.nsplit, p.chunk, part);
             else k_pattn_cols<HD, KV4, 8, 2><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.cw, p.nsplit, part);
             return;
         }
