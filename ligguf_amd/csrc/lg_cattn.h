@@ -174,6 +174,12 @@ struct CaMaxOf {
         if constexpr (LAG > 0) return __builtin_amdgcn_ballot_w64((mn - m) * sc > (float)LAG) || any_far;
         else return __builtin_amdgcn_ballot_w64(mn > m) || any_far;
     }
+    /* whether some weights (sum: a lane's, which no one of them exceeds) are too far above the maximum */
+    __device__ __forceinline__ bool over(float sum) const
+    {
+        constexpr float most = (float)(1 << (BASE_ + LAG));
+        return __builtin_amdgcn_ballot_w64(sum > most) || any_far;
+    }
     /* maximum mn of a tile's scores; returns what the sums so far are to be
      * multiplied by, and in *off what to take off the tile's scores */
     __device__ __forceinline__ float raise(float mn, float* off)

@@ -2,7 +2,7 @@
  * sequences shares once for the whole group (the kernels: lg_cattn.h). */
 #include "lg_cattn.h"
 
-constexpr int PT_NW = 16, PT_SLOTS = 256;
+template <int HD> constexpr int PT_NW_OF = HD <= 64 ? 16 : 12;
 
 /* Many columns: 16 a wave, NW waves a workgroup, which share tiles of KT keys in
  * LDS; the products of k_cattn_dec, SB keys at a time:
@@ -13,9 +13,9 @@ constexpr int PT_NW = 16, PT_SLOTS = 256;
  * while the one before does.  Maxima lag by up to 2^8: raised but once or twice. */
 template <int HD, bool KV4, int NW_>
 struct PaTile {
-    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 64 ? 128 : HD <= 128 ? 64 : 32, SB = HD <= 64 ? 64 : 32;
+    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 128 : 32;
     static constexpr int NS = (HD + 31) / 32, NT = HD / 16;
-    static constexpr int KST = HD + 8, VST = HD + 16;        /* halves per K and V row in LDS: 4 and 8 banks on */
+    static constexpr int KST = HD + 16, VST = HD + 16;       /* halves per K and V row in LDS: 8 banks on, no conflicts (4 for K: 1 in 2) */
     static constexpr int PW = KV4 ? 16 : 8, PR = HD / PW;    /* values of a piece that a thread moves, pieces of a row */
     static constexpr int NP = (2 * KT * PR + NTH - 1) / NTH; /* of a tile's keys and values per thread */
     static constexpr int STAGE = KT * (KST + VST);           /* halves */
@@ -116,10 +116,10 @@ struct PaPartly {
 };
 
 template <int HD, bool KV4, int NW>
-__global__ __launch_bounds__(64 * NW, 4) void k_pattn_tile(CAttnPaged a, int ncb, int nsplit, int chunk, float* __restrict__ part)
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(CAttnPaged a, int ncb, int nsplit, int chunk, float* __restrict__ part)
 {
     using C = PaTile<HD, KV4, NW>;
-    constexpr int KT = C::KT, NS = C::NS, NT = C::NT, SB = C::SB, NG = SB / 16;
+    constexpr int KT = C::KT, NS = C::NS, NT = C::NT;
     __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
     __shared__ int s_pos[2 * NW];
     __shared__ uint32_t s_bad[3][KT / 32];
@@ -202,17 +202,20 @@ __global__ __launch_bounds__(64 * NW, 4) void k_pattn_tile(CAttnPaged a, int ncb
         int none = id.none(a, KT / 16);   /* rows 16 j .. of the present tile have no page: bit j */
         v8h qh[NS], ql[NS];
         float big = 0.0f;
+        CaMaxOf<7, 8> mx(0.0f);
+        if (wmax >= 0) {   /* (a wave without rows has but the tiles to move) */
 #pragma unroll
         for (int j = 0; j < 2 * NS; j++)
             big = fmaxf(fmaxf(big, fmaxf(fabsf(x[j][0]), fabsf(x[j][1]))), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
         big = fmaxf(big, lg_partner<4>(big));
         big = fmaxf(big, lg_partner<5>(big));
         const int ex = __builtin_amdgcn_frexp_expf(big);
-        CaMaxOf<7, 8> mx(ca_scale(a.scale2, ex));
+        mx = CaMaxOf<7, 8>(ca_scale(a.scale2, ex));
 #pragma unroll
         for (int j = 0; j < NS; j++)
 #pragma unroll
             for (int e = 0; e < 8; e += 2) ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
+        }
         P.store(s_kv, some(kb, none) ? s_bad[0] : nullptr);
         __syncthreads();
         for (int it = t0; it < t1; it++) {
@@ -237,15 +240,15 @@ __global__ __launch_bounds__(64 * NW, 4) void k_pattn_tile(CAttnPaged a, int ncb
             else {
                 const bool part_seen = mine(kb, none);
 #pragma unroll
-                for (int b = 0; b < KT / SB; b++) {
-                    v4f s[NG];
+                for (int b = 0; b < KT / 32; b++) {
+                    v4f s[2];
 #pragma unroll
-                    for (int u = 0; u < NG; u++) {
+                    for (int u = 0; u < 2; u++) {
                         s[u] = (v4f){};
 #pragma unroll
                         for (int j = 0; j < NS; j++) {
                             const v8h k = HD % 32 == 0 || 32 * j + 8 * c < HD ?
-                                              *(const v8h*)(sK + (SB * b + 16 * u + col) * C::KST + 32 * j + 8 * c) : (v8h){};
+                                              *(const v8h*)(sK + (32 * b + 16 * u + col) * C::KST + 32 * j + 8 * c) : (v8h){};
                             s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], s[u], 0, 0, 0);
                             s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], s[u], 0, 0, 0);
                         }
@@ -253,17 +256,23 @@ __global__ __launch_bounds__(64 * NW, 4) void k_pattn_tile(CAttnPaged a, int ncb
                     if (b == 0) next();
                     if (part_seen) {
 #pragma unroll
-                        for (int u = 0; u < NG; u++)
+                        for (int u = 0; u < 2; u++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                s[u][i] = seen(kb + SB * b + 16 * u + 4 * c + i, kb, none) ? s[u][i] : -INFINITY;
+                                s[u][i] = seen(kb + 32 * b + 16 * u + 4 * c + i, kb, none) ? s[u][i] : -INFINITY;
                     }
-                    float mn = s[0][0];
+                    /* the weights; whether one outgrew its maximum, their sum tells */
+                    float w[8], sum;
+                    auto weigh = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                    for (int u = 0; u < NG; u++)
+                        for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], mx.sc, mx.cc));
+                        sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                    };
+                    weigh();
+                    if (mx.over(sum)) {
+                        float mn = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) mn = fmaxf(mn, s[u][i]);
-                    if (mx.due(mn)) {
+                        for (int i = 1; i < 4; i++) mn = fmaxf(mn, fmaxf(s[0][i], s[1][i]));
                         mn = fmaxf(mn, lg_partner<4>(mn));
                         mn = fmaxf(mn, lg_partner<5>(mn));
                         float off;
@@ -271,29 +280,21 @@ __global__ __launch_bounds__(64 * NW, 4) void k_pattn_tile(CAttnPaged a, int ncb
                         l *= al;
 #pragma unroll
                         for (int t = 0; t < NT; t++) o[t] *= al;
-#pragma unroll
-                        for (int u = 0; u < NG; u++) s[u] -= off;
+                        s[0] -= off;
+                        s[1] -= off;
+                        weigh();
                     }
+                    l += sum;
+                    v8h ph, pl;
 #pragma unroll
-                    for (int d = 0; d < SB / 32; d++) {
-                        v8h ph, pl;
+                    for (int i = 0; i < 8; i += 2) ca_split2(w[i], w[i + 1], ph, pl, i);
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            float w[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * d + u][i], mx.sc, mx.cc));
-                            l += (w[0] + w[1]) + (w[2] + w[3]);
-                            ca_split2(w[0], w[1], ph, pl, 4 * u);
-                            ca_split2(w[2], w[3], ph, pl, 4 * u + 2);
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            const _Float16* const v = sV + (SB * b + 32 * d + 4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
-                            const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
-                            const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-                            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, o[t], 0, 0, 0);
-                            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
-                        }
+                    for (int t = 0; t < NT; t++) {
+                        const _Float16* const v = sV + (32 * b + 4 * c + col / 4) * C::VST + 16 * t + 4 * (col % 4);
+                        const v4s x0 = ca_tr16(v), x1 = ca_tr16(v + 16 * C::VST);
+                        const v8h y = __builtin_bit_cast(v8h, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
                     }
                 }
                 /* infinities and NaN of keys that only some rows see: added by
@@ -630,7 +631,7 @@ static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, 
     const int64_t nb = (cols + 31) / 32;
     if (hd <= 128 && cols > 64) {
         p.tile = true;
-        const int kt = hd <= 64 ? 128 : 64;   /* (PaTile::KT) */
+        const int kt = 128, PT_NW = hd <= 64 ? 16 : 12, PT_SLOTS = 256;   /* (PaTile::KT) */
         p.ncb = (int)((cols + 16 * PT_NW - 1) / (16 * PT_NW));
         int64_t keys = (int64_t)max_pos + 1;
         if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
@@ -693,7 +694,7 @@ static void pa_launch(const CAttnPaged& a, const PaCut& p, int units, float* par
     if constexpr (HD <= 128)
         if (p.wide) {
             if (p.dec) k_cattn_dec<HD, KV4, 8, CAttnPaged><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
-            else if (p.tile) k_pattn_tile<HD, KV4, PT_NW><<<(unsigned)(n * p.ncb), 64 * PT_NW, 0, s>>>(a, p.ncb, p.nsplit, p.chunk, part);
+            else if (p.tile) k_pattn_tile<HD, KV4, PT_NW_OF<HD>><<<(unsigned)(n * p.ncb), 64 * PT_NW_OF<HD>, 0, s>>>(a, p.ncb, p.nsplit, p.chunk, part);
             else k_pattn_cols<HD, KV4, 8, 2><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.cw, p.nsplit, part);
             return;
         }
