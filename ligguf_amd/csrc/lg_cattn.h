@@ -404,19 +404,19 @@ struct CaRows {
 };
 
 template <int HD, bool KV4, int NW, class A>
-__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a, int nsplit, int chunk,
-                                                                           float* __restrict__ part)
+__device__ __forceinline__ void ca_dec(const A& a, int blk, int nsplit, int chunk, float* __restrict__ part, uint8_t* s_raw,
+                                       float (*s_ml)[16][2])
 {
     using C = CaDec<HD, KV4>;
     constexpr int KT = C::KT, NU = C::NU, NB = C::NB, NS = C::NS, NT = C::NT;
-    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * C::WAVE];
-    __shared__ float s_ml[NW][16][2];
-    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, sp = blockIdx.x / n_kv % nsplit, seq = blockIdx.x / n_kv / nsplit;
+    const int n_kv = a.c.n_kv, g = blk % n_kv, sp = blk / n_kv % nsplit, seq = blk / n_kv / nsplit;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, c = lane >> 4;
     const int tok = col / a.nrep, ncol = a.ntok * a.nrep;
     const int64_t row = (int64_t)seq * a.ntok + min(tok, a.ntok - 1);
     const int head = g * a.nrep + col % a.nrep;
+    int klo = 0, khi = INT32_MAX;
+    if constexpr (A::paged) a.range(seq, &klo, &khi);
     int p = a.pos[row];
     /* the column's query, on its way before the first keys: loads come back in order */
     v4f x[2 * NS];
@@ -446,6 +446,25 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
             K.load(a, kc, g, early, at, c);
             V.load(a, vc, g, early, at, c);
         }
+    /* Of pages, likewise: the table's entries and their rows, while the positions
+     * come.  (Which tile is the first is known: splits are of `chunk` tiles, unless
+     * the launch was cut for fewer keys; then that is not this wave's, and is read again.) */
+    CaEntries id, id1, id2;   /* of the present tile, the next and the one after */
+    const int* trow = nullptr;
+    int ahead = -1;
+    if constexpr (A::paged) {
+        trow = a.table + (int64_t)seq * a.tstep * a.tstride;
+        if (a.window <= 0) {
+            ahead = (klo / KT + sp * chunk + wave) * KT;
+            if (ahead > a.max_pos) ahead = -1;
+        }
+        if (ahead >= 0) {
+            id.load(a, trow, ahead);
+            id1.load(a, trow, ahead + NW * KT);
+            K.load(a, kc, g, ahead, id, col, c);
+            V.load(a, vc, g, ahead, id, col, c);
+        }
+    }
     if (col >= ncol || p > a.max_pos) p = -1;
     int pmin = p < 0 ? INT32_MAX : p, pmax = p;
 #pragma unroll
@@ -456,8 +475,6 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
     pmin = __builtin_amdgcn_readfirstlane(pmin);
     pmax = __builtin_amdgcn_readfirstlane(pmax);
 
-    int klo = 0, khi = INT32_MAX;
-    if constexpr (A::paged) a.range(seq, &klo, &khi);
     const CaTiles tiles = ca_tiles(a, pmin, pmax, KT, klo, khi);
     int t0, t1;
     tiles.chunk(sp, nsplit, chunk, &t0, &t1);
@@ -474,12 +491,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
     float l = 0.0f, unit = -INFINITY;   /* sum of weights (this lane's keys) */
     if (t0 + wave < t1) {
         _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
-        /* of pages: those of the present tile, the next and the one after (their
-         * table entries are on their way a tile ahead) */
-        CaEntries id, id1, id2;
-        const int* trow = nullptr;
         int none = 0;   /* rows 16 u .. of the present tile have no page: bit u */
-        if constexpr (A::paged) trow = a.table + (int64_t)seq * a.tstep * a.tstride;
         auto ids_of = [&](int i, CaEntries& to) __attribute__((always_inline)) {
             if constexpr (A::paged)
                 if (i < t1) to.load(a, trow, tiles.at(i) * KT);
@@ -509,10 +521,12 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
         };
         int it = t0 + wave, kb = tiles.at(it) * KT;
         if constexpr (A::paged) {
-            ids_of(it, id);
-            ids_of(it + NW, id1);
-            K.load(a, kc, g, kb, id, col, c);
-            V.load(a, vc, g, kb, id, col, c);
+            if (kb != ahead) {
+                ids_of(it, id);
+                ids_of(it + NW, id1);
+                K.load(a, kc, g, kb, id, col, c);
+                V.load(a, vc, g, kb, id, col, c);
+            }
         } else if (kb != early || (pmin == pmax && partly(kb))) {
             rows_of(kb);
             K.load(a, kc, g, kb, at, c);
@@ -680,6 +694,15 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(A a,
             *(v4f*)(a.out + r * a.os + (size_t)hh * HD + d) = pk < 0 || pk > a.max_pos || (A::paged && L == 0.0f) ? (v4f){} : y * inv;
         }
     }
+}
+
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_cattn_dec(CAttn a, int nsplit, int chunk,
+                                                                           float* __restrict__ part)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * CaDec<HD, KV4>::WAVE];
+    __shared__ float s_ml[NW][16][2];
+    ca_dec<HD, KV4, NW>(a, blockIdx.x, nsplit, chunk, part, s_raw, s_ml);
 }
 
 /* The parts of a row's head together: sum w_i o_i / sum w_i l_i, w_i = 2^(M_i - M).

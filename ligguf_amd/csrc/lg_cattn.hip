@@ -372,12 +372,12 @@ static void ca_launch(const CAttn& a, const CaPlan& p, int nseq, float* part, hi
     const int64_t n = (int64_t)nseq * a.c.n_kv * p.nsplit;
     if constexpr (HD <= 128)
         if (p.wide) {
-            if (p.dec) k_cattn_dec<HD, KV4, 8, CAttn><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
+            if (p.dec) k_cattn_dec<HD, KV4, 8><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
             else k_cattn_tile<HD, KV4, 8><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.nsplit, part);
             return;
         }
     if (p.dec)
-        k_cattn_dec<HD, KV4, 4, CAttn><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
+        k_cattn_dec<HD, KV4, 4><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
     else
         k_cattn_tile<HD, KV4, 4><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.nsplit, part);
 }

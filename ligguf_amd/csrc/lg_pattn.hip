@@ -2,7 +2,23 @@
  * sequences shares once for the whole group (the kernels: lg_cattn.h). */
 #include "lg_cattn.h"
 
-template <int HD> constexpr int PT_NW_OF = HD <= 64 ? 16 : 12;
+/* A phase of a call: the shared rows (units are groups) or the own ones
+ * (sequences), and how it is cut. */
+enum PaKind { PA_DEC, PA_COLS, PA_TILE };
+struct PaPhase {
+    CAttnPaged a;
+    int kind, ncb, cw, nsplit, chunk;
+};
+/* Both phases in one launch, the first one's workgroups before the second's. */
+struct PaArgs {
+    PaPhase f[2];
+    int na;
+    float* part;
+    __device__ __forceinline__ const PaPhase& of(int blk) const { return f[blk < na ? 0 : 1]; }
+    __device__ __forceinline__ int in(int blk) const { return blk < na ? blk : blk - na; }
+};
+
+constexpr int pa_waves(int hd) { return hd <= 64 ? 16 : 12; }   /* of k_pattn_tile's workgroups */
 
 /* Many columns: 16 a wave, NW waves a workgroup, which share tiles of KT keys in
  * LDS; the products of k_cattn_dec, SB keys at a time:
@@ -116,16 +132,20 @@ struct PaPartly {
 };
 
 template <int HD, bool KV4, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(CAttnPaged a, int ncb, int nsplit, int chunk, float* __restrict__ part)
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
 {
     using C = PaTile<HD, KV4, NW>;
     constexpr int KT = C::KT, NS = C::NS, NT = C::NT;
+    const PaPhase& f = args.of(blockIdx.x);
+    const CAttnPaged& a = f.a;
+    const int ncb = f.ncb, nsplit = f.nsplit, chunk = f.chunk, blk = args.in(blockIdx.x);
+    float* const part = args.part;
     __shared__ __attribute__((aligned(16))) _Float16 s_kv[2 * C::STAGE];
     __shared__ int s_pos[2 * NW];
     __shared__ uint32_t s_bad[3][KT / 32];
     /* key head fastest, then the units; the last columns, which may see most, first */
-    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, units = a.rows / a.ntok;
-    const int unit = blockIdx.x / n_kv % units, rest = blockIdx.x / n_kv / units;
+    const int n_kv = a.c.n_kv, g = blk % n_kv, units = a.rows / a.ntok;
+    const int unit = blk / n_kv % units, rest = blk / n_kv / units;
     const int sp = rest % nsplit, cb = ncb - 1 - rest / nsplit;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, c = lane >> 4;
@@ -194,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(CAttnPaged a, in
         const int wfirst = a.window > 0 ? wmin - a.window - KT + 1 : INT32_MIN;   /* tiles up to it are before the wave's windows */
         const CaSeen seen(a, p, klo, khi);
         int kb = tiles.at(t0) * KT, kn = tiles.at(min(t0 + 1, t1 - 1)) * KT;
-        if (!early) {
+        if (!early || kb != sp * chunk * KT) {
             id.load(a, trow, kb);
             id1.load(a, trow, kn);
             P.load(a, g, kb, id);
@@ -349,22 +369,33 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(CAttnPaged a, in
  * then do the same at the same time, than their reads took.  Maxima lag by up
  * to 2^8: raised but once or twice. */
 template <int HD, bool KV4, int NW, int NCB>
-__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAttnPaged a, int ncb, int cw, int nsplit,
-                                                                           float* __restrict__ part)
+__device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, int cw, int nsplit, int chunk, float* __restrict__ part,
+                                        uint8_t* s_raw, float (*s_ml)[16][2])
 {
     using C = CaDec<HD, KV4>;
     constexpr int KT = C::KT, NU = C::NU, NB = C::NB, NS = C::NS, NT = C::NT;
-    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * C::WAVE];
-    __shared__ float s_ml[NW][16][2];
     /* key head fastest, then columns, which read the same keys; the last ones, which may see most, first */
-    const int n_kv = a.c.n_kv, g = blockIdx.x % n_kv, units = a.rows / a.ntok;
-    const int cb = ncb - 1 - blockIdx.x / n_kv % ncb, rest = blockIdx.x / n_kv / ncb, unit = rest % units, sp = rest / units;
+    const int n_kv = a.c.n_kv, g = blk % n_kv, units = a.rows / a.ntok;
+    const int cb = ncb - 1 - blk / n_kv % ncb, rest = blk / n_kv / ncb, unit = rest % units, sp = rest / units;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kg = wave / cw, nkg = NW / cw, cwave = wave - kg * cw;
     const int col = lane & 15, c = lane >> 4;
     const int ncol = a.ntok * a.nrep, idx0 = ((cb * cw + cwave) * NCB) * 16 + col;
     int klo, khi;
     a.range(unit, &klo, &khi);
+    /* the first tile's entries and rows on their way before the positions are, where it is known (see ca_dec) */
+    CaEntries id, id1, id2;   /* of the present tile, the next and the one after */
+    CaRows<HD, KV4> K, V;
+    const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
+    int ahead = -1;
+    if (a.window <= 0 && kg < nkg) {
+        ahead = (klo / KT + sp * chunk + kg) * KT;
+        if (ahead > a.max_pos) ahead = -1;
+    }
+    if (ahead >= 0) {
+        id.load(a, trow, ahead);
+        id1.load(a, trow, ahead + nkg * KT);
+    }
     int p[NCB];
     v4f x[NCB][2 * NS];
     float big[NCB];
@@ -381,6 +412,10 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAt
             x[n][2 * s] = in ? *(const v4f*)(q + d) : (v4f){};
             x[n][2 * s + 1] = in ? *(const v4f*)(q + d + 4) : (v4f){};
         }
+    }
+    if (ahead >= 0) {
+        K.load(a, a.c.k, g, ahead, id, col, c);
+        V.load(a, a.c.v, g, ahead, id, col, c);
     }
     int pmin = INT32_MAX, pmax = -1;   /* of the wave's columns */
 #pragma unroll
@@ -408,19 +443,18 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAt
     }
     const CaTiles tiles(a, pmin, pmax, KT, klo, khi);
     int t0, t1;
-    tiles.chunk(sp, nsplit, 0, &t0, &t1);
+    tiles.chunk(sp, nsplit, chunk, &t0, &t1);
     if (kg >= nkg) t1 = t0;   /* (a wave too many) */
     if (t0 + kg < t1) {       /* (the wave's) */
         _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
-        const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
         int it = t0 + kg, kb = tiles.at(it) * KT;
-        CaEntries id, id1, id2;   /* of the present tile, the next and the one after */
-        CaRows<HD, KV4> K, V;
         auto ids_of = [&](int i, CaEntries& to) __attribute__((always_inline)) { to.load(a, trow, tiles.at(min(i, t1 - 1)) * KT); };
-        ids_of(it, id);
-        ids_of(it + nkg, id1);
-        K.load(a, a.c.k, g, kb, id, col, c);
-        V.load(a, a.c.v, g, kb, id, col, c);
+        if (kb != ahead) {
+            ids_of(it, id);
+            ids_of(it + nkg, id1);
+            K.load(a, a.c.k, g, kb, id, col, c);
+            V.load(a, a.c.v, g, kb, id, col, c);
+        }
         v8h qh[NCB][NS], ql[NCB][NS];
         int ex[NCB];
 #pragma unroll
@@ -471,25 +505,6 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAt
                         for (int i = 0; i < 4; i++) s[u][n][i] = seen(kb + 16 * u + 4 * c + i, kb, none) ? s[u][n][i] : -INFINITY;
                 }
             }
-#pragma unroll
-            for (int n = 0; n < NCB; n++) {
-                float mn = s[0][n][0];
-#pragma unroll
-                for (int u = 0; u < NU; u++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) mn = fmaxf(mn, s[u][n][i]);
-                if (mx[n].due(mn)) {
-                    mn = fmaxf(mn, lg_partner<4>(mn));
-                    mn = fmaxf(mn, lg_partner<5>(mn));
-                    float off;
-                    const float al = mx[n].raise(mn, &off);
-                    l[n] *= al;
-#pragma unroll
-                    for (int t = 0; t < NT; t++) o[n][t] *= al;
-#pragma unroll
-                    for (int u = 0; u < NU; u++) s[u][n] -= off;
-                }
-            }
             uint64_t bad = 0;   /* keys of the tile */
 #pragma unroll
             for (int b = 0; b < NB; b++) {
@@ -504,17 +519,38 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAt
                 if (b == NB - 1 && kn >= 0) V.load(a, a.c.v, g, kn, id1, col, c);
                 v8h ph[NCB], pl[NCB];
 #pragma unroll
-                for (int n = 0; n < NCB; n++)
+                for (int n = 0; n < NCB; n++) {
+                    /* the weights; whether one outgrew its maximum, their sum tells */
+                    v4f &s0 = s[2 * b][n], &s1 = s[2 * b + 1][n];
+                    float w[8], sum;
+                    auto weigh = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        float w[4];
+                        for (int i = 0; i < 4; i++) {
+                            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s0[i], mx[n].sc, mx[n].cc));
+                            w[4 + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[i], mx[n].sc, mx[n].cc));
+                        }
+                        sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                    };
+                    weigh();
+                    if (mx[n].over(sum)) {
+                        float mn = fmaxf(s0[0], s1[0]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * b + u][n][i], mx[n].sc, mx[n].cc));
-                        l[n] += (w[0] + w[1]) + (w[2] + w[3]);
-                        ca_split2(w[0], w[1], ph[n], pl[n], 4 * u);
-                        ca_split2(w[2], w[3], ph[n], pl[n], 4 * u + 2);
+                        for (int i = 1; i < 4; i++) mn = fmaxf(mn, fmaxf(s0[i], s1[i]));
+                        mn = fmaxf(mn, lg_partner<4>(mn));
+                        mn = fmaxf(mn, lg_partner<5>(mn));
+                        float off;
+                        const float al = mx[n].raise(mn, &off);
+                        l[n] *= al;
+#pragma unroll
+                        for (int t = 0; t < NT; t++) o[n][t] *= al;
+                        s0 -= off;
+                        s1 -= off;
+                        weigh();
                     }
+                    l[n] += sum;
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) ca_split2(w[i], w[i + 1], ph[n], pl[n], i);
+                }
                 ca_wave_sync();
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
@@ -605,63 +641,86 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(CAt
     }
 }
 
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(PaArgs args)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * CaDec<HD, KV4>::WAVE];
+    __shared__ float s_ml[NW][16][2];
+    const PaPhase& f = args.of(blockIdx.x);
+    pa_cols<HD, KV4, NW, 2>(f.a, args.in(blockIdx.x), f.ncb, f.cw, f.nsplit, f.chunk, args.part, s_raw, s_ml);
+}
+
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_dec(PaArgs args)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * CaDec<HD, KV4>::WAVE];
+    __shared__ float s_ml[NW][16][2];
+    const PaPhase& f = args.of(blockIdx.x);
+    ca_dec<HD, KV4, NW>(f.a, args.in(blockIdx.x), f.nsplit, f.chunk, args.part, s_raw, s_ml);
+}
+
+/* shared rows by the one, own rows by the other */
+template <int HD, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols_dec(PaArgs args)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * CaDec<HD, KV4>::WAVE];
+    __shared__ float s_ml[NW][16][2];
+    const PaPhase& f = args.of(blockIdx.x);
+    if ((int)blockIdx.x < args.na)
+        pa_cols<HD, KV4, NW, 2>(f.a, blockIdx.x, f.ncb, f.cw, f.nsplit, f.chunk, args.part, s_raw, s_ml);
+    else ca_dec<HD, KV4, NW>(f.a, blockIdx.x - args.na, f.nsplit, f.chunk, args.part, s_raw, s_ml);
+}
+
 /* How a phase is cut. */
 struct PaCut {
-    bool dec;            /* up to 16 columns a key head: k_cattn_dec, as over contiguous caches */
-    bool wide;           /* eight waves a workgroup, else four */
-    bool tile;
-    int cw, ncb;         /* else: waves with columns of their own, blocks of their columns */
+    int kind;
+    int cw, ncb;         /* waves with columns of their own; blocks of columns */
     int nsplit, chunk;   /* parts of the keys, tiles in a part */
+    int64_t blocks;
 };
 
-static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos, bool kv4)
+/* Four waves a workgroup, or eight: of phases that share a launch the same. */
+static int pa_dec_waves(int hd) { return hd <= 128 ? 8 : 4; }
+
+static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos, bool kv4, bool lone)
 {
     const int64_t cols = ntok * (n_heads / n_kv);
     PaCut p = {};
-    if (cols <= 16) {
-        const CaPlan d = lg_ca_plan(units, ntok, n_heads, n_kv, hd, window, sinks, max_pos, kv4);
-        p.dec = true;
-        p.wide = d.wide;
-        p.nsplit = d.nsplit;
-        p.chunk = d.chunk;
-        return p;
-    }
-    p.wide = hd <= 128;
-    const int nw = p.wide ? 8 : 4, kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec::KT) */
-    const int64_t nb = (cols + 31) / 32;
-    if (hd <= 128 && cols > 64) {
-        p.tile = true;
-        const int kt = 128, PT_NW = hd <= 64 ? 16 : 12, PT_SLOTS = 256;   /* (PaTile::KT) */
-        p.ncb = (int)((cols + 16 * PT_NW - 1) / (16 * PT_NW));
-        int64_t keys = (int64_t)max_pos + 1;
-        if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
-        const double tiles = (double)((keys + kt - 1) / kt);
-        const int64_t wgs = units * n_kv * p.ncb;
-        double best = 0.0;
-        for (int ns = 1; ns <= 64 && (ns == 1 || tiles / ns >= 1.5); ns++) {
-            const double cost = (double)((wgs * ns + PT_SLOTS - 1) / PT_SLOTS) * (2.5 + tiles / ns) + (ns > 1 ? 1.0 + 0.5e-6 * ns * (double)(units * ntok) * n_heads * hd : 0.0);
-            if (ns == 1 || cost < best) {
-                best = cost;
-                p.nsplit = ns;
-            }
-        }
-        p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
-        return p;
-    }
-    for (p.cw = nw; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
-    p.ncb = (int)((nb + p.cw - 1) / p.cw);
     int64_t keys = (int64_t)max_pos + 1;
     if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
-    const double tiles = (double)((keys + kt - 1) / kt) / (nw / p.cw);   /* of a wave */
+    const int nw = pa_dec_waves(hd);
+    int kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec::KT) */
+    p.cw = p.ncb = 1;
+    double slots = 256.0, start = 6.0, join = 1.5e-6;
+    int64_t wide = nw;   /* tiles that a workgroup has at a time */
+    if (cols <= 16) p.kind = PA_DEC;
+    else if (hd <= 128 && cols > 64) {
+        p.kind = PA_TILE;
+        p.ncb = (int)((cols + 16 * pa_waves(hd) - 1) / (16 * pa_waves(hd)));
+        kt = 128;   /* (PaTile::KT) */
+        wide = 1;
+        start = 1.5;
+        join = 0.3e-6;
+    } else {
+        p.kind = PA_COLS;
+        const int64_t nb = (cols + 31) / 32;
+        for (p.cw = nw; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
+        p.ncb = (int)((nb + p.cw - 1) / p.cw);
+        wide = nw / p.cw;
+    }
+    const double tiles = std::max(1.0, (double)((keys + kt - 1) / kt) / (double)wide);   /* one after the other */
     const int64_t wgs = units * n_kv * p.ncb;
     double best = 0.0;
     for (int ns = 1; ns <= CA_PARTS && (ns == 1 || tiles / ns >= 1.0); ns++) {
-        const double cost = (double)((wgs * ns + 255) / 256) * (6.0 + tiles / ns) + (ns > 1 ? 2.0 + 1.5e-6 * ns * (double)(units * ntok) * n_heads * hd : 0.0);
+        const double rounds = ceil((double)(wgs * ns) / slots);
+        const double cost = rounds * (start + tiles / ns) + (lone && ns > 1 ? 2.0 : 0.0) + (ns > 1 ? join * ns * (double)(units * ntok) * n_heads * hd : 0.0);
         if (ns == 1 || cost < best) {
             best = cost;
             p.nsplit = ns;
         }
     }
+    p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
+    p.blocks = wgs * p.nsplit;
     return p;
 }
 
@@ -679,46 +738,41 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
 {
     PaPlan p = {};
     p.shared = group > 1 && max_prefix > 0;
-    if (p.shared) p.a = pa_cut(nseq / group, ntok * group, n_heads, n_kv, hd, window, sinks, std::min(max_prefix - 1, max_pos), kv4);
+    if (p.shared) p.a = pa_cut(nseq / group, ntok * group, n_heads, n_kv, hd, window, sinks, std::min(max_prefix - 1, max_pos), kv4, false);
     /* (the own rows' number lies in device memory: of the longest prompt's) */
-    p.b = pa_cut(nseq, ntok, n_heads, n_kv, hd, window, sinks, p.shared ? std::max(max_pos - max_prefix, 0) : max_pos, kv4);
+    p.b = pa_cut(nseq, ntok, n_heads, n_kv, hd, window, sinks, p.shared ? std::max(max_pos - max_prefix, 0) : max_pos, kv4, !p.shared);
     p.parts = p.b.nsplit + (p.shared ? p.a.nsplit : 0);
     if (p.parts > 1) p.ws = (size_t)p.parts * nseq * ntok * n_heads * (hd + 2) * sizeof(float);
     return p;
 }
 
 template <int HD, bool KV4>
-static void pa_launch(const CAttnPaged& a, const PaCut& p, int units, float* part, hipStream_t s)
+static void pa_launch(const PaArgs& x, int64_t nb, hipStream_t s)
 {
-    const int64_t n = (int64_t)units * a.c.n_kv * p.nsplit;
-    if constexpr (HD <= 128)
-        if (p.wide) {
-            if (p.dec) k_cattn_dec<HD, KV4, 8, CAttnPaged><<<(unsigned)n, 512, 0, s>>>(a, p.nsplit, p.chunk, part);
-            else if (p.tile) k_pattn_tile<HD, KV4, PT_NW_OF<HD>><<<(unsigned)(n * p.ncb), 64 * PT_NW_OF<HD>, 0, s>>>(a, p.ncb, p.nsplit, p.chunk, part);
-            else k_pattn_cols<HD, KV4, 8, 2><<<(unsigned)(n * p.ncb), 512, 0, s>>>(a, p.ncb, p.cw, p.nsplit, part);
-            return;
-        }
-    if (p.dec) k_cattn_dec<HD, KV4, 4, CAttnPaged><<<(unsigned)n, 256, 0, s>>>(a, p.nsplit, p.chunk, part);
-    else k_pattn_cols<HD, KV4, 4, 2><<<(unsigned)(n * p.ncb), 256, 0, s>>>(a, p.ncb, p.cw, p.nsplit, part);
+    constexpr int NW = HD <= 128 ? 8 : 4;   /* (pa_dec_waves) */
+    const int ka = x.na ? x.f[0].kind : x.f[1].kind, kb = x.f[1].kind;
+    const unsigned n = (unsigned)(x.na + nb);
+    auto one = [&](const PaArgs& y, int kind, unsigned blocks) {
+        if (kind == PA_DEC) k_pattn_dec<HD, KV4, NW><<<blocks, 64 * NW, 0, s>>>(y);
+        else if (kind == PA_COLS) k_pattn_cols<HD, KV4, NW><<<blocks, 64 * NW, 0, s>>>(y);
+        else if constexpr (HD <= 128) k_pattn_tile<HD, KV4, pa_waves(HD)><<<blocks, 64 * pa_waves(HD), 0, s>>>(y);
+    };
+    if (ka == kb) one(x, ka, n);
+    else if (ka == PA_COLS && kb == PA_DEC) k_pattn_cols_dec<HD, KV4, NW><<<n, 64 * NW, 0, s>>>(x);
+    else {
+        one(x, ka, (unsigned)x.na);
+        PaArgs y = x;
+        y.na = 0;
+        one(y, kb, (unsigned)nb);
+    }
 }
 
 template <int HD>
-static void pa_type(const CAttnPaged& a, const PaCut& p, int units, float* part, hipStream_t s)
+static void pa_type(const PaArgs& x, int64_t nb, hipStream_t s)
 {
     if constexpr (HD != 48)
-        if (a.c.type == LG_KV4) return pa_launch<HD, true>(a, p, units, part, s);
-    pa_launch<HD, false>(a, p, units, part, s);
-}
-
-static void pa_phase(const CAttnPaged& a, const PaCut& p, int units, float* part, hipStream_t s)
-{
-    switch (a.c.hd) {
-    case 48: pa_type<48>(a, p, units, part, s); break;
-    case 64: pa_type<64>(a, p, units, part, s); break;
-    case 96: pa_type<96>(a, p, units, part, s); break;
-    case 128: pa_type<128>(a, p, units, part, s); break;
-    default: pa_type<256>(a, p, units, part, s); break;
-    }
+        if (x.f[1].a.c.type == LG_KV4) return pa_launch<HD, true>(x, nb, s);
+    pa_launch<HD, false>(x, nb, s);
 }
 
 static bool pa_head_dim(int hd, int type)
@@ -796,11 +850,10 @@ extern "C" int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages
     a.max_prefix = max_prefix;
     a.prefix = p.shared ? prefix : nullptr;
     a.nparts = p.parts;
-    const int64_t na = p.shared ? (int64_t)(nseq / group) * a.c.n_kv * p.a.nsplit * (p.a.dec ? 1 : p.a.ncb) : 0;
-    const int64_t nb = (int64_t)nseq * a.c.n_kv * p.b.nsplit * (p.b.dec ? 1 : p.b.ncb);
+    const int64_t na = p.shared ? p.a.blocks : 0, nb = p.b.blocks;
     const bool by_group = p.parts > 8 || rows * n_heads <= 4096;   /* (as lg_attn_cache) */
     const int64_t joins = p.ws ? by_group ? rows * n_heads : (rows * n_heads * (hd / 4) + 255) / 256 : 0;
-    if (!lg_grid_fits(na, 512) || !lg_grid_fits(nb, 512) || !lg_grid_fits(joins, 256)) {
+    if (!lg_grid_fits(na + nb, 1024) || !lg_grid_fits(joins, 256)) {
         lg_set_error("%s: %lld rows of %d heads are too many for one call", who, (long long)rows, n_heads);
         return LG_ERR_ARG;
     }
@@ -810,17 +863,29 @@ extern "C" int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages
     }
     hipStream_t s = (hipStream_t)stream;
     float* const part = p.ws ? (float*)workspace : nullptr;
+    auto phase = [&](const PaCut& c, int units_of, int part0) {
+        PaPhase f = {a, c.kind, c.ncb, c.cw, c.nsplit, c.chunk};
+        f.a.ntok = ntok * units_of;
+        f.a.tstep = units_of;
+        f.a.part0 = part0;
+        return f;
+    };
+    PaArgs x = {};
+    x.na = (int)na;
+    x.part = part;
     if (p.shared) {
-        a.ntok = ntok * group;
-        a.tstep = group;
-        a.share = 1;
-        pa_phase(a, p.a, nseq / group, part, s);
-        a.part0 = p.a.nsplit;
+        x.f[0] = phase(p.a, group, 0);
+        x.f[0].a.share = 1;
+    }
+    x.f[1] = phase(p.b, 1, p.shared ? p.a.nsplit : 0);
+    switch (hd) {
+    case 48: pa_type<48>(x, nb, s); break;
+    case 64: pa_type<64>(x, nb, s); break;
+    case 96: pa_type<96>(x, nb, s); break;
+    case 128: pa_type<128>(x, nb, s); break;
+    default: pa_type<256>(x, nb, s); break;
     }
     a.ntok = ntok;
-    a.tstep = 1;
-    a.share = 0;
-    pa_phase(a, p.b, nseq, part, s);
     if (part) {
         if (by_group) k_cattn_merge_wide<CAttnPaged><<<(unsigned)joins, 256, 0, s>>>(a, p.parts, part);
         else k_cattn_merge<CAttnPaged><<<(unsigned)joins, 256, 0, s>>>(a, p.parts, part);
