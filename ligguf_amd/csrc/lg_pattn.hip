@@ -18,7 +18,26 @@ struct PaArgs {
     __device__ __forceinline__ int in(int blk) const { return blk < na ? blk : blk - na; }
 };
 
+constexpr int PA_WAVES = 4;                                      /* of the other kernels' */
 constexpr int pa_waves(int hd) { return hd <= 64 ? 16 : 12; }   /* of k_pattn_tile's workgroups */
+
+/* ca_query2 in 11 operations for two values, not 19: lo is 0 only where hi is, which
+ * is rounded to 0 below 2^-37 of the row's largest value (there an infinite key's
+ * score is NaN, as at a query's 0). */
+__device__ __forceinline__ void pa_query2(float x0, float x1, int ex, v8h& hi, v8h& lo, int i)
+{
+    typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+    const u2 sign = {0x8000, 0x8000}, least = {1, 1};
+    const float y0 = ldexpf(x0, 14 - ex), y1 = ldexpf(x1, 14 - ex);
+    const lg_h2 h = __builtin_bit_cast(lg_h2, __builtin_amdgcn_cvt_pkrtz(y0, y1));
+    const lg_h2 l = __builtin_convertvector(((lg_f2){__builtin_fmaf(-(float)h[0], 1.0f, y0), __builtin_fmaf(-(float)h[1], 1.0f, y1)}), lg_h2);
+    const u2 hb = __builtin_bit_cast(u2, h), lb = __builtin_bit_cast(u2, l), ha = hb & ~sign;
+    const lg_h2 b = __builtin_bit_cast(lg_h2, __builtin_elementwise_max(lb & ~sign, __builtin_elementwise_min(ha, least)) | (hb & sign));
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = b[0];
+    lo[i + 1] = b[1];
+}
 
 /* Many columns: 16 a wave, NW waves a workgroup, which share tiles of KT keys in
  * LDS; the products of k_cattn_dec, SB keys at a time:
@@ -234,7 +253,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
 #pragma unroll
         for (int j = 0; j < NS; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) ca_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
+            for (int e = 0; e < 8; e += 2) pa_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
         }
         P.store(s_kv, some(kb, none) ? s_bad[0] : nullptr);
         __syncthreads();
@@ -470,7 +489,7 @@ __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, i
             for (int j = 0; j < NS; j++)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2)
-                    ca_query2(x[n][2 * j + e / 4][e % 4], x[n][2 * j + e / 4][e % 4 + 1], ex[n], qh[n][j], ql[n][j], e);
+                    pa_query2(x[n][2 * j + e / 4][e % 4], x[n][2 * j + e / 4][e % 4 + 1], ex[n], qh[n][j], ql[n][j], e);
         }
         CaMaxOf<7, 8> mx[NCB] = {CaMaxOf<7, 8>(ca_scale(a.scale2, ex[0])), CaMaxOf<7, 8>(ca_scale(a.scale2, ex[NCB - 1]))};
         for (; it < t1; it += nkg) {
@@ -679,25 +698,23 @@ struct PaCut {
     int64_t blocks;
 };
 
-/* Four waves a workgroup, or eight: of phases that share a launch the same. */
-static int pa_dec_waves(int hd) { return hd <= 128 ? 8 : 4; }
-
 static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos, bool kv4, bool lone)
 {
     const int64_t cols = ntok * (n_heads / n_kv);
     PaCut p = {};
     int64_t keys = (int64_t)max_pos + 1;
     if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
-    const int nw = pa_dec_waves(hd);
+    const int nw = PA_WAVES;
     int kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec::KT) */
     p.cw = p.ncb = 1;
-    double slots = 256.0, start = 6.0, join = 1.5e-6;
+    double slots = hd <= 128 ? 512.0 : 256.0, start = 3.0, join = 1.5e-6;
     int64_t wide = nw;   /* tiles that a workgroup has at a time */
     if (cols <= 16) p.kind = PA_DEC;
     else if (hd <= 128 && cols > 64) {
         p.kind = PA_TILE;
         p.ncb = (int)((cols + 16 * pa_waves(hd) - 1) / (16 * pa_waves(hd)));
         kt = 128;   /* (PaTile::KT) */
+        slots = 256.0;
         wide = 1;
         start = 1.5;
         join = 0.3e-6;
@@ -749,7 +766,7 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
 template <int HD, bool KV4>
 static void pa_launch(const PaArgs& x, int64_t nb, hipStream_t s)
 {
-    constexpr int NW = HD <= 128 ? 8 : 4;   /* (pa_dec_waves) */
+    constexpr int NW = PA_WAVES;
     const int ka = x.na ? x.f[0].kind : x.f[1].kind, kb = x.f[1].kind;
     const unsigned n = (unsigned)(x.na + nb);
     auto one = [&](const PaArgs& y, int kind, unsigned blocks) {
