@@ -792,6 +792,9 @@ static void pa_type(const PaArgs& x, int64_t nb, hipStream_t s)
     pa_launch<HD, false>(x, nb, s);
 }
 
+/* a window of all positions is none (and differences of positions and windows fit 32 bits) */
+static int pa_window(int window, int max_pos) { return window > max_pos ? 0 : window; }
+
 static bool pa_head_dim(int hd, int type)
 {
     return hd == 64 || hd == 96 || hd == 128 || hd == 256 || (hd == 48 && type == LG_F16);
@@ -803,8 +806,8 @@ extern "C" size_t lg_attn_paged_workspace_size(const lg_kv_pages* cache, int nse
     if (!cache || cache->pool.n_kv_heads <= 0 || cache->pool.head_dim <= 0 || nseq <= 0 || ntok <= 0 || n_heads <= 0 ||
         window < 0 || sinks < 0 || max_pos < 0 || group <= 0 || nseq % group || max_prefix < 0)
         return 0;
-    return pa_plan(nseq, ntok, n_heads, cache->pool.n_kv_heads, cache->pool.head_dim, window, sinks, max_pos,
-                   cache->pool.type == LG_KV4, group, max_prefix).ws;
+    return pa_plan(nseq, ntok, n_heads, cache->pool.n_kv_heads, cache->pool.head_dim, pa_window(window, max_pos), sinks, max_pos,
+                   cache->pool.type == LG_KV4, group, std::min(max_prefix, max_pos + 1)).ws;
 }
 
 extern "C" int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages* cache, const int* pos, int nseq, int ntok,
@@ -836,6 +839,8 @@ extern "C" int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages
         lg_set_error("%s: groups of %d of %d sequences, %d rows shared", who, group, nseq, max_prefix);
         return LG_ERR_ARG;
     }
+    window = pa_window(window, max_pos);
+    max_prefix = std::min(max_prefix, max_pos + 1);   /* (rows behind are not seen) */
     const int64_t rows = (int64_t)nseq * ntok, width = (int64_t)n_heads * hd;
     if (!rows) return LG_OK;
     if (!pos || !q || !out || !lg_al16(q) || !lg_al16(out) || q_stride % 4 || out_stride % 4 || q_stride < width ||
