@@ -299,9 +299,8 @@ extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* 
     const int64_t rows = (int64_t)ngroups * beams;
     BeamArgs a = {logits, scores, done, stride, end, beams, vocab, top, bm_parts(rows, beams, vocab, top), 0, nullptr, nullptr,
                   score, parent, token};
-    /* (parts begin 16 bytes apart, so that all are as aligned as the row) */
+    /* (parts begin 16 bytes apart, so that all are as aligned as the row; up to 512 of 4096 at least: none is empty) */
     a.part = (vocab / a.parts + 4) & ~3;
-    if ((int64_t)a.part * (a.parts - 1) >= vocab) a.part = (vocab + a.parts - 1) / a.parts;
     if (!lg_grid_fits(rows * a.parts, 1024)) {
         lg_set_error("%s: %lld rows are too many for one call", who, (long long)rows);
         return LG_ERR_ARG;
@@ -382,12 +381,14 @@ __global__ __launch_bounds__(256) void k_beam_tables(ReorderArgs a)
     }
 }
 
-constexpr int BM_POOLS = 64;   /* layers a launch */
+constexpr int BM_POOLS = 64;         /* layers a launch */
+constexpr int BM_SLICE = 65536;      /* bytes that a workgroup moves at most (or 16 rows) */
 
 struct CopyArgs {
     uint8_t* pool[BM_POOLS][2];
     const int4* jobs;
     LgKv c;
+    int slice;   /* rows a workgroup */
 };
 
 /* rows of a page: [rows][n_kv][hd] fp16 are one run, 4-bit ones a run of codes and
@@ -395,8 +396,9 @@ struct CopyArgs {
 __global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a)
 {
     const int4 j = a.jobs[blockIdx.x];
-    if (!j.z) return;
-    uint8_t* const p = a.pool[blockIdx.y][blockIdx.z];
+    const int r0 = blockIdx.z / 2 * a.slice, n = min(j.z - r0, a.slice);
+    if (n <= 0) return;
+    uint8_t* const p = a.pool[blockIdx.y][blockIdx.z % 2];
     const uint8_t* const src = p + (size_t)j.x * a.c.seq;
     uint8_t* const dst = p + (size_t)j.y * a.c.seq;
     auto run = [&](size_t at, int bytes) {   /* multiples of 4 from 16-byte addresses on */
@@ -415,11 +417,11 @@ __global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a)
         i = 4 * n + threadIdx.x;
         if (i < bytes / 4) ((uint32_t*)y)[i] = ((const uint32_t*)x)[i];
     };
-    if (a.c.type == LG_F16) run(0, j.z * a.c.n_kv * a.c.hd * 2);
+    if (a.c.type == LG_F16) run(lg_kv16_at(a.c, 0, r0), n * a.c.n_kv * a.c.hd * 2);
     else
         for (int g = 0; g < a.c.n_kv; g++) {
-            run(lg_kv4_codes(a.c, g, 0), j.z * (a.c.hd / 2));
-            run(lg_kv4_dm(a.c, g, 0), j.z * (a.c.hd / 8));
+            run(lg_kv4_codes(a.c, g, r0), n * (a.c.hd / 2));
+            run(lg_kv4_dm(a.c, g, r0), n * (a.c.hd / 8));
         }
 }
 
@@ -469,13 +471,16 @@ extern "C" int lg_beam_reorder(const lg_kv_cache* pools, int n_pools, int n_page
     hipStream_t s = (hipStream_t)stream;
     k_beam_tables<<<ngroups, 256, 0, s>>>(r);
     c.jobs = r.jobs;
+    const int64_t row = (int64_t)c.c.n_kv * (c.c.type == LG_F16 ? 2 * c.c.hd : c.c.hd / 2 + c.c.hd / 8);
+    c.slice = (int)std::min<int64_t>(std::max<int64_t>((BM_SLICE / row) & ~15, 16), c.c.n_ctx);
+    const unsigned slices = (c.c.n_ctx + c.slice - 1) / c.slice;
     for (int l = 0; l < n_pools; l += BM_POOLS) {
         const int n = std::min(BM_POOLS, n_pools - l);
         for (int i = 0; i < n; i++) {
             c.pool[i][0] = (uint8_t*)pools[l + i].k;
             c.pool[i][1] = (uint8_t*)pools[l + i].v;
         }
-        k_beam_copy<<<dim3((unsigned)nseq, n, 2), 256, 0, s>>>(c);
+        k_beam_copy<<<dim3((unsigned)nseq, n, 2 * slices), 256, 0, s>>>(c);
     }
     return lg_check_launch(who);
 }
