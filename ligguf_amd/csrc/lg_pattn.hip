@@ -742,7 +742,8 @@ static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, 
     const double tiles = std::max(1.0, (double)((keys + kt - 1) / kt) / (double)wide);   /* one after the other */
     const int64_t wgs = units * n_kv * p.ncb;
     double best = 0.0;
-    for (int ns = 1; ns <= CA_PARTS && (ns == 1 || tiles / ns >= 1.0); ns++) {
+    /* (those of both phases together: CA_PARTS at most) */
+    for (int ns = 1; ns <= (lone ? CA_PARTS : CA_PARTS / 2) && (ns == 1 || tiles / ns >= 1.0); ns++) {
         const double rounds = ceil((double)(wgs * ns) / slots);
         const double cost = rounds * (start + tiles / ns) + (lone && ns > 1 ? 2.0 : 0.0) + (ns > 1 ? join * ns * (double)(units * ntok) * n_heads * hd : 0.0);
         if (ns == 1 || cost < best) {

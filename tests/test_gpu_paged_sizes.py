@@ -241,3 +241,11 @@ def test_two_captured_calls_and_eager_ones(gpu):
             calls[i](eager)
             torch.cuda.synchronize()
             assert torch.equal(outs[i], want[i]) and torch.equal(eager, want[i]), (turn, i)
+
+
+@pytest.mark.parametrize("ctype", TYPES)
+@pytest.mark.parametrize("heads", [1, 6])
+def test_one_key_head_in_as_many_parts_as_there_are(gpu, ctype, heads):
+    """A single key head over long contexts: shared and own rows each in hundreds of parts."""
+    check(gpu, ctype, heads, 1, 64, 64, 1, 2, [50000], [90000, 70001], 1)
+    check(gpu, ctype, heads, 1, 64, 64, 1, 1, [0], [100000], 1)

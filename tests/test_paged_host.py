@@ -47,6 +47,19 @@ def test_attention_refusals(kw):
     assert attn(**kw) == -1 and L.load().lg_last_error(None)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kv,heads", [(1, 1), (1, 8), (2, 4), (8, 32)])
+def test_parts_of_long_contexts(kv, heads, hd):
+    """The join takes 512 parts at most, however many keys are shared and own."""
+    need = L.load().lg_attn_paged_workspace_size
+    c = pages(page=1 << 15, kv=kv, hd=hd, most=1 << 10)
+    for members in (1, 2, 3, 16):
+        for last in (1000, 50000, 90000, 10 ** 6, (1 << 25) - 1):
+            for prefix in (0, last // 3, last // 2, last):
+                n = need(C.byref(c), members, 1, heads, 0, 0, last, members, prefix)
+                assert n % (members * heads * (hd + 2) * 4) == 0 and n // (members * heads * (hd + 2) * 4) <= 512, (members, last, prefix)
+
+
 def test_attention_workspace():
     need = L.load().lg_attn_paged_workspace_size
     c = pages(most=1000)
