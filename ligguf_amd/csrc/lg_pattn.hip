@@ -710,34 +710,37 @@ struct PaCut {
     int cw, ncb;         /* waves with columns of their own; blocks of columns */
     int nsplit, chunk;   /* parts of the keys, tiles in a part */
     int64_t blocks;
+    double us;           /* about */
 };
 
-static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int window, int sinks, int max_pos, bool kv4, bool lone)
+/* units of ntok rows each over `keys` keys by one kind of kernel.  Its time is counted in tiles: rounds of workgroups,
+ * as many as fit the chip at once, each of a start worth some tiles and the tiles of its part; parts are written and
+ * read once.  More of them fill the chip, until their starts and the join cost more: 192 columns over 20000 keys
+ * in 14 parts 97 us, in 32 (all CUs) 70; 24 columns of nine groups over up to 5000 keys in 2 parts 55 us, 4 41,
+ * 7 (taken) 45, 14 58; 50 blocks of columns over 2900 keys in 1 part 104 us, 2 104, 3 114, 5 133. */
+static PaCut pa_cut(int kind, int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int64_t keys, bool kv4, bool lone)
 {
     const int64_t cols = ntok * (n_heads / n_kv);
-    PaCut p = {};
-    int64_t keys = (int64_t)max_pos + 1;
-    if (window > 0) keys = std::min(keys, (int64_t)window + sinks + ntok - 1);
-    const int nw = PA_WAVES;
+    PaCut p = {kind};
     int kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec::KT) */
     p.cw = p.ncb = 1;
-    double slots = hd <= 128 ? 512.0 : 256.0, start = 3.0, join = 1.5e-6;
-    int64_t wide = nw;   /* tiles that a workgroup has at a time */
-    if (cols <= 16) p.kind = PA_DEC;
-    else if (hd <= 128 && cols > 64) {
-        p.kind = PA_TILE;
-        p.ncb = (int)((cols + 16 * pa_waves(hd) - 1) / (16 * pa_waves(hd)));
+    double slots = hd <= 128 ? 512.0 : 256.0, start = 3.0, join = 1.5e-6, tile_us = (0.3 + 0.0164 * hd) * (kv4 ? 0.8 : 1.0);
+    int64_t wide = PA_WAVES;   /* tiles that a workgroup has at a time */
+    if (kind == PA_TILE) {
+        const int64_t width = 16 * pa_waves(hd);
+        p.ncb = (int)((cols + width - 1) / width);
         kt = 128;   /* (PaTile::KT) */
         slots = 256.0;
         wide = 1;
         start = 1.5;
         join = 0.3e-6;
-    } else {
-        p.kind = PA_COLS;
+        /* (waves without columns leave the others more of their SIMD) */
+        tile_us = (1.0 + 0.0234 * hd) * (0.2 + 0.8 * (double)cols / (double)(p.ncb * width));
+    } else if (kind == PA_COLS) {
         const int64_t nb = (cols + 31) / 32;
-        for (p.cw = nw; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
+        for (p.cw = PA_WAVES; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
         p.ncb = (int)((nb + p.cw - 1) / p.cw);
-        wide = nw / p.cw;
+        wide = PA_WAVES / p.cw;
     }
     const double tiles = std::max(1.0, (double)((keys + kt - 1) / kt) / (double)wide);   /* one after the other */
     const int64_t wgs = units * n_kv * p.ncb;
@@ -753,6 +756,7 @@ static PaCut pa_cut(int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, 
     }
     p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
     p.blocks = wgs * p.nsplit;
+    p.us = best * tile_us;
     return p;
 }
 
@@ -770,9 +774,38 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
 {
     PaPlan p = {};
     p.shared = group > 1 && max_prefix > 0;
-    if (p.shared) p.a = pa_cut(nseq / group, ntok * group, n_heads, n_kv, hd, window, sinks, std::min(max_prefix - 1, max_pos), kv4, false);
-    /* (the own rows' number lies in device memory: of the longest prompt's) */
-    p.b = pa_cut(nseq, ntok, n_heads, n_kv, hd, window, sinks, p.shared ? std::max(max_pos - max_prefix, 0) : max_pos, kv4, !p.shared);
+    auto cut = [&](int kind, bool shared, int top) {
+        const int64_t n = shared ? ntok * group : ntok;
+        int64_t keys = (int64_t)top + 1;
+        if (window > 0) keys = std::min(keys, (int64_t)window + sinks + n - 1);
+        return pa_cut(kind, shared ? nseq / group : nseq, n, n_heads, n_kv, hd, keys, kv4, !p.shared);
+    };
+    const int64_t rep = n_heads / n_kv, cols = ntok * rep;
+    /* Own rows (their number lies in device memory: of the longest prompt's).  Of many columns tiles in LDS: 2000 tokens
+     * of 32 heads of 128 92 us against 179, 64 18 against 20.  Not where heads of 64 fill the chip with less than a tile
+     * a workgroup: 64 tokens 15 against 13, 256 22 against 18, 512 27 and 26, 1024 39 against 47. */
+    const int top = p.shared ? std::max(max_pos - max_prefix, 0) : max_pos;
+    if (cols <= 16) p.b = cut(PA_DEC, false, top);
+    else {
+        if (hd <= 128 && cols > 64) p.b = cut(PA_TILE, false, top);
+        if (hd > 128 || cols <= 64 || (hd <= 64 && p.b.blocks * p.b.chunk < 256)) p.b = cut(PA_COLS, false, top);
+    }
+    /* Shared rows.  Tiles in LDS are a launch of their own unless the own rows have such too, which costs 13 us; the
+     * tiles' times are those with which the choice is the faster one most often (of 154 calls of both types 1 % from
+     * the best in the mean; always the one or the other 4 % and 15 %).  With single tokens' own rows, 32 heads of 128, 8 key
+     * heads: 192 columns over 700 keys 36 us against 26, over 5000 44 against 40, over 20000 61 against 80; 64 over 3000 28
+     * against 27, over 20000 37 against 44; twelve groups of 80 columns over 600 61 against 51. */
+    if (p.shared) {
+        const int last = std::min(max_prefix - 1, max_pos);
+        if (cols * group <= 16) p.a = cut(PA_DEC, true, last);
+        else {
+            p.a = cut(PA_COLS, true, last);
+            if (hd <= 128 && cols * group > 32) {
+                const PaCut t = cut(PA_TILE, true, last);
+                if (t.us + (p.b.kind == PA_TILE ? 0.0 : 13.0) < p.a.us) p.a = t;
+            }
+        }
+    }
     p.parts = p.b.nsplit + (p.shared ? p.a.nsplit : 0);
     if (p.parts > 1) p.ws = (size_t)p.parts * nseq * ntok * n_heads * (hd + 2) * sizeof(float);
     return p;
