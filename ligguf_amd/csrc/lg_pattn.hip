@@ -54,12 +54,20 @@ __device__ __forceinline__ void pa_split2(float x0, float x1, v8h& hi, v8h& lo, 
 }
 
 /* Many columns: 16 a wave, NW waves a workgroup, which share tiles of KT keys in
- * LDS; the products of k_cattn_dec, SB keys at a time:
+ * LDS; the products of k_cattn_dec, 32 keys at a time:
  *   S^T[key][col] = K Q^T      O^T[d][col] += V^T P^T
- * 16 columns rather than 32 take half the registers, so that a SIMD has four
- * waves to fill each other's waits with.  The next tile's rows are on their way
- * while one computes (two LDS stages, one barrier a tile), its table entries
- * while the one before does.  Maxima lag by up to 2^8: raised but once or twice. */
+ * 16 columns take so few registers that a SIMD has three or four waves to fill
+ * each other's waits with.  More columns a wave read LDS less often, and are
+ * slower for want of waves: 192 columns over 20000 keys in 12 waves of 16 70 us
+ * in all, 8 of 32 82, 4 of 48 94; heads of 64, ten prompts, 16 waves of 16 104,
+ * 8 of 32 119, 4 of 64 175.  The next tile's rows are on their way while one
+ * computes (two LDS stages, one barrier a tile), its table entries while the one
+ * before does.  Maxima lag by up to 2^8, raised but once or twice: a weight is
+ * off by up to 2^-25, fp16's least step, where the largest is 2^7 or more.
+ * Bound by VALU and MFMA, which one SIMD hardly overlaps: 57 % and 36 % of the
+ * cycles with heads of 64 (ten prompts, 320 TFLOP/s of the products asked for, 640
+ * issued), 36 % and 32 % with 128 over 20000 keys, five tiles a workgroup after
+ * 8 us of first loads. */
 template <int HD, bool KV4, int NW_>
 struct PaTile {
     static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 128 : 32;
@@ -400,7 +408,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
  * through the first-level cache and wait for nothing but their own loads: tiles
  * shared in LDS cost more in barriers and address work, of which all waves
  * then do the same at the same time, than their reads took.  Maxima lag by up
- * to 2^8: raised but once or twice. */
+ * to 2^8, as above.  Bound by first loads, then VALU: nine groups of 24 columns over
+ * up to 5000 keys of 4 bits and 250 own 42 us, 46 % VALU, 12 % MFMA. */
 template <int HD, bool KV4, int NW, int NCB>
 __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, int cw, int nsplit, int chunk, float* __restrict__ part,
                                         uint8_t* s_raw, float (*s_ml)[16][2])
@@ -715,16 +724,18 @@ struct PaCut {
 
 /* units of ntok rows each over `keys` keys by one kind of kernel.  Its time is counted in tiles: rounds of workgroups,
  * as many as fit the chip at once, each of a start worth some tiles and the tiles of its part; parts are written and
- * read once.  More of them fill the chip, until their starts and the join cost more: 192 columns over 20000 keys
- * in 14 parts 97 us, in 32 (all CUs) 70; 24 columns of nine groups over up to 5000 keys in 2 parts 55 us, 4 41,
- * 7 (taken) 45, 14 58; 50 blocks of columns over 2900 keys in 1 part 104 us, 2 104, 3 114, 5 133. */
+ * read once.  More of them fill the chip, until their starts and the join cost more: 192 columns over 20000 keys in 13
+ * parts 95 us, in 32 (all CUs) 63; 24 columns of nine groups over 4000 keys, 4 bits, in 1 part 76 us, 4 41, 6 44, 13 56;
+ * 2240 columns of two groups over 1500 keys in 1 part 89 us, 2 114, 6 151. */
 static PaCut pa_cut(int kind, int64_t units, int64_t ntok, int n_heads, int n_kv, int hd, int64_t keys, bool kv4, bool lone)
 {
     const int64_t cols = ntok * (n_heads / n_kv);
     PaCut p = {kind};
     int kt = kv4 && hd <= 128 ? 64 : 32;   /* (CaDec::KT) */
     p.cw = p.ncb = 1;
-    double slots = hd <= 128 ? 512.0 : 256.0, start = 3.0, join = 1.5e-6, tile_us = (0.3 + 0.0164 * hd) * (kv4 ? 0.8 : 1.0);
+    double slots = hd <= 128 ? 512.0 : 256.0, start = 3.0, join = 1.5e-6;
+    /* about: a tile's microseconds, starts and tiles of 4 bits (twice the keys) in those of fp16 */
+    double tile_us = 0.3 + 0.0164 * hd, start_of = kv4 ? 0.6 : 1.0, tile_of = kv4 ? 2.0 : 1.0;
     int64_t wide = PA_WAVES;   /* tiles that a workgroup has at a time */
     if (kind == PA_TILE) {
         const int64_t width = 16 * pa_waves(hd);
@@ -735,7 +746,8 @@ static PaCut pa_cut(int kind, int64_t units, int64_t ntok, int n_heads, int n_kv
         start = 1.5;
         join = 0.3e-6;
         /* (waves without columns leave the others more of their SIMD) */
-        tile_us = (1.0 + 0.0234 * hd) * (0.2 + 0.8 * (double)cols / (double)(p.ncb * width));
+        tile_us = (0.6 + 0.0234 * hd) * (0.5 + 0.5 * (double)cols / (double)(p.ncb * width));
+        start_of = tile_of = 1.0;
     } else if (kind == PA_COLS) {
         const int64_t nb = (cols + 31) / 32;
         for (p.cw = PA_WAVES; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
@@ -747,16 +759,16 @@ static PaCut pa_cut(int kind, int64_t units, int64_t ntok, int n_heads, int n_kv
     double best = 0.0;
     /* (those of both phases together: CA_PARTS at most) */
     for (int ns = 1; ns <= (lone ? CA_PARTS : CA_PARTS / 2) && (ns == 1 || tiles / ns >= 1.0); ns++) {
-        const double rounds = ceil((double)(wgs * ns) / slots);
-        const double cost = rounds * (start + tiles / ns) + (lone && ns > 1 ? 2.0 : 0.0) + (ns > 1 ? join * ns * (double)(units * ntok) * n_heads * hd : 0.0);
+        const double rounds = ceil((double)(wgs * ns) / slots), parts = ns > 1 ? join * ns * (double)(units * ntok) * n_heads * hd : 0.0;
+        const double cost = rounds * (start + tiles / ns) + (lone && ns > 1 ? 2.0 : 0.0) + parts;
         if (ns == 1 || cost < best) {
             best = cost;
             p.nsplit = ns;
+            p.us = tile_us * (rounds * (start * start_of + tiles / ns * tile_of) + parts);
         }
     }
     p.chunk = (int)((keys + (int64_t)kt * p.nsplit - 1) / ((int64_t)kt * p.nsplit));
     p.blocks = wgs * p.nsplit;
-    p.us = best * tile_us;
     return p;
 }
 
@@ -790,11 +802,12 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         if (hd <= 128 && cols > 64) p.b = cut(PA_TILE, false, top);
         if (hd > 128 || cols <= 64 || (hd <= 64 && p.b.blocks * p.b.chunk < 256)) p.b = cut(PA_COLS, false, top);
     }
-    /* Shared rows.  Tiles in LDS are a launch of their own unless the own rows have such too, which costs 13 us; the
-     * tiles' times are those with which the choice is the faster one most often (of 154 calls of both types 1 % from
-     * the best in the mean; always the one or the other 4 % and 15 %).  With single tokens' own rows, 32 heads of 128, 8 key
-     * heads: 192 columns over 700 keys 36 us against 26, over 5000 44 against 40, over 20000 61 against 80; 64 over 3000 28
-     * against 27, over 20000 37 against 44; twelve groups of 80 columns over 600 61 against 51. */
+    /* Shared rows: whichever takes less by the estimates.  Tiles in LDS are a launch of their own unless the own rows have
+     * such too, which counts as 25 us; with that and the tiles' times the choice is 1 % from the faster one in the mean of
+     * 222 calls of both types, always the one or the other 9 % and 12 %.  With single tokens' own rows, 32 heads of 128, 8
+     * key heads: 192 columns over 700 keys 36 us against 26, over 5000 44 against 40, over 20000 61 against 80; 64 over
+     * 3000 28 against 27, over 20000 37 against 44; twelve groups of 80 columns over 600 61 against 51.  Two groups of
+     * prompts, 2240 columns over 1500 keys, 4 bits, 90 against 165. */
     if (p.shared) {
         const int last = std::min(max_prefix - 1, max_pos);
         if (cols * group <= 16) p.a = cut(PA_DEC, true, last);
@@ -802,7 +815,7 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
             p.a = cut(PA_COLS, true, last);
             if (hd <= 128 && cols * group > 32) {
                 const PaCut t = cut(PA_TILE, true, last);
-                if (t.us + (p.b.kind == PA_TILE ? 0.0 : 13.0) < p.a.us) p.a = t;
+                if (t.us + (p.b.kind == PA_TILE ? 0.0 : 25.0) < p.a.us) p.a = t;
             }
         }
     }
