@@ -513,8 +513,8 @@ int lg_logprobs(const float* logits, int64_t stride, int rows, int vocab, const 
  * copies of them.  Conventions as above; no counterpart in the reference.
  *
  * A layer's caches in pages: page i < n_pages is "sequence" i of `pool`, whose
- * n_ctx is the rows of a page (a power of two, 16 .. 65536; seq_bytes below 2^32).  Row j of
- * sequence s is row j % n_ctx of page table[s * table_stride + j / n_ctx]
+ * n_ctx is the rows of a page (a power of two, 16 .. 65536; seq_bytes below
+ * 2^32).  Row j of sequence s is row j % n_ctx of page table[s * table_stride + j / n_ctx]
  * (device memory, read by the kernels); entries outside 0 .. n_pages - 1 are no
  * pages.  A table row has max_pages entries that may be read, max_pages * n_ctx
  * <= 2^30. */
@@ -542,8 +542,9 @@ int lg_qk_norm_rope_paged(const float* q, int64_t q_stride, float* q_out, int64_
  * sequence, once for all of them, the others from each sequence's own; values
  * outside 0 .. max_prefix count as the nearest.  NULL or max_prefix 0: nothing is
  * shared.  Keys without a page are not seen.  A row's head is zeros where no
- * key that it sees has a weight (none seen, or all at -infinity).  max_pos <
- * max_pages * n_ctx. */
+ * key that it sees has a weight (none seen, or all at -infinity).  An infinite
+ * key may also make it NaN where the query's value is below 2^-37 of its largest.
+ * max_pos < max_pages * n_ctx. */
 size_t lg_attn_paged_workspace_size(const lg_kv_pages* cache, int nseq, int ntok, int n_heads, int window, int sinks,
                                     int max_pos, int group, int max_prefix);
 int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages* cache, const int* pos, int nseq, int ntok,
@@ -554,11 +555,13 @@ int lg_attn_paged(const float* q, int64_t q_stride, const lg_kv_pages* cache, co
  * (rows as lg_logprobs takes them): candidate (b, t) has the score
  *   scores[b] + log softmax(row b)[t]
  * and the `top` highest, ties by the lower beam and then the lower token, go to
- * score, parent (the beam, 0 .. beams - 1) and token, [ngroups][top] each.  With done (may be NULL), a beam whose done is not 0 has the one
- * candidate (b, end) of score scores[b]; its logits are not read.  No
- * candidates: scores and sums that are no finite numbers (an idle beam has
- * -infinity), logits of -infinity.  Where there are fewer than top, the rest is
- * (-infinity, -1, -1).  Sums and scores are joined in double and rounded once.
+ * score, parent (the beam, 0 .. beams - 1) and token, [ngroups][top] each.  With
+ * done (may be NULL), a beam whose done is not 0 has the one candidate (b, end)
+ * of score scores[b]; its logits are not read.  No candidates: scores and sums
+ * that are no finite numbers (an idle beam has -infinity), logits of -infinity.
+ * Where there are fewer than top, the rest is (-infinity, -1, -1).  Sums and
+ * scores are joined in double and rounded once; scores that are the same in
+ * double count as equal (of one beam the higher logit goes first).
  * beams and top are 1 .. 64.  workspace as lg_attn_cache. */
 #define LG_BEAMS_MAX 64
 size_t lg_beam_select_workspace_size(int ngroups, int beams, int vocab, int top);

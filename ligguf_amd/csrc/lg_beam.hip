@@ -24,7 +24,9 @@ __device__ __forceinline__ bool bm_live(const BeamArgs& a, int64_t row)
 
 /* A part of a row: its maximum, the sum of e^(x - m) and its `top` highest
  * entries in order.  16 values of a thread at a time, the next ones on their way
- * (as k_logp). */
+ * (as k_logp).  Bound by the logits' bytes, read once: 320 rows of 151936, a fifth of
+ * them finished, 38 us, 4.1 TB/s (a copy's 4.9; 32 values at a time spill, 55; parts
+ * and 256 or 512 threads 44 to 50); of few rows by its chain: 4 of 32000 6.5 us. */
 template <int T>
 __global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
 {
@@ -123,7 +125,7 @@ constexpr int BM_VALS = 256;     /* candidates whose values lie side by side */
  * top-th highest of their own, and only entries that are no lower than it are
  * compared with each other: places by counting, first a hundred or so, then
  * hardly more than `top`.  Bound by its chain: loads, an exponential and a
- * logarithm in double, six barriers. */
+ * logarithm in double, six barriers: 5 to 8 us. */
 template <int T>
 __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
 {
@@ -258,13 +260,15 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
     }
 }
 
-/* Parts of a row: enough of them for the 256 CUs, of 4096 logits at least; and the
- * entries of a group's parts, which a workgroup holds as doubles, at most 4096
- * (more where one part a beam has them). */
+/* Parts of a row: enough of them for the 256 CUs, of 16384 logits at least (4 rows of
+ * 151936 whole 17.4 us, in parts of 4096 16.5, of 16384 12.4; 35 of 50257 13.8,
+ * 16.4, 12.6; 240 of 32000 13.9, 15.8, 13.7); and the entries of a group's parts,
+ * which a workgroup holds as doubles, at most 4096 (more where one part a beam
+ * has them). */
 static int bm_parts(int64_t rows, int beams, int vocab, int top)
 {
     const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(rows, 1));
-    return (int)std::max<int64_t>(1, std::min({want, (int64_t)vocab / 4096, (int64_t)BM_HELD / ((int64_t)beams * top),
+    return (int)std::max<int64_t>(1, std::min({want, (int64_t)vocab / 16384, (int64_t)BM_HELD / ((int64_t)beams * top),
                                                   (int64_t)BM_LISTS / beams}));
 }
 
@@ -299,7 +303,7 @@ extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* 
     const int64_t rows = (int64_t)ngroups * beams;
     BeamArgs a = {logits, scores, done, stride, end, beams, vocab, top, bm_parts(rows, beams, vocab, top), 0, nullptr, nullptr,
                   score, parent, token};
-    /* (parts begin 16 bytes apart, so that all are as aligned as the row; up to 512 of 4096 at least: none is empty) */
+    /* (parts begin 16 bytes apart, so that all are as aligned as the row; up to 512 of 16384 at least: none is empty) */
     a.part = (vocab / a.parts + 4) & ~3;
     if (!lg_grid_fits(rows * a.parts, 1024)) {
         lg_set_error("%s: %lld rows are too many for one call", who, (long long)rows);
@@ -331,7 +335,7 @@ struct ReorderArgs {
 
 constexpr int BM_ENTRIES = 64;   /* table entries of a group's beams that LDS holds at a time */
 
-/* A group: who takes which part-filled page, then the full pages' entries. */
+/* A group: who takes which part-filled page, then the full pages' entries.  Bound by its dependent loads, 2.5 to 5 us. */
 __global__ __launch_bounds__(256) void k_beam_tables(ReorderArgs a)
 {
     __shared__ int s_par[LG_BEAMS_MAX], s_page[LG_BEAMS_MAX], s_spare[LG_BEAMS_MAX], s_tab[LG_BEAMS_MAX][BM_ENTRIES];
@@ -392,7 +396,10 @@ struct CopyArgs {
 };
 
 /* rows of a page: [rows][n_kv][hd] fp16 are one run, 4-bit ones a run of codes and
- * one of pairs for each head */
+ * one of pairs for each head.  Bound by scattered runs of a few KB, read and written:
+ * 40 groups of 8 beams, 24 layers, 16 rows of 2 KB each on average, 335 MB in 88 us, 3.8
+ * TB/s (a copy's 4.9); runs of 32 KB at most a workgroup, twice the loads ahead or
+ * stores past the caches 95 to 99 us in all against 96. */
 __global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a)
 {
     const int4 j = a.jobs[blockIdx.x];

@@ -70,7 +70,7 @@ __device__ __forceinline__ void pa_split2(float x0, float x1, v8h& hi, v8h& lo, 
  * 8 us of first loads. */
 template <int HD, bool KV4, int NW_>
 struct PaTile {
-    static constexpr int NW = NW_, NTH = 64 * NW, KT = HD <= 128 ? 128 : 32;
+    static constexpr int NW = NW_, NTH = 64 * NW, KT = 128;
     static constexpr int NS = (HD + 31) / 32, NT = HD / 16;
     static constexpr int KST = HD + 16, VST = HD + 16;       /* halves per K and V row in LDS: 8 banks on, no conflicts (4 for K: 1 in 2) */
     static constexpr int PW = KV4 ? 16 : 8, PR = HD / PW;    /* values of a piece that a thread moves, pieces of a row */
@@ -405,9 +405,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
  * with each key's and value's fragment used for all of a wave's columns.  Of a
  * workgroup's NW waves `cw` have columns of their own and NW / cw share those,
  * each with tiles of KT keys of its own.  Waves with the same keys read them
- * through the first-level cache and wait for nothing but their own loads: tiles
- * shared in LDS cost more in barriers and address work, of which all waves
- * then do the same at the same time, than their reads took.  Maxima lag by up
+ * through the first-level cache and wait for nothing but their own loads: of few
+ * columns or keys tiles in LDS cost more in barriers and address work, of which
+ * all waves then do the same at the same time, than their reads took (both
+ * measured: pa_plan).  Maxima lag by up
  * to 2^8, as above.  Bound by first loads, then VALU: nine groups of 24 columns over
  * up to 5000 keys of 4 bits and 250 own 42 us, 46 % VALU, 12 % MFMA. */
 template <int HD, bool KV4, int NW, int NCB>

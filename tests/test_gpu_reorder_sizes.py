@@ -49,12 +49,13 @@ def test_large_pages(gpu, ctype, page, kv, hd, beams):
 
 
 @pytest.mark.parametrize("ng,nb,vocab,top", [(1, 1, 4095, 3), (1, 1, 4096, 3), (1, 2, 8191, 7), (1, 2, 8192, 7), (1, 3, 8193, 64), (1, 64, 8200, 64),
-                                             (1, 1, 151936, 64), (300, 2, 5000, 4), (1, 16, 65537, 32), (513, 1, 3000, 1)])
+                                             (1, 1, 151936, 64), (300, 2, 5000, 4), (1, 16, 65537, 32), (513, 1, 3000, 1), (1, 3, 32767, 5),
+                                             (1, 3, 32768, 5), (2, 3, 32769, 9), (1, 2, 49155, 64)])
 def test_vocabularies_at_borders_of_parts(gpu, ng, nb, vocab, top):
     g = np.random.default_rng(vocab)
     x = (g.standard_normal((ng, nb, vocab)) * 3).astype(np.float32)
     s = -np.sort(g.random((ng, nb)).astype(np.float32) * 9, axis=1)
     # the best ones at the ends of rows and of parts
-    for p in (0, vocab - 1, min(4095, vocab - 1), min(4096, vocab - 1), vocab // 2):
+    for p in (0, vocab - 1, min(4095, vocab - 1), min(4096, vocab - 1), min(16384, vocab - 1), vocab // 2, vocab // 3):
         x[:, :, p] = 12 + g.random((ng, nb)).astype(np.float32)
     check(gpu, x, s, top)
