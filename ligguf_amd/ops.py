@@ -235,7 +235,7 @@ class PagedLayers:
     def __init__(self, caches):
         c = caches[0] if caches else _refuse("no layers")
         for x in caches:
-            if (x.table.data_ptr() != c.table.data_ptr() or x.table.shape != c.table.shape or x.table.stride() != c.table.stride()
+            if (not isinstance(x, PagedKvCache) or x.table.data_ptr() != c.table.data_ptr() or x.table.shape != c.table.shape or x.table.stride() != c.table.stride()
                     or (x.type, x.page, x.n_pages, x.n_kv_heads, x.head_dim) != (c.type, c.page, c.n_pages, c.n_kv_heads, c.head_dim)):
                 _refuse("layers of one table and pages of one form wanted")
         self.caches, self.table, self.index, self.nseq = list(caches), c.table, c.index, c.nseq
@@ -285,7 +285,7 @@ def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None,
             _refuse(f"cache: values and {nseq} sequences on GPU {i} wanted")
         rv, desc = _rows(v, *at, kd, "v"), C.byref(cache.desc)
     lib = load()
-    fn = lib.lg_qk_norm_rope_paged if cache.__class__ is PagedKvCache else lib.lg_qk_norm_rope_tokens
+    fn = lib.lg_qk_norm_rope_paged if isinstance(cache, PagedKvCache) else lib.lg_qk_norm_rope_tokens
     _on(i, fn, *rq, *rqo, *rk, *rko, *rv, _vec(qw, head_dim, i, "qw"), _vec(kw, head_dim, i, "kw"),
         qd // head_dim, kd // head_dim, head_dim, rope_dim, 1 if half else 0, _vec(freq, rope_dim // 2, i, "freq"), mscale, eps, p,
         nseq, ntok, desc)
@@ -295,6 +295,8 @@ def qk_norm_rope_tokens(q, k, v, pos, freq, head_dim: int, rope_dim: int = None,
 def kv_values(cache: KvCache, pos0: int = 0, npos: int = None):
     """lg_kv4_read: the fp16 values [nseq, npos, kv_dim] that rows pos0 .. of a
     KV4 cache stand for, keys and values."""
+    if isinstance(cache, PagedKvCache):
+        _refuse("cache: a KvCache wanted (of pages: cache.pool)")
     npos = cache.n_ctx - pos0 if npos is None else npos
     if npos < 0:
         _refuse(f"{npos} rows")
@@ -323,8 +325,8 @@ def attention_cache(q, cache: KvCache, pos, window: int = 0, sinks: int = 0, max
     (n_ctx - 1 by default), sizes the launch."""
     p, i = _pos(pos), pos.get_device()
     nseq, ntok = pos.shape
-    if cache.index != i or cache.nseq != nseq:
-        _refuse(f"cache: {nseq} sequences on GPU {i} wanted")
+    if isinstance(cache, PagedKvCache) or cache.index != i or cache.nseq != nseq:
+        _refuse(f"cache: a KvCache of {nseq} sequences on GPU {i} wanted")
     max_pos = cache.n_ctx - 1 if max_pos is None else max_pos
     width, hd = q.shape[-1], cache.head_dim
     heads = width // hd
@@ -346,8 +348,8 @@ def attention_paged(q, cache: PagedKvCache, pos, window: int = 0, sinks: int = 0
     max_prefix, a bound of them (max_pos + 1 by default), sizes the launch."""
     p, i = _pos(pos), pos.get_device()
     nseq, ntok = pos.shape
-    if cache.index != i or cache.nseq != nseq:
-        _refuse(f"cache: {nseq} sequences on GPU {i} wanted")
+    if not isinstance(cache, PagedKvCache) or cache.index != i or cache.nseq != nseq:
+        _refuse(f"cache: a PagedKvCache of {nseq} sequences on GPU {i} wanted")
     max_pos = cache.n_ctx - 1 if max_pos is None else max_pos
     group, pp = 1, None
     if prefix is None:

@@ -249,3 +249,24 @@ def test_one_key_head_in_as_many_parts_as_there_are(gpu, ctype, heads):
     """A single key head over long contexts: shared and own rows each in hundreds of parts."""
     check(gpu, ctype, heads, 1, 64, 64, 1, 2, [50000], [90000, 70001], 1)
     check(gpu, ctype, heads, 1, 64, 64, 1, 1, [0], [100000], 1)
+
+
+def test_the_other_kind_of_cache_is_refused(gpu):
+    """Before anything is launched: a table has other sequences than its pool has pages."""
+    import torch
+    from ligguf_amd import ops
+    paged = ops.PagedKvCache.empty(ops.KV4, 3, 16, 2, 64, torch.zeros((8, 2), dtype=torch.int32, device=gpu))
+    flat = ops.KvCache.empty(ops.KV4, 32, 2, 64, 8, gpu)
+    q, pos = torch.zeros(8, 1, 256, device=gpu), torch.zeros(8, 1, dtype=torch.int32, device=gpu)
+    for bad in (lambda: ops.attention_cache(q, paged, pos, max_pos=8), lambda: ops.attention_paged(q, flat, pos), lambda: ops.kv_values(paged),
+                lambda: ops.PagedLayers([flat])):
+        with pytest.raises(L.LgError):
+            bad()
+
+    class Mine(ops.PagedKvCache):
+        pass
+
+    mine = Mine(paged.k, paged.v, paged.table, 2, 64, ops.KV4, 16)
+    pos[1:] = -1          # (one row, or all would write to one place)
+    r, _ = ops.qk_norm_rope_tokens(q, q[:, :, :128], q[:, :, 128:], pos, torch.ones(32, device=gpu), 64, cache=mine)
+    assert ops.attention_paged(r, mine, pos).isfinite().all() and ops.kv_values(paged.pool)[0].shape == (3, 16, 128)
