@@ -163,7 +163,7 @@ struct CaMaxOf {
     float sc, m, cc;
     bool any_far;                         /* of the wave */
 
-    __device__ __forceinline__ explicit CaMaxOf(float scale) : sc(scale), m(-0x1p40f), any_far(true)   /* (-2^40: below any score) */
+    __device__ __forceinline__ explicit CaMaxOf(float scale = 0.0f) : sc(scale), m(-0x1p40f), any_far(true)   /* (-2^40: below any score) */
     {
         const float c = __builtin_fmaf(-m, sc, BASE);
         cc = far(c) ? BASE : c;

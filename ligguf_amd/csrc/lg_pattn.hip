@@ -19,6 +19,7 @@ struct PaArgs {
 };
 
 constexpr int PA_WAVES = 4;                                      /* of the other kernels' */
+constexpr int pa_blocks(int hd) { return hd <= 128 ? 2 : 1; }    /* of 16 columns, of pa_cols' waves */
 constexpr int pa_waves(int hd) { return hd <= 64 ? 16 : 12; }   /* of k_pattn_tile's workgroups */
 
 /* ca_query2 in 11 operations for two values, not 19: lo is 0 only where hi is, which
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
         int none = id.none(a, KT / 16);   /* rows 16 j .. of the present tile have no page: bit j */
         v8h qh[NS], ql[NS];
         float big = 0.0f;
-        CaMaxOf<7, 8> mx(0.0f);
+        CaMaxOf<7, 8> mx;
         if (wmax >= 0) {   /* (a wave without rows has but the tiles to move) */
 #pragma unroll
         for (int j = 0; j < 2 * NS; j++)
@@ -402,7 +403,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
 /* More than 16 columns (query heads of a key head, tokens in order): 16 NCB a wave,
  * the products of k_cattn_dec,
  *   S^T[key][col] = K Q^T      O^T[d][col] += V^T P^T
- * with each key's and value's fragment used for all of a wave's columns.  Of a
+ * with each key's and value's fragment used for all of a wave's columns, 32 of them
+ * or, with heads of 256, 16, which need no more registers than there are (48 sequences
+ * behind 5000 rows, 16 heads 72 -> 64 us, a prompt of 300 tokens 74 -> 46).  Of a
  * workgroup's NW waves `cw` have columns of their own and NW / cw share those,
  * each with tiles of KT keys of its own.  Waves with the same keys read them
  * through the first-level cache and wait for nothing but their own loads: of few
@@ -515,7 +518,9 @@ __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, i
                 for (int e = 0; e < 8; e += 2)
                     pa_query2(x[n][2 * j + e / 4][e % 4], x[n][2 * j + e / 4][e % 4 + 1], ex[n], qh[n][j], ql[n][j], e);
         }
-        CaMaxOf<7, 8> mx[NCB] = {CaMaxOf<7, 8>(ca_scale(a.scale2, ex[0])), CaMaxOf<7, 8>(ca_scale(a.scale2, ex[NCB - 1]))};
+        CaMaxOf<7, 8> mx[NCB];
+#pragma unroll
+        for (int n = 0; n < NCB; n++) mx[n] = CaMaxOf<7, 8>(ca_scale(a.scale2, ex[n]));
         for (; it < t1; it += nkg) {
             v4f s[NU][NCB];
 #pragma unroll
@@ -690,7 +695,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols(PaA
     __shared__ __attribute__((aligned(16))) uint8_t s_raw[NW * CaDec<HD, KV4>::WAVE];
     __shared__ float s_ml[NW][16][2];
     const PaPhase& f = args.of(blockIdx.x);
-    pa_cols<HD, KV4, NW, 2>(f.a, args.in(blockIdx.x), f.ncb, f.cw, f.nsplit, f.chunk, args.part, s_raw, s_ml);
+    pa_cols<HD, KV4, NW, pa_blocks(HD)>(f.a, args.in(blockIdx.x), f.ncb, f.cw, f.nsplit, f.chunk, args.part, s_raw, s_ml);
 }
 
 template <int HD, bool KV4, int NW>
@@ -710,7 +715,7 @@ __global__ __launch_bounds__(64 * NW, (HD <= 128 ? 2 : 1)) void k_pattn_cols_dec
     __shared__ float s_ml[NW][16][2];
     const PaPhase& f = args.of(blockIdx.x);
     if ((int)blockIdx.x < args.na)
-        pa_cols<HD, KV4, NW, 2>(f.a, blockIdx.x, f.ncb, f.cw, f.nsplit, f.chunk, args.part, s_raw, s_ml);
+        pa_cols<HD, KV4, NW, pa_blocks(HD)>(f.a, blockIdx.x, f.ncb, f.cw, f.nsplit, f.chunk, args.part, s_raw, s_ml);
     else ca_dec<HD, KV4, NW>(f.a, blockIdx.x - args.na, f.nsplit, f.chunk, args.part, s_raw, s_ml);
 }
 
@@ -750,7 +755,7 @@ static PaCut pa_cut(int kind, int64_t units, int64_t ntok, int n_heads, int n_kv
         tile_us = (0.6 + 0.0234 * hd) * (0.5 + 0.5 * (double)cols / (double)(p.ncb * width));
         start_of = tile_of = 1.0;
     } else if (kind == PA_COLS) {
-        const int64_t nb = (cols + 31) / 32;
+        const int64_t nb = (cols + 16 * pa_blocks(hd) - 1) / (16 * pa_blocks(hd));
         for (p.cw = PA_WAVES; p.cw > 1 && (nb + p.cw - 1) / p.cw * p.cw * 8 > nb * 9; p.cw /= 2) {}
         p.ncb = (int)((nb + p.cw - 1) / p.cw);
         wide = PA_WAVES / p.cw;
