@@ -278,7 +278,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
 #pragma unroll
             for (int e = 0; e < 8; e += 2) pa_query2(x[2 * j + e / 4][e % 4], x[2 * j + e / 4][e % 4 + 1], ex, qh[j], ql[j], e);
         }
-        P.store(s_kv, some(kb, none) ? s_bad[0] : nullptr);
+        bool dropped = some(kb, none);   /* the present tile's infinities and NaN are zeros, their keys in s_bad */
+        P.store(s_kv, dropped ? s_bad[0] : nullptr);
         __syncthreads();
         for (int it = t0; it < t1; it++) {
             const bool more = it + 1 < t1;
@@ -359,9 +360,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
                         o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, o[t], 0, 0, 0);
                     }
                 }
-                /* infinities and NaN of keys that only some rows see: added by
-                 * itself to those that do, whatever the (positive) weight */
-                if (part_seen)
+                /* infinities and NaN of keys that only some rows of the workgroup see:
+                 * added by itself to those that do, whatever the (positive) weight,
+                 * in waves that see all of the tile too */
+                if (dropped)
                     for (int w = 0; w < KT / 32; w++)
                         for (uint32_t keys = __builtin_amdgcn_readfirstlane(s_bad[slot][w]); keys; keys &= keys - 1) {
                             const int key = kb + 32 * w + __builtin_ctz(keys);
@@ -374,7 +376,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
                                 }
                         }
             }
-            if (more) P.store(s_kv + (cur ^ 1) * C::STAGE, some(kn, none1) ? s_bad[(slot + 1) % 3] : nullptr);
+            dropped = some(kn, none1);
+            if (more) P.store(s_kv + (cur ^ 1) * C::STAGE, dropped ? s_bad[(slot + 1) % 3] : nullptr);
             none = none1;
             kb = kn;
             kn = k2;
