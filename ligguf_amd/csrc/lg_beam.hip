@@ -116,7 +116,7 @@ __global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
     lp_emit<T>(s, c, top, [&](int rank, uint64_t k) { a.keys[at * a.top + rank] = k - (uint32_t)first; });   /* (~id - first = ~(id + first)) */
 }
 
-constexpr int BM_HELD = 4096;    /* entries of a group's parts that its workgroup holds as doubles */
+constexpr int BM_HELD = 4096;    /* entries of a group's parts that its workgroup holds, as doubles and keys */
 constexpr int BM_LISTS = 1024;   /* and parts */
 constexpr int BM_VALS = 256;     /* candidates whose values lie side by side */
 
@@ -129,9 +129,8 @@ constexpr int BM_VALS = 256;     /* candidates whose values lie side by side */
 template <int T>
 __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
 {
-    extern __shared__ double s_score[];   /* [beams][parts][top] */
+    extern __shared__ double s_score[];   /* [beams][parts][top] and, behind, their keys */
     __shared__ double s_off[LG_BEAMS_MAX], s_lse[LG_BEAMS_MAX], s_val[BM_VALS], s_least;
-    __shared__ uint32_t s_id[BM_HELD];    /* the complements of the entries' tokens */
     union Lists {
         float2 mz[BM_LISTS];
         double z[BM_LISTS];
@@ -141,6 +140,7 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
     __shared__ int s_kind[LG_BEAMS_MAX], s_n;   /* 0: no candidates, 1: logits, 2: finished */
     const int64_t row0 = (int64_t)blockIdx.x * a.beams, key0 = row0 * a.parts * a.top;
     const int t = threadIdx.x, lists = a.beams * a.parts, n = lists * a.top, run = a.parts * a.top;
+    uint64_t* const s_key = (uint64_t*)(s_score + n);
     if (t < a.beams) {
         const float sc = a.scores[row0 + t];
         s_kind[t] = !(fabsf(sc) <= FLT_MAX) ? 0 : a.done && a.done[row0 + t] ? 2 : 1;
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
     for (int i = t; i < n; i += T) {
         const uint64_t k = a.keys[key0 + i];
         s_score[i] = (double)lp_value(k);
-        s_id[i] = (uint32_t)k;
+        s_key[i] = k;
     }
     if (t == 0) {
         s_n = 0;
@@ -191,12 +191,12 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
         if (s_kind[b] == 1 && at < held) v = s_off[b] + (s_score[i] - s_lse[b]);
         if (s_kind[b] == 2 && in == 0) {
             v = s_off[b];
-            s_id[i] = ~(uint32_t)a.end;
+            s_key[i] = ~(uint32_t)a.end;
         }
         s_score[i] = v;
     }
-    /* place of entry i, value v, among the c entries of s.list: those that are higher, or equal and ahead in the order of
-     * beams, parts and entries.  Eight values at a time, no branches (16 entries of 8 beams: 12 us with them), whatever
+    /* place of entry i, value v, among the c entries of s.list: those that are higher, or equal and of a lower beam or,
+     * of the same one, of a higher key (logit, then token), whatever parts they come from.  Eight values at a time, no branches (16 entries of 8 beams: 12 us with them), whatever
      * lies behind the c-th being -infinity; equal values are rare and looked at again. */
     auto place = [&](int c, int i, double v) __attribute__((always_inline)) {
         int rank = 0, same = 0;
@@ -213,8 +213,17 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
             rank += w > v ? 1 : 0;
             same += w == v ? 1 : 0;
         }
-        if (same > 1)
-            for (int o = 0; o < c; o++) rank += s.list[o] < i && s_score[s.list[o]] == v ? 1 : 0;
+        if (same > 1) {
+            const int first = i / run * run;   /* the beam's entries */
+            const uint64_t key = s_key[i];
+#pragma unroll 4
+            for (int o = 0; o < c; o++) {
+                const int j = s.list[o];
+                const double w = s_score[j];
+                const uint64_t k = s_key[j];
+                rank += (w == v) & ((j < first) | ((j < first + run) & (k > key))) ? 1 : 0;
+            }
+        }
         return rank;
     };
     auto gather = [&](int c) {
@@ -249,7 +258,7 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
             const int64_t at = (int64_t)blockIdx.x * a.top + rank;
             a.score[at] = (float)v;
             a.parent[at] = i / run;
-            a.token[at] = (int)~s_id[i];
+            a.token[at] = (int)~(uint32_t)s_key[i];
         }
     }
     if (t >= cand && t < a.top) {
@@ -263,7 +272,7 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
 /* Parts of a row: enough of them for the 256 CUs, of 16384 logits at least (4 rows of
  * 151936 whole 17.4 us, in parts of 4096 16.5, of 16384 12.4; 35 of 50257 13.8,
  * 16.4, 12.6; 240 of 32000 13.9, 15.8, 13.7); and the entries of a group's parts,
- * which a workgroup holds as doubles, at most 4096 (more where one part a beam
+ * which a workgroup holds with their keys, at most 4096 (more where one part a beam
  * has them). */
 static int bm_parts(int64_t rows, int beams, int vocab, int top)
 {
@@ -319,7 +328,7 @@ extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* 
     hipStream_t s = (hipStream_t)stream;
     const int lists = beams * a.parts * top;
     k_beam_rows<1024><<<(unsigned)(rows * a.parts), 1024, 0, s>>>(a);
-    k_beam_group<256><<<ngroups, 256, lists * sizeof(double), s>>>(a);
+    k_beam_group<256><<<ngroups, 256, lists * (sizeof(double) + sizeof(uint64_t)), s>>>(a);
     return lg_check_launch(who);
 }
 
