@@ -513,8 +513,8 @@ int lg_logprobs(const float* logits, int64_t stride, int rows, int vocab, const 
  * copies of them.  Conventions as above; no counterpart in the reference.
  *
  * A layer's caches in pages: page i < n_pages is "sequence" i of `pool`, whose
- * n_ctx is the rows of a page (a power of two, 16 .. 65536; seq_bytes below
- * 2^32).  Row j of sequence s is row j % n_ctx of page table[s * table_stride + j / n_ctx]
+ * n_ctx is the rows of a page (a power of two, 16 .. 65536; its bytes and
+ * seq_bytes below 2^32).  Row j of sequence s is row j % n_ctx of page table[s * table_stride + j / n_ctx]
  * (device memory, read by the kernels); entries outside 0 .. n_pages - 1 are no
  * pages.  A table row has max_pages entries that may be read, max_pages * n_ctx
  * <= 2^30. */

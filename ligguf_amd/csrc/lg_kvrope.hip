@@ -45,8 +45,10 @@ int lg_kv_pages_arg(const lg_kv_pages* c, const char* who, LgKv* out, int* shift
     const int rc = lg_kv_arg(&c->pool, c->n_pages, who, out);
     if (rc) return rc;
     const int n = c->pool.n_ctx;
-    if (n < 16 || n > 65536 || (n & (n - 1)) || c->pool.seq_bytes > UINT32_MAX) {
-        lg_set_error("%s: pages of %d rows, %zu bytes (a power of two from 16 to 65536, bytes below 2^32)", who, n, c->pool.seq_bytes);
+    /* (the rows' own bytes too: of one page seq_bytes says nothing, and rows are found in a page by 32 bits) */
+    const size_t bytes = std::max(c->pool.seq_bytes, (size_t)lg_kv_bytes(out->type, n, out->n_kv, out->hd));
+    if (n < 16 || n > 65536 || (n & (n - 1)) || bytes > UINT32_MAX) {
+        lg_set_error("%s: pages of %d rows, %zu bytes (a power of two from 16 to 65536, bytes below 2^32)", who, n, bytes);
         return LG_ERR_ARG;
     }
     if (c->n_pages <= 0 || c->max_pages <= 0 || c->max_pages > (1 << 30) / n) {
