@@ -196,8 +196,9 @@ __global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
         s_score[i] = v;
     }
     /* place of entry i, value v, among the c entries of s.list: those that are higher, or equal and of a lower beam or,
-     * of the same one, of a higher key (logit, then token), whatever parts they come from.  Eight values at a time, no branches (16 entries of 8 beams: 12 us with them), whatever
-     * lies behind the c-th being -infinity; equal values are rare and looked at again. */
+     * of the same one, of a higher key (logit, then token), whatever parts they come from.  Eight values at a time, no
+     * branches (16 entries of 8 beams: 12 us with them), whatever lies behind the c-th being -infinity; equal values are
+     * rare and looked at again. */
     auto place = [&](int c, int i, double v) __attribute__((always_inline)) {
         int rank = 0, same = 0;
         const int fast = min(c, BM_VALS);
