@@ -136,14 +136,15 @@ def test_python_handles_refuse_tensors_elsewhere():
 
 @pytest.mark.parametrize("kw", [
     dict(page=65536, kv=512, hd=128), dict(page=65536, kv=128, hd=256), dict(page=32768, kv=1 << 10, hd=64),
-    dict(page=65536, kv=1024, hd=128, type=L.KV4),
+    dict(page=65536, kv=1024, hd=128, type=L.KV4), dict(page=65536, kv=2048, hd=64, type=L.KV4),
 ])
 def test_a_single_page_past_32_bits_is_refused(kw):
     """Rows are found in their page by 32 bits; seq_bytes, which says nothing of a pool of one page, does not hide its size."""
     for seq in (0, 16, None):
         c = pages(n=1, **kw, **({} if seq is None else dict(seq=seq)))
-        assert attn(c=c, heads=kw["kv"], nseq=0) == -1 and b"pages" in L.load().lg_last_error(None)
-        assert append(c=c, kv=kw["kv"], hd=kw["hd"], nseq=0) == -1
-        assert reorder(c=c.pool, n_pages=1, groups=0) == -1
+        assert attn(c=c, heads=kw["kv"], nseq=0) == -1 and b"bytes below" in L.load().lg_last_error(None)
+        if kw["hd"] == 64:
+            assert append(c=c, kv=kw["kv"], ks=kw["kv"] * 64, vs=kw["kv"] * 64) == -1 and b"bytes below" in L.load().lg_last_error(None)
+        assert reorder(c=c.pool, n_pages=1, groups=0) == -1 and b"bytes below" in L.load().lg_last_error(None)
     # the largest page that fits is none of these
     assert attn(c=pages(page=65536, kv=255, hd=128, n=1, seq=0), heads=255, nseq=0) == 0
