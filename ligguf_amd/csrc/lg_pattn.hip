@@ -409,7 +409,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
  * with each key's and value's fragment used for all of a wave's columns, 32 of them
  * or, with heads of 256, 16, which need no more registers than there are (48 sequences
  * behind 5000 rows, 16 heads 72 -> 64 us, a prompt of 300 tokens 74 -> 46).  Of a
- * workgroup's NW waves `cw` have columns of their own and NW / cw share those,
+ * workgroup's NW waves `cw`, which divides them, have columns of their own and NW / cw share those,
  * each with tiles of KT keys of its own.  Waves with the same keys read them
  * through the first-level cache and wait for nothing but their own loads: of few
  * columns or keys tiles in LDS cost more in barriers and address work, of which
@@ -437,7 +437,7 @@ __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, i
     CaRows<HD, KV4> K, V;
     const int* const trow = a.table + (int64_t)unit * a.tstep * a.tstride;
     int ahead = -1;
-    if (a.window <= 0 && kg < nkg) {
+    if (a.window <= 0) {
         ahead = (klo / KT + sp * chunk + kg) * KT;
         if (ahead > a.max_pos) ahead = -1;
     }
@@ -493,7 +493,6 @@ __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, i
     const CaTiles tiles(a, pmin, pmax, KT, klo, khi);
     int t0, t1;
     tiles.chunk(sp, nsplit, chunk, &t0, &t1);
-    if (kg >= nkg) t1 = t0;   /* (a wave too many) */
     if (t0 + kg < t1) {       /* (the wave's) */
         _Float16* const sV = (_Float16*)(s_raw + wave * C::WAVE);
         int it = t0 + kg, kb = tiles.at(it) * KT;
@@ -654,8 +653,7 @@ __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, i
             *(v4f*)(a.out + row * a.os + (size_t)head * HD + d) = pk < 0 || pk > a.max_pos || L == 0.0f ? (v4f){} : y * (1.0f / L);
         }
     };
-    if (nkg == 1) {
-        if (kg) return;
+    if (nkg == 1) {   /* (kg is 0) */
 #pragma unroll
         for (int n = 0; n < NCB; n++)
 #pragma unroll
@@ -677,9 +675,9 @@ __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, i
         for (int i = threadIdx.x; i < cw * 16 * (HD / 4); i += 64 * NW) {
             const int w0 = i / (16 * (HD / 4)), k = i / (HD / 4) % 16, d = i % (HD / 4) * 4;
             float M = -INFINITY, L = 0.0f;
-            for (int w = w0; w < cw * nkg; w += cw) M = fmaxf(M, s_ml[w][k][0]);
+            for (int w = w0; w < NW; w += cw) M = fmaxf(M, s_ml[w][k][0]);
             v4f y = {};
-            for (int w = w0; w < cw * nkg; w += cw) {
+            for (int w = w0; w < NW; w += cw) {
                 /* (a wave without keys has l = 0 and all zeros) */
                 const float lw = s_ml[w][k][1], f = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][k][0] - M);
                 const v4f v = *(const v4f*)((const float*)(s_raw + w * C::WAVE) + k * C::OST + d);
