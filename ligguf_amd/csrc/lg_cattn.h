@@ -171,8 +171,8 @@ struct CaMaxOf {
     __device__ __forceinline__ bool far(float c) const { return fabsf(c) > 0x1p22f; }
     __device__ __forceinline__ bool due(float mn) const
     {
-        if constexpr (LAG > 0) return __builtin_amdgcn_ballot_w64((mn - m) * sc > (float)LAG) || any_far;
-        else return __builtin_amdgcn_ballot_w64(mn > m) || any_far;
+        static_assert(LAG == 0, "a maximum that lags goes by over()");
+        return __builtin_amdgcn_ballot_w64(mn > m) || any_far;
     }
     /* whether some weights (sum: a lane's, which no one of them exceeds) are too far above the maximum */
     __device__ __forceinline__ bool over(float sum) const
