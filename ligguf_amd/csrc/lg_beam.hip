@@ -27,9 +27,10 @@ __device__ __forceinline__ bool bm_live(const BeamArgs& a, int64_t row)
  * (as k_logp).  Bound by the logits' bytes, read once: 320 rows of 151936, a fifth of
  * them finished, 38 us, 4.1 TB/s (a copy's 4.9; 32 values at a time spill, 55; parts
  * and 256 or 512 threads 44 to 50); of few rows by its chain: 4 of 32000 6.5 us. */
-template <int T>
-__global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
+constexpr int BM_ROW_THREADS = 1024;
+__global__ __launch_bounds__(BM_ROW_THREADS) void k_beam_rows(BeamArgs a)
 {
+    constexpr int T = BM_ROW_THREADS;
     __shared__ LpShared s;
     const int64_t row = blockIdx.x / a.parts;
     const int part = blockIdx.x % a.parts, t = threadIdx.x;
@@ -89,11 +90,10 @@ __global__ __launch_bounds__(T) void k_beam_rows(BeamArgs a)
         v[1] = v[2] = v[3] = none;
         take(v);
     }
-    {   /* of T / 256 neighbours */
-        uint32_t o = ord;
-        if constexpr (T >= 512) o = max(o, (uint32_t)lg_partner<0>((int)o));
-        if constexpr (T >= 1024) o = max(o, (uint32_t)lg_partner<1>((int)o));
-        if (t % (T / 256) == 0) s.top[t / (T / 256)] = o;
+    {   /* of T / 256 = 4 neighbours */
+        uint32_t o = max(ord, (uint32_t)lg_partner<0>((int)ord));
+        o = max(o, (uint32_t)lg_partner<1>((int)o));
+        if (t % 4 == 0) s.top[t / 4] = o;
     }
     auto join = [&]() {   /* m, z over the wave */
         const float M = lg_group_max<64>(m);
@@ -126,9 +126,10 @@ constexpr int BM_VALS = 256;     /* candidates whose values lie side by side */
  * compared with each other: places by counting, first a hundred or so, then
  * hardly more than `top`.  Bound by its chain: loads, an exponential and a
  * logarithm in double, six barriers: 5 to 8 us. */
-template <int T>
-__global__ __launch_bounds__(T) void k_beam_group(BeamArgs a)
+constexpr int BM_GROUP_THREADS = 256;
+__global__ __launch_bounds__(BM_GROUP_THREADS) void k_beam_group(BeamArgs a)
 {
+    constexpr int T = BM_GROUP_THREADS;
     extern __shared__ double s_score[];   /* [beams][parts][top] and, behind, their keys */
     __shared__ double s_off[LG_BEAMS_MAX], s_lse[LG_BEAMS_MAX], s_val[BM_VALS], s_least;
     union Lists {
@@ -315,7 +316,7 @@ extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* 
                   score, parent, token};
     /* (parts begin 16 bytes apart, so that all are as aligned as the row; up to 512 of 16384 at least: none is empty) */
     a.part = (vocab / a.parts + 4) & ~3;
-    if (!lg_grid_fits(rows * a.parts, 1024)) {
+    if (!lg_grid_fits(rows * a.parts, BM_ROW_THREADS)) {
         lg_set_error("%s: %lld rows are too many for one call", who, (long long)rows);
         return LG_ERR_ARG;
     }
@@ -328,8 +329,8 @@ extern "C" int lg_beam_select(const float* logits, int64_t stride, const float* 
     a.keys = (uint64_t*)(a.mz + rows * a.parts);
     hipStream_t s = (hipStream_t)stream;
     const int lists = beams * a.parts * top;
-    k_beam_rows<1024><<<(unsigned)(rows * a.parts), 1024, 0, s>>>(a);
-    k_beam_group<256><<<ngroups, 256, lists * (sizeof(double) + sizeof(uint64_t)), s>>>(a);
+    k_beam_rows<<<(unsigned)(rows * a.parts), BM_ROW_THREADS, 0, s>>>(a);
+    k_beam_group<<<ngroups, BM_GROUP_THREADS, lists * (sizeof(double) + sizeof(uint64_t)), s>>>(a);
     return lg_check_launch(who);
 }
 
