@@ -541,7 +541,9 @@ int lg_qk_norm_rope_paged(const float* q, int64_t q_stride, float* q_out, int64_
  * their first rows: rows j < prefix[g] are read from the pages of its first
  * sequence, once for all of them, the others from each sequence's own; values
  * outside 0 .. max_prefix count as the nearest.  NULL or max_prefix 0: nothing is
- * shared.  Keys without a page are not seen.  A row's head is zeros where no
+ * shared.  max_pos and max_prefix also size the launch: own rows are cut for
+ * max_pos - max_prefix + 1 of them, and more take fewer workgroups than they
+ * need.  Keys without a page are not seen.  A row's head is zeros where no
  * key that it sees has a weight (none seen, or all at -infinity).  An infinite
  * key may also make it NaN where the query's value is below 2^-37 of its largest.
  * max_pos < max_pages * n_ctx. */

@@ -410,7 +410,9 @@ struct CopyArgs {
  * one of pairs for each head.  Bound by scattered runs of a few KB, read and written:
  * 40 groups of 8 beams, 24 layers, 16 rows of 2 KB each on average, 335 MB in 88 us, 3.8
  * TB/s (a copy's 4.9); runs of 32 KB at most a workgroup, twice the loads ahead or
- * stores past the caches 95 to 99 us in all against 96. */
+ * stores past the caches 95 to 99 us in all against 96.  Of 4 bits by the heads' short
+ * runs one after the other, a fraction of the threads each: the same rows, 119 MB,
+ * 46 us, 2.6 TB/s. */
 __global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a)
 {
     const int4 j = a.jobs[blockIdx.x];

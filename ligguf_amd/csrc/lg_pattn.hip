@@ -65,10 +65,10 @@ __device__ __forceinline__ void pa_split2(float x0, float x1, v8h& hi, v8h& lo, 
  * computes (two LDS stages, one barrier a tile), its table entries while the one
  * before does.  Maxima lag by up to 2^8, raised but once or twice: a weight is
  * off by up to 2^-25, fp16's least step, where the largest is 2^7 or more.
- * Bound by VALU and MFMA, which one SIMD hardly overlaps: 57 % and 36 % of the
+ * Bound by VALU and MFMA, which one SIMD hardly overlaps: 55 % and 38 % of the
  * cycles with heads of 64 (ten prompts, 320 TFLOP/s of the products asked for, 640
- * issued), 36 % and 32 % with 128 over 20000 keys, five tiles a workgroup after
- * 8 us of first loads. */
+ * issued; 4 bits 110 us, 58 % and 36 %), 35 % and 33 % with 128 over 20000 keys, five
+ * tiles a workgroup after 8 us of first loads. */
 template <int HD, bool KV4, int NW_>
 struct PaTile {
     static constexpr int NW = NW_, NTH = 64 * NW, KT = 128;
@@ -409,14 +409,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_pattn_tile(PaArgs args)
  * with each key's and value's fragment used for all of a wave's columns, 32 of them
  * or, with heads of 256, 16, which need no more registers than there are (48 sequences
  * behind 5000 rows, 16 heads 72 -> 64 us, a prompt of 300 tokens 74 -> 46).  Of a
- * workgroup's NW waves `cw`, which divides them, have columns of their own and NW / cw share those,
- * each with tiles of KT keys of its own.  Waves with the same keys read them
- * through the first-level cache and wait for nothing but their own loads: of few
- * columns or keys tiles in LDS cost more in barriers and address work, of which
- * all waves then do the same at the same time, than their reads took (both
- * measured: pa_plan).  Maxima lag by up
- * to 2^8, as above.  Bound by first loads, then VALU: nine groups of 24 columns over
- * up to 5000 keys of 4 bits and 250 own 42 us, 46 % VALU, 12 % MFMA. */
+ * workgroup's NW waves `cw` (1, 2 or all) have columns of their own and NW / cw
+ * share those, each with tiles of KT keys of its own.  Waves with the same keys
+ * read them through the first-level cache and wait for nothing but their own
+ * loads: of few columns or keys tiles in LDS cost more in barriers and address
+ * work, of which all waves then do the same at the same time, than their reads
+ * took (both measured: pa_plan).  Maxima lag by up to 2^8, as above.  Bound by
+ * first loads, then VALU: nine groups of 24 columns over up to 5000 keys of 4 bits
+ * and 250 own 42 us, 47 % VALU, 12 % MFMA. */
 template <int HD, bool KV4, int NW, int NCB>
 __device__ __forceinline__ void pa_cols(const CAttnPaged& a, int blk, int ncb, int cw, int nsplit, int chunk, float* __restrict__ part,
                                         uint8_t* s_raw, float (*s_ml)[16][2])
@@ -800,7 +800,8 @@ static PaPlan pa_plan(int64_t nseq, int64_t ntok, int n_heads, int n_kv, int hd,
         return pa_cut(kind, shared ? nseq / group : nseq, n, n_heads, n_kv, hd, keys, kv4, !p.shared);
     };
     const int64_t rep = n_heads / n_kv, cols = ntok * rep;
-    /* Own rows (their number lies in device memory: of the longest prompt's).  Of many columns tiles in LDS: 2000 tokens
+    /* Own rows (their number lies in device memory: taken to be what max_pos leaves beyond max_prefix; four sequences of
+     * 3000 behind 2000 shared rows 23 us, with max_prefix 5000, for one own row, 54).  Of many columns tiles in LDS: 2000 tokens
      * of 32 heads of 128 92 us against 179, 64 18 against 20.  Not where heads of 64 fill the chip with less than a tile
      * a workgroup: 64 tokens 15 against 13, 256 22 against 18, 512 27 and 26, 1024 39 against 47. */
     const int top = p.shared ? std::max(max_pos - max_prefix, 0) : max_pos;

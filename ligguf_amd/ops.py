@@ -345,7 +345,9 @@ def attention_paged(q, cache: PagedKvCache, pos, window: int = 0, sinks: int = 0
     """lg_attn_paged: attention_cache over pages.  prefix, int32 [groups] on the GPU
     (nseq is a multiple of groups): the sequences of a group share so many first
     rows, which lie in the pages of its first one and are read once for all;
-    max_prefix, a bound of them (max_pos + 1 by default), sizes the launch."""
+    max_prefix, a bound of them (max_pos + 1 by default), sizes the launch with max_pos: the own rows are cut for
+    max_pos - max_prefix + 1, by default for one, so that many of them run in a single part.  Pass it where it is known
+    (four sequences, 2000 shared and 3000 own rows: 23 us with it, 54 without)."""
     p, i = _pos(pos), pos.get_device()
     nseq, ntok = pos.shape
     if not isinstance(cache, PagedKvCache) or cache.index != i or cache.nseq != nseq:
